@@ -25,7 +25,7 @@ OUT = os.path.join(PKG, "libdilution_hip.so")
 HOST_OUT = os.path.join(PKG, "_host.so")
 BUILD = os.path.join(HERE, "_build")
 SOURCES = ["dil_api.hip", "dil_decode.hip", "dil_forward.hip", "dil_backward.hip", "dil_timing.hip",
-           "dil_noalloc.hip", "dil_linear.hip"]
+           "dil_noalloc.hip", "dil_linear.hip", "dil_tree.hip", "dil_evict.hip"]
 # (object stem, source, extra flags): the ablation variants of each bid
 # function are one object each, built from the same source
 VARIANT_OBJECTS = [(f"dil_variants_b{b}", "dil_variants.hip", [f"-DDIL_VARIANT_BID={b}"]) for b in range(8)]

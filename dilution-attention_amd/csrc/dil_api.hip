@@ -24,6 +24,12 @@ bool all_set(const Ps*... ps) {
   return ((ps != nullptr) && ...);
 }
 
+// 16-byte aligned, as the kernels' wide loads and stores need
+template <typename... Ps>
+bool aligned16(const Ps*... ps) {
+  return ((reinterpret_cast<uintptr_t>(ps) % 16 == 0) && ...);
+}
+
 // The layout rules of dil_rows: data 16-byte aligned, every stride that is
 // stepped over a multiple of 16 bytes, rows at least head_dim elements apart
 // (so a chunk past the last row lies past the resource that covers the rows)
@@ -132,6 +138,34 @@ void fill_forward(dil::ForwardArgs& a, int64_t n, int64_t seq, int head_dim, int
   a.var = dil::Variant{bid, share, shift};
   a.workspace = workspace;
   a.workspace_bytes = workspace_bytes;
+  a.stream = stream;
+}
+
+// What a tree step and an acceptance have in common.
+int check_tree(const dil_rows* q, int64_t batch, int64_t heads, int64_t nodes, int64_t capacity, int64_t length,
+               int head_dim, int dtype) {
+  if (!valid_head_dim(head_dim)) return dil::kErrHeadDim;
+  if (!valid_dtype(dtype)) return dil::kErrDtype;
+  if (!valid_slices(batch, heads) || nodes < 1 || nodes > dil::kTreeMaxNodes || length < 0 ||
+      length > capacity - nodes || capacity >= (int64_t{1} << 31))
+    return dil::kErrShape;
+  return valid_rows(q, batch, heads, head_dim, dtype) ? 0 : dil::kErrShape;
+}
+void fill_tree(dil::TreeArgs& a, const dil_rows* q, void* k_cache, void* v_cache, float* committed, int64_t batch,
+               int64_t heads, int64_t nodes, int64_t capacity, int64_t length, int head_dim, int dtype, void* stream) {
+  a.q = q->data;
+  a.qv = view_of(q, batch, heads, nodes, head_dim);
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.committed = committed;
+  a.cap = capacity;
+  a.batch = batch;
+  a.heads = heads;
+  a.n = batch * heads;
+  a.length = length;
+  a.nodes = static_cast<int>(nodes);
+  a.head_dim = head_dim;
+  a.dtype = dtype;
   a.stream = stream;
 }
 
@@ -482,6 +516,78 @@ int dil_backward(const void* q, const void* k, const void* v, const void* dout,
   return dil_backward_variant(q, k, v, dout, out, rmax, rden, ssum, carry, pk, n, seq, head_dim,
                               dtype, dout_dtype, grad_dtype, precision, 0, 1, 1.f, dq, dk, dv,
                               workspace, workspace_bytes, stream);
+}
+
+int64_t dil_tree_workspace_bytes(int64_t n, int64_t length, int64_t nodes, int head_dim, int dtype) {
+  return dil::tree_workspace_bytes(n, length, nodes, head_dim, dtype);
+}
+
+int dil_tree_step(const dil_rows* q, const void* k_cache, const void* v_cache, const float* committed,
+                  int64_t batch, int64_t heads, int64_t nodes, int64_t capacity, int64_t length,
+                  const int32_t* parents, int64_t parents_stride, int head_dim, int dtype, const dil_rows* out,
+                  float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int err = check_tree(q, batch, heads, nodes, capacity, length, head_dim, dtype)) return err;
+  if (!valid_rows(out, batch, heads, head_dim, dtype) || parents_stride < 0) return dil::kErrShape;
+  if (!all_set(k_cache, v_cache, static_cast<const void*>(committed), static_cast<const void*>(parents),
+               static_cast<const void*>(lse), static_cast<const void*>(workspace)) ||
+      !aligned16(k_cache, v_cache))
+    return dil::kErrShape;
+  if (workspace_bytes < dil::tree_workspace_bytes(batch * heads, length, nodes, head_dim, dtype))
+    return dil::kErrWorkspace;
+  dil::TreeArgs a{};
+  fill_tree(a, q, const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(committed), batch, heads,
+            nodes, capacity, length, head_dim, dtype, stream);
+  a.parents = parents;
+  a.parents_sb = parents_stride;
+  a.out = const_cast<void*>(out->data);
+  a.ov = view_of(out, batch, heads, nodes, head_dim);
+  a.lse = lse;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  return dil::tree_step(a);
+}
+
+int dil_tree_accept(const dil_rows* q, void* k_cache, void* v_cache, float* committed, int64_t batch, int64_t heads,
+                    int64_t nodes, int64_t capacity, int64_t length, const float* lse, const int32_t* path,
+                    int64_t path_stride, int64_t count, int head_dim, int dtype, void* stream) {
+  if (const int err = check_tree(q, batch, heads, nodes, capacity, length, head_dim, dtype)) return err;
+  if (count < 1 || count > nodes || path_stride < 0) return dil::kErrShape;
+  if (!all_set(static_cast<const void*>(k_cache), static_cast<const void*>(v_cache),
+               static_cast<const void*>(committed), static_cast<const void*>(lse), static_cast<const void*>(path)) ||
+      !aligned16(k_cache, v_cache))
+    return dil::kErrShape;
+  dil::TreeArgs a{};
+  fill_tree(a, q, k_cache, v_cache, committed, batch, heads, nodes, capacity, length, head_dim, dtype, stream);
+  a.lse = const_cast<float*>(lse);
+  a.path = path;
+  a.path_sb = path_stride;
+  a.count = static_cast<int>(count);
+  return dil::tree_accept(a);
+}
+
+int64_t dil_evict_workspace_bytes(int64_t n, int64_t length, int64_t keep) {
+  return dil::evict_workspace_bytes(n, length, keep);
+}
+
+int dil_evict(const void* k_cache, const void* v_cache, const float* committed, int64_t n, int64_t capacity,
+              int64_t length, int64_t keep, int64_t first, int64_t recent, int64_t out_capacity, int head_dim,
+              int dtype, void* k_out, void* v_out, float* committed_out, int32_t* index, void* workspace,
+              int64_t workspace_bytes, void* stream) {
+  if (!valid_head_dim(head_dim)) return dil::kErrHeadDim;
+  if (!valid_dtype(dtype)) return dil::kErrDtype;
+  if (n < 1 || n >= (int64_t{1} << 31) || length < 1 || length > capacity || length >= (int64_t{1} << 31) ||
+      keep < 1 || keep > length || first < 0 || recent < 0 || first > keep || recent > keep - first ||
+      out_capacity < keep || out_capacity >= (int64_t{1} << 31))
+    return dil::kErrShape;
+  if (!all_set(k_cache, v_cache, static_cast<const void*>(committed), static_cast<const void*>(k_out),
+               static_cast<const void*>(v_out), static_cast<const void*>(committed_out),
+               static_cast<const void*>(index), static_cast<const void*>(workspace)))
+    return dil::kErrShape;
+  if (!aligned16(k_cache, v_cache, k_out, v_out)) return dil::kErrShape;
+  if (workspace_bytes < dil::evict_workspace_bytes(n, length, keep)) return dil::kErrWorkspace;
+  return dil::evict(dil::EvictArgs{k_cache, v_cache, committed, capacity, n, length, keep, first, recent, out_capacity,
+                                   head_dim, dtype, k_out, v_out, committed_out, index, workspace, workspace_bytes,
+                                   stream});
 }
 
 }  // extern "C"

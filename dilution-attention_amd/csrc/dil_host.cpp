@@ -44,6 +44,11 @@ struct Api {
   decltype(&dil_decode_step_variant) decode_step_variant = nullptr;
   decltype(&dil_rows_linear) rows_linear = nullptr;
   decltype(&dil_rows_linear_qkv) rows_linear_qkv = nullptr;
+  decltype(&dil_tree_workspace_bytes) tree_workspace_bytes = nullptr;
+  decltype(&dil_tree_step) tree_step = nullptr;
+  decltype(&dil_tree_accept) tree_accept = nullptr;
+  decltype(&dil_evict_workspace_bytes) evict_workspace_bytes = nullptr;
+  decltype(&dil_evict) evict = nullptr;
 };
 Api api;
 bool bound = false;
@@ -67,6 +72,11 @@ void bind(const py::dict& a) {
   take(api.decode_step_variant, a, "dil_decode_step_variant");
   take(api.rows_linear, a, "dil_rows_linear");
   take(api.rows_linear_qkv, a, "dil_rows_linear_qkv");
+  take(api.tree_workspace_bytes, a, "dil_tree_workspace_bytes");
+  take(api.tree_step, a, "dil_tree_step");
+  take(api.tree_accept, a, "dil_tree_accept");
+  take(api.evict_workspace_bytes, a, "dil_evict_workspace_bytes");
+  take(api.evict, a, "dil_evict");
   bound = true;
 }
 
@@ -400,6 +410,122 @@ at::Tensor decode_step(const at::Tensor& q1, const at::Tensor& k, const at::Tens
 }
 
 // ---------------------------------------------------------------------------
+// drafted tokens and eviction
+
+// The nodes' queries against the cache; returns the capacity.
+int64_t check_nodes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& committed,
+                    int64_t length) {
+  if (q.dim() != 4) throw py::value_error("q must be (B, H, N, D), got " + dims(q));
+  const int64_t nodes = q.size(2);
+  if (nodes < 1 || nodes > 64)
+    throw py::value_error("a tree holds 1 to 64 drafted nodes, got " + std::to_string(nodes));
+  const int64_t capacity = check_cache(q, k, v, committed);
+  check_head_dim(q.size(3), nullptr);
+  if (length < 0 || length + nodes > capacity)
+    throw py::value_error("drafted rows [" + std::to_string(length) + ", " + std::to_string(length + nodes) +
+                          ") outside cache capacity " + std::to_string(capacity));
+  cache_type(k, v);
+  if (q.scalar_type() != k.scalar_type()) throw py::value_error("q must have the caches' dtype");
+  return capacity;
+}
+// (count,) or (B, count) node numbers: the step from one batch's to the next's
+int64_t nodes_step(const at::Tensor& x, int64_t batch, const char* name) {
+  const bool each = x.dim() == 2 && x.size(0) == batch;
+  if (x.scalar_type() != at::kInt || !(each || x.dim() == 1) || !x.is_contiguous())
+    throw py::value_error(std::string(name) + " must be contiguous int32 node numbers, (N,) or (B, N), got " + dims(x));
+  return each ? x.size(1) : 0;
+}
+
+// (out (B, H, N, D) in q's dtype and memory order, lse (B, H, N) fp32)
+std::tuple<at::Tensor, at::Tensor> tree_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                             const at::Tensor& committed, int64_t length, const at::Tensor& parents,
+                                             uintptr_t stream) {
+  const int64_t capacity = check_nodes(q, k, v, committed, length);
+  const int64_t batch = q.size(0), heads = q.size(1), nodes = q.size(2), d = q.size(3), n = batch * heads;
+  const int64_t step = nodes_step(parents, batch, "parents");
+  if (parents.size(-1) != nodes)
+    throw py::value_error("parents " + dims(parents) + " do not match the queries " + dims(q));
+  check_device({&q, &k, &v, &committed, &parents});
+  need_library();
+  const int tc = type_code(k.scalar_type());
+  c10::DeviceGuard guard(q.device());
+  const auto sd = slice_dims(batch, heads);
+  if (sd.first != batch) throw py::value_error("a tree step takes fewer than 65536 heads and B H H below 2^32");
+  const at::Tensor qs = operand(q, k.scalar_type(), false);
+  at::Tensor out = empty_as(q, k.scalar_type());
+  at::Tensor lse = at::empty({batch, heads, nodes}, q.options().dtype(at::kFloat));
+  if (n == 0) return {out, lse};
+  const at::Tensor ws = workspace(api.tree_workspace_bytes(n, length, nodes, static_cast<int>(d), tc), q);
+  launch("dil_tree_step", [&]() -> int {
+    const dil_rows rq = row_ref(qs), ro = row_ref(out);
+    return api.tree_step(&rq, k.data_ptr(), v.data_ptr(), f32(committed), batch, heads, nodes, capacity, length,
+                         static_cast<const int32_t*>(parents.data_ptr()), step, static_cast<int>(d), tc, &ro, f32(lse),
+                         ws.data_ptr(), ws.numel(), reinterpret_cast<void*>(stream));
+  });
+  return {out, lse};
+}
+
+void tree_accept(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& committed,
+                 int64_t length, const at::Tensor& lse, const at::Tensor& path, uintptr_t stream) {
+  const int64_t capacity = check_nodes(q, k, v, committed, length);
+  const int64_t batch = q.size(0), heads = q.size(1), nodes = q.size(2), d = q.size(3), n = batch * heads;
+  if (lse.scalar_type() != at::kFloat || lse.dim() != 3 || lse.size(0) != batch || lse.size(1) != heads ||
+      lse.size(2) != nodes || !lse.is_contiguous())
+    throw py::value_error("lse must be the contiguous float32 (B, H, N) of the tree step, got " + dims(lse));
+  const int64_t step = nodes_step(path, batch, "path"), count = path.size(-1);
+  if (count > nodes)
+    throw py::value_error("a path of " + std::to_string(count) + " nodes in a tree of " + std::to_string(nodes));
+  check_device({&q, &k, &v, &committed, &lse, &path});
+  need_library();
+  const int tc = type_code(k.scalar_type());
+  c10::DeviceGuard guard(q.device());
+  if (slice_dims(batch, heads).first != batch)
+    throw py::value_error("an acceptance takes fewer than 65536 heads and B H H below 2^32");
+  if (n == 0 || count == 0) return;
+  const at::Tensor qs = operand(q, k.scalar_type(), false);
+  launch("dil_tree_accept", [&]() -> int {
+    const dil_rows rq = row_ref(qs);
+    return api.tree_accept(&rq, k.data_ptr(), v.data_ptr(), f32(committed), batch, heads, nodes, capacity, length, f32(lse),
+                           static_cast<const int32_t*>(path.data_ptr()), step, count, static_cast<int>(d), tc,
+                           reinterpret_cast<void*>(stream));
+  });
+}
+
+// (k, v, committed, index) of the smaller cache
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> evict(const at::Tensor& k, const at::Tensor& v,
+                                                                 const at::Tensor& committed, int64_t length, int64_t keep,
+                                                                 int64_t first, int64_t recent, int64_t out_capacity,
+                                                                 uintptr_t stream) {
+  const int64_t capacity = check_cache(k, k, v, committed);
+  const int64_t batch = k.size(0), heads = k.size(1), d = k.size(3), n = batch * heads;
+  check_head_dim(d, nullptr);
+  if (length < 1 || length > capacity)
+    throw py::value_error("length " + std::to_string(length) + " outside cache capacity " + std::to_string(capacity));
+  if (keep < 1 || keep > length)
+    throw py::value_error("keep must be in [1, length " + std::to_string(length) + "], got " + std::to_string(keep));
+  if (first < 0 || recent < 0 || first > keep || recent > keep - first)
+    throw py::value_error("first and recent must be at least 0 and no more than keep together, got " +
+                          std::to_string(first) + " and " + std::to_string(recent) + " of " + std::to_string(keep));
+  if (out_capacity < keep)
+    throw py::value_error("capacity " + std::to_string(out_capacity) + " holds fewer than keep " + std::to_string(keep));
+  const int tc = cache_type(k, v);
+  check_device({&k, &v, &committed});
+  need_library();
+  c10::DeviceGuard guard(k.device());
+  at::Tensor ko = at::empty({batch, heads, out_capacity, d}, k.options()), vo = at::empty_like(ko);
+  at::Tensor co = at::empty({batch, heads, out_capacity}, committed.options());
+  at::Tensor index = at::empty({batch, heads, keep}, k.options().dtype(at::kInt));
+  if (n == 0) return {ko, vo, co, index};
+  const at::Tensor ws = workspace(api.evict_workspace_bytes(n, length, keep), k);
+  launch("dil_evict", [&]() -> int {
+    return api.evict(k.data_ptr(), v.data_ptr(), f32(committed), n, capacity, length, keep, first, recent, out_capacity,
+                     static_cast<int>(d), tc, ko.data_ptr(), vo.data_ptr(), f32(co), static_cast<int32_t*>(index.data_ptr()),
+                     ws.data_ptr(), ws.numel(), reinterpret_cast<void*>(stream));
+  });
+  return {ko, vo, co, index};
+}
+
+// ---------------------------------------------------------------------------
 // the decode step's few-row projections
 
 enum { kPlain = 0, kResid = 1, kNorm = 2, kSwiglu = 3 };
@@ -493,6 +619,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("backward", &backward);
   m.def("prefill_chunk", &prefill_chunk);
   m.def("decode_step", &decode_step);
+  m.def("tree_step", &tree_step);
+  m.def("tree_accept", &tree_accept);
+  m.def("evict", &evict);
   m.def("rows_linear", &rows_linear);
   m.def("rows_linear_qkv", &rows_linear_qkv);
 }

@@ -215,4 +215,51 @@ template <int BID> int forward_bid(const ForwardArgs& a);
 template <int BID> int backward_bid(const BackwardArgs& a);
 template <int BID> int decode_bid(const DecodeArgs& a);
 
+// Attention for a tree of drafted tokens over a cache, and the acceptance of one
+// of its paths (dil_tree.hip).
+constexpr int kTreeMaxNodes = 64;
+
+struct TreeArgs {
+  const void* q;             // the nodes' queries, in dtype
+  RowsView qv;
+  void* k_cache;             // (n, cap, D): cached keys [0, length), node i at length + i
+  void* v_cache;
+  int64_t cap;
+  float* committed;          // (n, cap) fp32
+  int64_t batch, heads, n, length;
+  int nodes, head_dim, dtype;
+  const int32_t* parents;    // step: node i of batch b at b * parents_sb + i
+  int64_t parents_sb;
+  void* out;                 // step: the nodes' outputs, in dtype
+  RowsView ov;
+  float* lse;                // (n, nodes) base-2 row statistics: written by the step, read by the acceptance
+  const int32_t* path;       // acceptance: the r-th accepted node of batch b at b * path_sb + r
+  int64_t path_sb;
+  int count;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+};
+int64_t tree_workspace_bytes(int64_t n, int64_t length, int64_t nodes, int head_dim, int dtype);
+int tree_step(const TreeArgs& a);
+int tree_accept(const TreeArgs& a);
+
+// Eviction by demand (dil_evict.hip).
+struct EvictArgs {
+  const void* k_cache;       // (n, cap, D)
+  const void* v_cache;
+  const float* committed;    // (n, cap)
+  int64_t cap, n, length, keep, first, recent, out_cap;
+  int head_dim, dtype;
+  void* k_out;               // (n, out_cap, D)
+  void* v_out;
+  float* committed_out;      // (n, out_cap)
+  int32_t* index;            // (n, keep)
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+};
+int64_t evict_workspace_bytes(int64_t n, int64_t length, int64_t keep);
+int evict(const EvictArgs& a);
+
 }  // namespace dil

@@ -21,6 +21,11 @@ one-call forward as the reference does.  Both give the same outputs and demand.
 The ablation variants (``bid`` / ``share_cumsum`` / ``shift`` keywords, the
 operators of ``kernels_bid``) prefill in one call and decode through the
 variant decode step (model.py:198-241 with ``_bid_kw``).
+
+``tree_step`` and ``accept_tree`` decode several drafted tokens at once (a tree
+of them, of which one path is taken), and ``evict_cache`` shrinks a cache to the
+keys that carry the demand.  The reference has no counterpart: it decodes one
+token at a time and its caches only grow.
 """
 
 from __future__ import annotations
@@ -102,3 +107,40 @@ def step_cache(q1: torch.Tensor, k1: torch.Tensor, v1: torch.Tensor, cache: dict
     if bid_kw:
         return kernels_bid.dilution_decode_step(q1, cache["k"], cache["v"], cache["committed"], t, **bid_kw)
     return kernels.dilution_decode_step(q1, cache["k"], cache["v"], cache["committed"], t)
+
+
+def tree_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, parents):
+    """Attention for N drafted tokens (q, k, v: (B, H, N, D)) that hang in a tree
+    below the cached context (``parents`` as in ``kernels.dilution_tree_step``).
+    Writes their k and v behind the cached positions and returns (y, draft): y
+    (B, H, N, D) in q.dtype, draft what ``accept_tree`` needs.  The cache's
+    length and demand stay; a later step overwrites rows that were not accepted."""
+    t, stop = cache["len"], cache["len"] + q.shape[2]
+    if stop > cache["k"].shape[2]:
+        raise ValueError("drafted tokens past the cache capacity (context_length)")
+    cache["k"][:, :, t:stop] = k
+    cache["v"][:, :, t:stop] = v
+    y, aux = kernels.dilution_tree_step(q, cache["k"], cache["v"], cache["committed"], t, parents, return_aux=True)
+    return y, {"q": q, "lse": aux["lse"], "len": t}
+
+
+def accept_tree(cache: dict, draft: dict, path) -> int:
+    """Take a path of the tree of the last ``tree_step`` on this cache into it
+    (``path`` as in ``kernels.dilution_tree_accept``); returns the new length."""
+    if draft["len"] != cache["len"]:
+        raise ValueError("the cache has moved on since this tree step")
+    cache["len"] = kernels.dilution_tree_accept(draft["q"], cache["k"], cache["v"], cache["committed"], cache["len"],
+                                                draft["lse"], path)
+    return cache["len"]
+
+
+def evict_cache(cache: dict, keep: int, first: int = 0, recent: int = 0, capacity: int | None = None) -> dict:
+    """A cache of the ``keep`` positions that carry the demand (the first
+    ``first`` and the last ``recent`` stay whatever they carry), in new buffers of
+    ``max(capacity, keep)`` positions.  The keys hold no position, so decoding
+    goes on over the kept ones.  A cache of at most ``keep`` positions is returned as it is."""
+    if cache["len"] <= keep:
+        return cache
+    k, v, committed, _ = kernels.dilution_evict(cache["k"], cache["v"], cache["committed"], cache["len"], keep,
+                                                first=first, recent=recent, capacity=capacity)
+    return {"k": k, "v": v, "len": keep, "committed": committed}

@@ -414,3 +414,139 @@ def decode_workspace(batch: int, heads: int, max_length: int, head_dim: int, dev
     """A workspace for ``decode_step_device_length`` up to ``max_length``."""
     lib = _hip.lib()
     return _workspace(lib.dil_decode_workspace_bytes(batch * heads, max_length, head_dim), device)
+
+
+# ---------------------------------------------------------------------------
+# drafted tokens over a cache (no reference counterpart)
+
+MAX_TREE_NODES = 64
+"""The most drafted nodes of one tree step."""
+
+
+def _node_numbers(x, device, low: int, high: int, name: str) -> torch.Tensor:
+    """Node numbers as int32 on ``device``.  Host values (sequences, CPU tensors)
+    come checked and are copied over; device tensors are taken as they are, int64
+    ones brought into [low, high] first, so that no value wraps into another."""
+    if not torch.is_tensor(x):
+        x = torch.tensor(x, dtype=torch.int64)
+    if x.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be int32 or int64, got {x.dtype}")
+    if x.dtype == torch.int64:
+        x = x.clamp(low, high).to(torch.int32)
+    return x.to(device).contiguous()
+
+
+def _check_parents(parents) -> None:
+    """ValueError unless every host value is -1, -2 (absent) or an earlier node."""
+    if torch.is_tensor(parents) and parents.is_cuda:
+        return
+    p = torch.as_tensor(parents)
+    if p.dtype in (torch.int32, torch.int64) and p.dim() in (1, 2):
+        if bool(((p < -2) | (p >= torch.arange(p.shape[-1]))).any()):
+            raise ValueError("each parent must be an earlier node, -1 (a child of the context) or -2 (absent)")
+
+
+def _check_path(path, nodes: int) -> None:
+    if torch.is_tensor(path) and path.is_cuda:
+        return
+    p = torch.as_tensor(path)
+    if p.dtype in (torch.int32, torch.int64) and p.numel():
+        if bool(((p < 0) | (p >= nodes)).any()) or bool((p.diff(dim=-1) <= 0).any()):
+            raise ValueError(f"a path runs down the tree: ascending node numbers in [0, {nodes})")
+
+
+def dilution_tree_step(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    committed: torch.Tensor,
+    length: int,
+    parents,
+    return_aux: bool = False,
+):
+    """Attention for a tree of drafted tokens over a decode cache; returns the
+    nodes' outputs (B, H, N, D) in q's dtype and memory order.
+
+    q: (B, H, N, D) in the caches' dtype, N <= 64 (views of a fused projection
+    need no copy).  k_cache / v_cache: contiguous (B, H, capacity, D) buffers
+    holding ``length`` cached keys (0 is allowed) and node i's row at position
+    ``length + i``.  committed: contiguous (B, H, capacity) fp32 demand of the
+    cached keys; what it holds for the drafted positions is not read.
+    ``parents``: (N,) for one tree or (B, N) for a tree per sequence, int32 or
+    int64 (on the caches' device, or on the host, where the values are checked):
+    an earlier node, or -1 for a child of the context.  Any other value marks an
+    absent node, the padding of a smaller tree; it and the nodes below it get a
+    zero output.
+
+    Node i sees the cached keys, its ancestors and itself, with the demand that
+    its ancestors add: its output is what ``dilution_decode_step`` gives after
+    decoding its path token by token, up to rounding.  It does not depend on the
+    nodes that it does not see.  Nothing in the cache changes:
+    ``dilution_tree_accept`` takes a path of the tree into it.
+
+    With return_aux also returns dict(lse): the (B, H, N) fp32 row statistics,
+    p_ij = 2^(log2(e) q_i.k_j / sqrt(D) - lse_i), +inf for absent nodes.
+    """
+    _check_parents(parents)
+    parents = _node_numbers(parents, q.device, -2, MAX_TREE_NODES, "parents")
+    out, lse = _native().tree_step(q, k_cache, v_cache, committed, length, parents, _raw_stream(q))
+    return (out, dict(lse=lse)) if return_aux else out
+
+
+def dilution_tree_accept(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    committed: torch.Tensor,
+    length: int,
+    lse: torch.Tensor,
+    path,
+) -> int:
+    """Take a path of a drafted tree into the cache, in place; returns the new
+    length.
+
+    q, the caches and ``length`` as in the ``dilution_tree_step`` before, ``lse``
+    from its aux.  ``path``: (A,) or (B, A) node numbers (int32 or int64, device
+    or host), from a child of the context down, each the parent of the next; the
+    sequences of a batch accept equally many, since a cache has one length.
+    ``committed`` takes the accepted rows' bids over the cached keys and holds
+    the accepted positions' own demand; the accepted K and V rows move to
+    positions length, length + 1, ...  Positions from the new length on are left
+    as they are (zero demand stays zero).  A device path is not checked: an entry
+    outside [0, N) counts for nothing and leaves its row.
+    """
+    if q.dim() == 4:
+        _check_path(path, q.shape[2])
+    path = _node_numbers(path, q.device, -1, MAX_TREE_NODES, "path")
+    _native().tree_accept(q, k_cache, v_cache, committed, length, lse, path, _raw_stream(q))
+    return length + path.shape[-1]
+
+
+# ---------------------------------------------------------------------------
+# eviction (no reference counterpart; the reference's caches only grow)
+
+
+def dilution_evict(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    committed: torch.Tensor,
+    length: int,
+    keep: int,
+    first: int = 0,
+    recent: int = 0,
+    capacity: int | None = None,
+):
+    """A smaller cache of the ``keep`` keys that carry the demand: returns
+    (k, v, committed, index).
+
+    Per (batch, head) the ``first`` first and the ``recent`` last of the
+    ``length`` cached positions stay, and of those between, the keep - first -
+    recent with the largest ``committed`` (the attention weight that every row so
+    far has put on the key).  Equal demands: the lower position stays; a NaN
+    counts as the largest.  Kept rows keep their order.  k and v are new
+    (B, H, max(capacity, keep), D) buffers and committed their fp32 demand, zero
+    past ``keep``; index (B, H, keep) int32 holds the positions that stayed.
+    The caches given are not changed.
+    """
+    capacity = max(keep if capacity is None else capacity, keep)
+    return _native().evict(k_cache, v_cache, committed, length, keep, first, recent, capacity, _raw_stream(k_cache))

@@ -21,7 +21,9 @@ weights).  It follows the reference's module layout and cache protocol
 * ``DilutionLM``: embedding tied to the LM head, blocks, final norm;
   ``forward(idx, targets)`` -> (logits, loss), ``prefill``, ``decode_step``
   and cached greedy / sampled ``generate`` (model.py:342-512, sampling with
-  ``filter_logits``, model.py:289-304);
+  ``filter_logits``, model.py:289-304), with caches bounded by ``Eviction``;
+* ``tree_step`` / ``accept_tree`` / ``generate_drafted``: several drafted tokens
+  checked in one step (no reference counterpart);
 * ``rows_linear``: the decode step's projections at M = batch (<= 8 rows) on
   the HIP library (``dil_rows_linear``), with the RMSNorms, the residual adds
   and the SwiGLU activation folded in: a bf16 model's cached decode step (eager
@@ -241,6 +243,12 @@ class DilutionAttention(_AttentionBase):
         y = dcache.step_cache(q1, k1, v1, cache, **self.bid_kw)
         return self._merge_heads(y.to(x1.dtype), batch, 1)
 
+    def tree_step(self, x: torch.Tensor, cache: dict, parents):
+        batch, nodes, _ = x.shape
+        q, k, v = self._split_heads(x)
+        y, draft = dcache.tree_step(q, k, v, cache, parents)
+        return self._merge_heads(y, batch, nodes), draft
+
 
 class SwiGLUMLP(nn.Module):
     def __init__(self, cfg: LMConfig):
@@ -277,6 +285,11 @@ class Block(nn.Module):
     def step_cache(self, x1: torch.Tensor, cache: dict) -> torch.Tensor:
         x1 = x1 + self.attn.step_cache(self.ln_1(x1), cache)
         return x1 + self.mlp(self.ln_2(x1))
+
+    def tree_step(self, x: torch.Tensor, cache: dict, parents):
+        y, draft = self.attn.tree_step(self.ln_1(x), cache, parents)
+        x = x + y
+        return x + self.mlp(self.ln_2(x)), draft
 
 
 class DilutionLM(nn.Module):
@@ -353,6 +366,41 @@ class DilutionLM(nn.Module):
             x = block.step_cache(x, cache)
         return self.lm_head(self.ln_f(x))
 
+    @torch.no_grad()
+    def tree_step(self, tokens: torch.Tensor, parents, caches):
+        """Logits (B, N, vocab) behind each of N drafted tokens (B, N) that hang in
+        a tree below the cached context (``parents`` as in
+        ``kernels.dilution_tree_step``), and the drafts that ``accept_tree``
+        takes.  The caches' lengths and demands stay.  Every layer has to run the
+        production dilution operator."""
+        self._need_production("tree_step")
+        x, drafts = self.wte(tokens), []
+        for block, cache in zip(self.h, caches):
+            x, draft = block.tree_step(x, cache, parents)
+            drafts.append(draft)
+        return self.lm_head(self.ln_f(x)), drafts
+
+    def accept_tree(self, caches, drafts, path) -> int:
+        """Take a path of the last ``tree_step``'s tree into every layer's cache
+        (``cache.accept_tree``); returns the new length."""
+        if not torch.is_tensor(path):
+            path = torch.tensor(path, dtype=torch.int64)
+        if not path.is_cuda:
+            kernels._check_path(path, drafts[0]["q"].shape[2])
+            path = path.to(caches[0]["k"].device)       # once, not in every layer
+        for cache, draft in zip(caches, drafts):
+            length = dcache.accept_tree(cache, draft, path)
+        return length
+
+    def evict(self, caches, eviction: "Eviction", capacity: int | None = None) -> list:
+        """Every layer's cache shrunk by its own demand (``cache.evict_cache``)."""
+        self._need_production("evict")
+        return [dcache.evict_cache(c, eviction.keep, eviction.first, eviction.recent, capacity) for c in caches]
+
+    def _need_production(self, what: str) -> None:
+        if not self.graph_decode_eligible():
+            raise ValueError(f"{what} needs every layer on the production dilution operator")
+
     def graph_decode_eligible(self) -> bool:
         """Every layer runs the production dilution operator (the decode step
         GraphDecoder captures)."""
@@ -405,17 +453,25 @@ class DilutionLM(nn.Module):
     def generate(self, idx: torch.Tensor, max_new_tokens: int, temperature: float = 0.0,
                  top_k: int | None = None, top_p: float | None = None,
                  generator: torch.Generator | None = None, vocab_limit: int | None = None,
-                 graph: bool = False) -> torch.Tensor:
+                 graph: bool = False, eviction: "Eviction | None" = None) -> torch.Tensor:
         """Cached generation with caches sized prompt + max_new_tokens
         (model.py:473-509): temperature 0 is greedy, otherwise a sample of
         softmax(logits / temperature) after top-k / nucleus truncation;
         ``generator`` makes sampling reproducible, ``vocab_limit`` keeps the
         new tokens below that id.  ``graph=True`` runs greedy decoding of an
         all-dilution production stack through ``GraphDecoder`` (the same
-        tokens, one HIP graph replay per step)."""
+        tokens, one HIP graph replay per step).  ``eviction`` bounds the caches:
+        when they hold ``eviction.limit`` positions they shrink to its ``keep``
+        (not with ``graph``, whose captured step holds the caches' addresses)."""
         if vocab_limit is not None and not 0 < vocab_limit <= self.cfg.vocab_size:
             raise ValueError(f"vocab_limit must be in (0, {self.cfg.vocab_size}]")
-        logits, caches = self.prefill(idx, capacity=idx.shape[1] + max_new_tokens)
+        capacity = idx.shape[1] + max_new_tokens
+        if eviction is not None:
+            if graph:
+                raise ValueError("a graph-replayed generation keeps its caches: eviction needs graph=False")
+            self._need_production("eviction")
+            capacity = min(capacity, max(idx.shape[1], eviction.limit) + 1)
+        logits, caches = self.prefill(idx, capacity=capacity)
         tokens = idx
         if graph and max_new_tokens > 0 and not (temperature and temperature > 0.0) and self.graph_decode_eligible():
             last = logits[:, -1, :].float()
@@ -444,8 +500,84 @@ class DilutionLM(nn.Module):
                     nxt = torch.multinomial(probs, 1, generator=generator)
             tokens = torch.cat([tokens, nxt], dim=1)
             if step + 1 < max_new_tokens:
+                if eviction is not None and caches[0]["len"] >= eviction.limit:
+                    caches = self.evict(caches, eviction, capacity)
                 logits = self.decode_step(nxt, caches)
         return tokens
+
+
+    @torch.no_grad()
+    def generate_drafted(self, idx: torch.Tensor, max_new_tokens: int, draft, vocab_limit: int | None = None,
+                         eviction: "Eviction | None" = None) -> torch.Tensor:
+        """Greedy generation that checks drafted tokens, several per step: the tokens
+        of ``generate`` (up to rounding, where two logits nearly tie), in fewer
+        steps the better the drafts are.
+
+        ``draft(tokens)`` gets the (B, T) tokens so far and returns (drafted,
+        parents): (B, M) tokens and the M parents of their tree (-1: right behind
+        the last token; M <= 63, and 0 is allowed).  One ``tree_step`` runs the last token
+        and the drafted ones; each sequence takes the path whose tokens are
+        the greedy picks, the shortest of the batch's paths counts (a cache has one
+        length), and the pick behind it is the next token.  (No reference counterpart:
+        the reference's sampler decodes token by token, model.py:473-509.)"""
+        self._need_production("generate_drafted")
+        if vocab_limit is not None and not 0 < vocab_limit <= self.cfg.vocab_size:
+            raise ValueError(f"vocab_limit must be in (0, {self.cfg.vocab_size}]")
+        batch, prompt = idx.shape
+        if max_new_tokens <= 0:
+            return idx
+        room = kernels.MAX_TREE_NODES
+        capacity = prompt + max_new_tokens + room
+        if eviction is not None:
+            capacity = min(capacity, max(prompt, eviction.limit) + room)
+        logits, caches = self.prefill(idx, capacity=capacity)
+
+        def pick(x):
+            x = x if vocab_limit is None else x[..., :vocab_limit]
+            return x.float().argmax(dim=-1)
+
+        tokens = torch.cat([idx, pick(logits[:, -1:])], dim=1)
+        while tokens.shape[1] < prompt + max_new_tokens:
+            if eviction is not None and caches[0]["len"] >= eviction.limit:
+                caches = self.evict(caches, eviction, capacity)
+            drafted, parents = draft(tokens)
+            left = prompt + max_new_tokens - tokens.shape[1]
+            tree = torch.cat([tokens[:, -1:], drafted.to(tokens)], dim=1)
+            # node 0 is the last token, the drafted ones follow
+            below = [-1] + [int(p) + 1 for p in parents]
+            if len(below) != tree.shape[1]:
+                raise ValueError(f"{len(below) - 1} parents for {tree.shape[1] - 1} drafted tokens")
+            logits, drafts = self.tree_step(tree, below, caches)
+            picks, host = pick(logits), tree.tolist()
+            wanted, paths = picks.tolist(), []
+            for b in range(batch):
+                path = [0]
+                for node in range(1, len(below)):
+                    if below[node] == path[-1] and host[b][node] == wanted[b][path[-1]]:
+                        path.append(node)
+                paths.append(path)
+            count = min(left, *(len(p) for p in paths))
+            path = torch.tensor([p[:count] for p in paths], device=tokens.device)
+            self.accept_tree(caches, drafts, path)
+            # the accepted nodes' picks: the drafted tokens below the first, and one more
+            tokens = torch.cat([tokens, picks.gather(1, path)], dim=1)
+        return tokens
+
+
+@dataclass
+class Eviction:
+    """When and how a generation's caches shrink: at ``limit`` positions to the
+    ``keep`` that carry the demand, among them the ``first`` first and the
+    ``recent`` last."""
+
+    limit: int
+    keep: int
+    first: int = 4
+    recent: int = 0
+
+    def __post_init__(self):
+        if self.first < 0 or self.recent < 0 or not 1 <= self.first + self.recent <= self.keep < self.limit:
+            raise ValueError("an eviction needs 1 <= first + recent <= keep < limit")
 
 
 class GraphDecoder:

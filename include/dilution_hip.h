@@ -360,6 +360,72 @@ int dil_rows_argmax(const void* logits, int64_t rows, int64_t row_stride, int64_
                     void* stream);
 
 /*
+ * Attention for a tree of drafted tokens over a decode cache.  No counterpart in the
+ * reference, whose decode takes one token (src/dilution/kernels.py:994-1038).
+ *
+ * Every batch has `nodes` <= 64 drafted tokens whose K and V rows lie at positions
+ * length + i of its (n, capacity, head_dim) caches (n = batch * heads, length >= 0,
+ * length + nodes <= capacity, capacity < 2^31).  parents[b * parents_stride + i]
+ * (int32 on the device; stride 0: one tree for every batch) is an earlier node
+ * (0 <= parent < i) or -1, a child of the context; any other value marks an absent
+ * node (the padding of a smaller tree), and so are the nodes below one.  Node i
+ * sees the cached keys [0, length), its ancestors and itself, with the demand that
+ * decoding its path token by token would show:
+ *
+ *   p_ij  = 2^(a_ij - lse_i),  a_ij = log2(e) q_i.k_j / sqrt(head_dim)
+ *   t_ij  = committed_j + sum of p_aj over i's ancestors a + p_ij
+ *           (a drafted key's own committed entry counts as 0)
+ *   out_i = sum_j (p_ij / (t_ij + eps)) v_j / (sum_j p_ij / (t_ij + eps) + eps)
+ *
+ * q and out are dil_rows of nodes rows per slice in the caches' dtype; lse
+ * (n, nodes) float32.  An absent node's out is 0 and its lse +inf; its K, V and q
+ * rows are read but count for nothing, whatever they hold.  A node's results do not
+ * depend on nodes that it does not see.  Nothing in the caches changes.  The caches
+ * are 16-byte aligned.
+ */
+int64_t dil_tree_workspace_bytes(int64_t n, int64_t length, int64_t nodes, int head_dim, int dtype);
+int dil_tree_step(const dil_rows* q, const void* k_cache, const void* v_cache, const float* committed,
+                  int64_t batch, int64_t heads, int64_t nodes, int64_t capacity, int64_t length,
+                  const int32_t* parents, int64_t parents_stride, int head_dim, int dtype, const dil_rows* out,
+                  float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The acceptance of `count` of the drafted tokens (1 <= count <= nodes): path
+ * (int32 on the device, the r-th at b * path_stride + r) names a chain of nodes
+ * from one below the context on, each the parent of the next.  In place:
+ *
+ *   committed_j          += sum_r p_{path r, j}          for the cached keys j < length
+ *   committed_{length+r}  = sum_{s >= r} p_{path s, path r}
+ *   K and V rows length + path r  ->  length + r
+ *
+ * from the q and lse of the tree step over the same caches.  Positions from
+ * length + count on are left as they are.  An entry of path outside [0, nodes)
+ * counts for nothing: its K and V rows stay as they were, and its committed entry
+ * becomes 0.
+ */
+int dil_tree_accept(const dil_rows* q, void* k_cache, void* v_cache, float* committed, int64_t batch, int64_t heads,
+                    int64_t nodes, int64_t capacity, int64_t length, const float* lse, const int32_t* path,
+                    int64_t path_stride, int64_t count, int head_dim, int dtype, void* stream);
+
+/*
+ * Eviction by demand: `keep` of a cache's `length` keys into a new cache.  No
+ * counterpart in the reference, whose cache only grows (src/dilution/model.py:76-93).
+ *
+ * Per slice, the `first` first positions, the `recent` last ones and, of those
+ * between, the keep - first - recent whose committed is largest stay, in their
+ * order (first + recent <= keep <= length <= capacity, below 2^31).  Among equal
+ * values the lowest position stays; -0 equals +0, and a NaN counts as the largest.
+ * index (n, keep) int32 takes the positions; k_out, v_out (n, out_capacity,
+ * head_dim) and committed_out (n, out_capacity) the rows, zero from `keep` on.
+ * K and V are 16-byte aligned, and no output overlaps an input.
+ */
+int64_t dil_evict_workspace_bytes(int64_t n, int64_t length, int64_t keep);
+int dil_evict(const void* k_cache, const void* v_cache, const float* committed, int64_t n, int64_t capacity,
+              int64_t length, int64_t keep, int64_t first, int64_t recent, int64_t out_capacity, int head_dim,
+              int dtype, void* k_out, void* v_out, float* committed_out, int32_t* index, void* workspace,
+              int64_t workspace_bytes, void* stream);
+
+/*
  * Kernel timing for measurement harnesses.  No reference counterpart (the
  * reference times its Triton launches with torch.profiler and CUDA events in
  * scripts/step_profile.py:29-47 and scripts/profile_kernels.py:115-144).
