@@ -1,34 +1,74 @@
 // Attention for a tree of drafted tokens over a decode cache, and the acceptance
 // of one of its paths (include/dilution_hip.h: dil_tree_step, dil_tree_accept).
 //
-// A node's share of a key is p / (committed + the ancestors' p + p + eps): not
-// linear in p, so the row statistics have to be known before any share.  Launches:
+// For node i and key j, with anc(i) the ancestors of i among the drafted nodes:
+//   a_ij = log2(e) / sqrt(D) q_i.k_j      lse_i = log2 sum_j 2^a_ij
+//   p_ij = 2^(a_ij - lse_i)               t_ij  = committed_j + sum_{a in anc(i)} p_aj
+//   share = p / (t + p + eps)             out_i = sum_j share v_j / (sum_j share + eps)
+// A share is not linear in p, so lse has to be known first and K is read twice:
 //
-//   tree_stats  (chunks x slices)  per chunk and node: max and sum 2^(a - max)
-//   tree_lse    (slices)           the chunks' statistics joined: lse
-//   tree_apply  (chunks x slices)  one key per thread, the nodes in order: the
-//                                  demand goes down the tree through LDS; partial
-//                                  sums of the shares and of share V
-//   tree_finish (nodes x slices)   the chunks' partials added
+//   tree_stats   per chunk of keys and node: max and sum 2^(a - max)
+//   tree_apply   joins the chunks' statistics; per chunk and node: the sums of
+//                share and of share v
+//   tree_finish  joins the chunks' sums
+//   tree_demand  the acceptance: committed_j += sum of the accepted nodes' p_ij
 //
-// and for the acceptance
-//
-//   tree_accept (chunks + 1 x slices)  the demand of the cached keys; the last
-//                                      workgroup moves the drafted rows
-#include "dil_common.hpp"
-#include "dil_internal.hpp"
+// The cached keys go through matrix instructions in tiles of 32 keys x 32 nodes
+// (one or two node tiles), a wave per tile with no barrier and no LDS traffic but
+// the queries.  tree_apply's chain keeps every intermediate in the accumulators:
+//   1  S = Q K^T with the nodes as rows, permuted so that a lane (one key) holds
+//      runs of 8 consecutive nodes: p = 2^(S - lse) is then the A operand of
+//   2  t^T = P^T seen^T and p^T = P^T 1 (seen: the 0/1 matrix of the ancestors),
+//      which sum the demand down the tree for all nodes at once and leave a lane
+//      one node and 16 keys.  committed + eps is the accumulator's start value.
+//      p enters as two bf16 parts (16 bits of it, 2^-17), three for fp32 caches.
+//   3  the shares, in place, are the B operand of out^T += V^T share^T, whose A
+//      operand takes V rows as loaded, two head dims a register, regrouped by
+//      byte permutes.
+// The drafted keys (at most 64) are a workgroup of their own in plain fp32: there
+// the masks are, and what a node does not see it must not touch (NaN included).
+// A node whose own row statistics are NaN would spoil the others in step 2: its
+// bids are taken as 0 there (the clamp of p to [0, 1] does that), and tree_finish
+// makes it and the nodes below it NaN.
+#include "dil_tiles.hpp"
 
 namespace dil {
 namespace {
 
 constexpr int kTreeThreads = 256;
-constexpr int kTreeKeys = 256;                 // keys per workgroup, one a thread
+constexpr int kTreeWaves = kTreeThreads / 64;
+constexpr int kTileNodes = 32;
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// fp16 shares are scaled by 2^14: shares lie in [0, 1], those of a long context
+// near 1e-5 and below, under fp16's smallest normal number.
+template <int DT> constexpr float kShareScale = DT == DT_F16 ? 16384.f : 1.f;
+
+// One 16-byte piece of a row per lane (lane half h holds the h-th 16 bytes of each
+// 32): 8 elements of a 16-bit type, one instruction; 4 fp32, four instructions.
 template <int DT>
-__device__ __forceinline__ float elem(const void* p, int64_t i) {
-  if constexpr (DT == DT_F32) return static_cast<const float*>(p)[i];
-  else if constexpr (DT == DT_BF16) return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
-  else return f16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
+__device__ __forceinline__ floatx16 mma_piece(u32x4 a, u32x4 b, floatx16 c) {
+  if constexpr (DT == DT_BF16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else if constexpr (DT == DT_F16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+    return c;
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{lo, hi}, bf16x2));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{lo, hi}, f16x2));
 }
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t x, int lane) {
@@ -68,178 +108,655 @@ struct Tree {
   void* out;
   RowsView ov;
   float* lse;
-  float2* part;
-  float* part_out;
+  float2* part;              // (n, nchunk + 1, nodes): entry 0 of a slice is the drafted keys'
+  float* part_out;           // (n, nchunk + 1, nodes, D)
+  float* part_sum;           // (n, nchunk + 1, nodes)
+  float* aff;                // (n, nodes, nodes): the drafted keys' affinities
   int nchunk;
+  int chunk;                 // cached keys of a workgroup, a multiple of 32
   float scale;
   int64_t slice0;
+  // the acceptance
+  float* demand;
+  void* k_move;
+  void* v_move;
+  const int32_t* path;
+  int64_t path_sb;
+  int count;
 };
 
-// a_ij of the drafted node in q_s against key row j (from memory)
 template <int D, int DT>
-__device__ __forceinline__ float score(const float* q_s, const void* k, int64_t row) {
-  float s = 0.f;
-  for (int d = 0; d < D; ++d) s = fmaf(q_s[d], elem<DT>(k, row + d), s);
-  return s;
-}
+struct Shape {
+  static constexpr int kElt = DT == DT_F32 ? 4 : 2;
+  static constexpr int kRow = D * kElt;            // bytes
+  static constexpr int kPieces = kRow / 32;        // per lane half
+};
 
-template <int D, int DT>
-__global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
-  const int64_t slice = A.slice0 + blockIdx.y;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  __shared__ float q_s[D];
-  __shared__ uint64_t seen_s[kTreeMaxNodes];
-  __shared__ float sm[4], sl[4];
-  if (wave == 0) seen_s[lane] = nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, lane);
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * kTreeKeys + t, end = A.length + A.nodes;
-  const int64_t row = (slice * A.cap + (j < end ? j : end - 1)) * D;
-  const int64_t qbase = A.qv.slice(slice);
-  for (int i = 0; i < A.nodes; ++i) {
-    __syncthreads();
-    for (int d = t; d < D; d += kTreeThreads) q_s[d] = elem<DT>(A.q, qbase + i * A.qv.sr + d) * A.scale;
-    __syncthreads();
-    const uint64_t seen = seen_s[i];
-    const bool on = seen != 0 && j < end && (j < A.length || (seen >> (j - A.length) & 1));
-    const float a = on ? score<D, DT>(q_s, A.k, row) : -INFINITY;
-    const float m = wave_max(a);
-    if (lane == 0) sm[wave] = m;
-    __syncthreads();
-    const float mm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    const float l = wave_sum(on ? exp2f(a - mm) : 0.f);
-    if (lane == 0) sl[wave] = l;
-    __syncthreads();
-    if (t == 0)
-      A.part[(slice * A.nchunk + blockIdx.x) * A.nodes + i] = make_float2(mm, sl[0] + sl[1] + sl[2] + sl[3]);
+// The queries of up to NT * 32 rows in LDS, as pieces: [tile][piece][half][row].
+// row_of(r): the node of row r, or -1 for a row of zeros.
+template <int D, int DT, int NT, typename F>
+__device__ __forceinline__ void stage_queries(u32x4* q_s, const Tree& A, int64_t slice, F&& row_of) {
+  using S = Shape<D, DT>;
+  constexpr int kUnits = S::kRow / 16;
+  const char* base = static_cast<const char*>(A.q) + A.qv.slice(slice) * S::kElt;
+  for (int u = threadIdx.x; u < NT * kTileNodes * kUnits; u += kTreeThreads) {
+    const int r = u / kUnits, c = u % kUnits, node = row_of(r);
+    u32x4 x = {0, 0, 0, 0};
+    if (node >= 0) x = *reinterpret_cast<const u32x4*>(base + node * A.qv.sr * S::kElt + c * 16);
+    q_s[(((r >> 5) * S::kPieces + (c >> 1)) * 2 + (c & 1)) * kTileNodes + (r & 31)] = x;
   }
 }
 
-__global__ void tree_lse(Tree A) {
-  const int64_t slice = A.slice0 + blockIdx.x;
-  const int i = threadIdx.x;
-  const uint64_t seen = nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, i);
-  if (i >= A.nodes) return;
-  float m = -INFINITY, l = 0.f;
-  for (int c = 0; c < A.nchunk; ++c) {
-    const float2 p = A.part[(slice * A.nchunk + c) * A.nodes + i];
-    const float mn = fmaxf(m, p.x);
-    if (p.y != 0.f || p.y != p.y) {
-      l = l * exp2f(m - mn) + p.y * exp2f(p.x - mn);
-      m = mn;
+// 32 rows of a chunk, one per lane (l & 31): rows past the resource's end read 0.
+// The row offset is part of the per-lane offset: the range check of a buffer load
+// covers that one.
+template <int D, int DT>
+struct KeyRows {
+  u32x4 p[Shape<D, DT>::kPieces];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int row0, int lane) {
+    const uint32_t off = static_cast<uint32_t>(row0 + (lane & 31)) * Shape<D, DT>::kRow + (lane >> 5) * 16u;
+#pragma unroll
+    for (int g = 0; g < Shape<D, DT>::kPieces; ++g)
+      p[g] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 32u * g, 0, 0));
+  }
+};
+
+// 32 V rows as A operands of V^T: lane (d, h) of instruction step s, slot t holds key
+// 16 s + 8 (t >> 2) + 4 h + (t & 3) (fp32: register i, key acc_row(i, h)).  A lane
+// loads E = DV / 32 consecutive head dims of a row: row u of operand tile e is head
+// dim E * u + e.
+template <int DV, int DT>
+struct ValueRows {
+  static constexpr int E = DV < 32 ? 1 : DV / 32;
+  static constexpr int kBytes = E * (DT == DT_F32 ? 4 : 2);   // per lane and row: 2 to 32
+  static constexpr int kWords = kBytes < 4 ? 1 : kBytes / 4;
+  uint32_t w[16][kWords];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int row0, int lane, int rowbytes, int d0bytes) {
+    const int l32 = lane & 31, h = lane >> 5;
+    uint32_t off = static_cast<uint32_t>(row0 + 4 * h) * rowbytes + d0bytes + l32 * kBytes;
+    if constexpr (DV < 32) {
+      if (l32 >= DV) off = 0xf0000000u;              // past the end: zeros
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t o = off + static_cast<uint32_t>(8 * (i >> 2) + (i & 3)) * rowbytes;
+      if constexpr (kBytes == 2) {
+        w[i][0] = __builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0);
+      } else if constexpr (kBytes == 4) {
+        w[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+      } else if constexpr (kBytes == 8) {
+        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0));
+        w[i][0] = x[0];
+        w[i][1] = x[1];
+      } else {
+#pragma unroll
+        for (int c = 0; c < kBytes / 16; ++c) {
+          const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o + 16u * c, 0, 0));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[i][4 * c + e] = x[e];
+        }
+      }
     }
   }
-  A.lse[slice * A.nodes + i] = seen != 0 ? m + log2f(l) : INFINITY;
+  // 16-bit types: operand tile e, step s
+  __device__ __forceinline__ u32x4 frag(int e, int s) const {
+    u32x4 f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t lo = w[8 * s + 2 * t][e / 2], hi = w[8 * s + 2 * t + 1][e / 2];
+      f[t] = __builtin_amdgcn_perm(hi, lo, e & 1 ? 0x07060302u : 0x05040100u);
+    }
+    return f;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// the drafted keys
+
+// Affinities of every node for the drafted keys that it sees; the maxima and sums
+// of 2^(a - max) over them as the slice's entry 0.
+template <int D, int DT>
+__device__ void draft_stats(const Tree& A, int64_t slice, float (*a_s)[kTreeMaxNodes + 1], const uint64_t* seen_s) {
+  const int t = threadIdx.x, n = A.nodes;
+  const int64_t qbase = A.qv.slice(slice), kbase = (slice * A.cap + A.length) * D;
+  for (int p = t; p < n * n; p += kTreeThreads) {
+    const int i = p / n, a = p % n;
+    if (!(seen_s[i] >> a & 1)) continue;
+    float s = 0.f;
+    for (int d = 0; d < D; d += 8) {
+      float x[8], y[8];
+      load8_f32(A.q, qbase + i * A.qv.sr + d, DT, x);
+      load8_f32(A.k, kbase + static_cast<int64_t>(a) * D + d, DT, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+    }
+    s *= A.scale;
+    a_s[i][a] = s;
+    A.aff[(slice * n + i) * n + a] = s;
+  }
+  __syncthreads();
+  if (t >= n) return;
+  float m = -INFINITY, l = 0.f;
+  for (int a = 0; a <= t; ++a)
+    if (seen_s[t] >> a & 1) m = fmaxf(m, a_s[t][a]);
+  const float mr = m == -INFINITY ? 0.f : m;
+  for (int a = 0; a <= t; ++a)
+    if (seen_s[t] >> a & 1) l += fast_exp2(a_s[t][a] - mr);
+  A.part[slice * (A.nchunk + 1) * n + t] = make_float2(m, l);
 }
 
+constexpr int kShareStride = kTreeMaxNodes + 4;         // floats: 16-byte rows, a column on 16 banks
+
+// Shares of the drafted keys and their part of the outputs.  sh_s[a][i]: -1 where
+// node i does not see key a (shares are not negative there: the drafted keys start
+// without demand).
 template <int D, int DT>
-__global__ __launch_bounds__(kTreeThreads) void tree_apply(Tree A) {
+__device__ void draft_apply(const Tree& A, int64_t slice, float (*t_s)[kTreeMaxNodes + 1], float (*sh_s)[kShareStride],
+                            const uint64_t* seen_s, const int32_t* parents, const float* lse_s) {
+  const int t = threadIdx.x, n = A.nodes;
+  const int64_t p0 = slice * (A.nchunk + 1) * n;
+  if (t < 64) {                                        // one wave: lane = key
+    for (int i = 0; i < kTreeMaxNodes; ++i) {
+      const bool on = i < n && (seen_s[i] >> t & 1);
+      float sh = -1.f;
+      if (on) {
+        const float p = fast_exp2(A.aff[(slice * n + i) * n + t] - lse_s[i]);
+        const int par = parents[i];
+        // the parent does not see a node's own key: it starts at 0
+        const float tot = (par >= 0 && t != i ? t_s[par][t] : 0.f) + p;
+        t_s[i][t] = tot;
+        sh = p * fast_rcp(tot + kEps);
+      }
+      sh_s[t][i] = sh;
+      const float s = wave_sum(on ? sh : 0.f);
+      if (t == 0 && i < n) A.part_sum[p0 + i] = s;
+    }
+  }
+  __syncthreads();
+  constexpr int kPer = D * kTreeMaxNodes / kTreeThreads;        // nodes of a thread
+  const int d = t % D, i0 = t / D * kPer;
+  if (i0 >= n) return;
+  const int64_t vbase = (slice * A.cap + A.length) * D + d;
+  float x[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) x[u] = 0.f;
+  for (int a = 0; a < n; ++a) {
+    const int64_t at = vbase + static_cast<int64_t>(a) * D;
+    float v;
+    if constexpr (DT == DT_F32) v = static_cast<const float*>(A.v)[at];
+    else if constexpr (DT == DT_BF16) v = bf16_bits_to_f32(static_cast<const uint16_t*>(A.v)[at]);
+    else v = f16_bits_to_f32(static_cast<const uint16_t*>(A.v)[at]);
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const float w = sh_s[a][i0 + u];
+      x[u] = w < 0.f ? x[u] : fmaf(w, v, x[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kPer; ++u)
+    if (i0 + u < n) A.part_out[(p0 + i0 + u) * D + d] = x[u];
+}
+
+// ---------------------------------------------------------------------------
+// statistics
+
+template <int D, int DT, int NT>
+__global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
+  using S = Shape<D, DT>;
   const int64_t slice = A.slice0 + blockIdx.y;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  __shared__ float q_s[D], sh_s[kTreeKeys], ss[4];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, h = lane >> 5;
+  __shared__ union {
+    u32x4 q[NT * S::kPieces * 64];
+    float a[kTreeMaxNodes][kTreeMaxNodes + 1];
+  } s;
   __shared__ uint64_t seen_s[kTreeMaxNodes];
-  __shared__ float t_s[kTreeMaxNodes][kTreeKeys];
+  __shared__ float2 red[kTreeWaves][NT * kTileNodes];
+  if (blockIdx.x == 0) {
+    if (wave == 0) seen_s[lane] = nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, lane);
+    __syncthreads();
+    draft_stats<D, DT>(A, slice, s.a, seen_s);
+    return;
+  }
+  stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return r < A.nodes ? r : -1; });
+  const int64_t j0 = static_cast<int64_t>(blockIdx.x - 1) * A.chunk;
+  const int count = static_cast<int>(min(A.length - j0, static_cast<int64_t>(A.chunk)));
+  const __amdgpu_buffer_rsrc_t kr =
+      make_rsrc(static_cast<const char*>(A.k) + (slice * A.cap + j0) * S::kRow, static_cast<int64_t>(count) * S::kRow);
+  KeyRows<D, DT> cur, nxt;
+  cur.load(kr, wave * 32, lane);
+  __syncthreads();
+  float m[NT], l[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+  }
+  for (int row = wave * 32; row < count; row += kTreeWaves * 32) {
+    nxt.load(kr, row + kTreeWaves * 32, lane);
+    const int left = count - row;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      floatx16 x = {};
+#pragma unroll
+      for (int g = 0; g < S::kPieces; ++g) x = mma_piece<DT>(cur.p[g], s.q[(u * S::kPieces + g) * 64 + lane], x);
+      if (left < 32) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (acc_row(i, h) >= left) x[i] = -INFINITY;
+      }
+      float big = x[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) big = fmaxf(big, x[i]);
+      const float mn = fmaxf(m[u], big * A.scale);
+      const float mr = mn == -INFINITY ? 0.f : mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum += fast_exp2(fmaf(x[i], A.scale, -mr));
+      l[u] = fmaf(l[u], fast_exp2(m[u] - mr), sum);
+      m[u] = mn;
+    }
+    cur = nxt;
+  }
+  // the lane halves hold different keys of the same node; then the waves
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const float mo = __shfl_xor(m[u], 32, 64), lo = __shfl_xor(l[u], 32, 64);
+    const float mn = fmaxf(m[u], mo), mr = mn == -INFINITY ? 0.f : mn;
+    if (h == 0) red[wave][u * kTileNodes + l32] = make_float2(mn, l[u] * fast_exp2(m[u] - mr) + lo * fast_exp2(mo - mr));
+  }
+  __syncthreads();
+  if (t < A.nodes) {
+    float mn = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; ++w) mn = fmaxf(mn, red[w][t].x);
+    const float mr = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; ++w) sum += red[w][t].y * fast_exp2(red[w][t].x - mr);
+    A.part[(slice * (A.nchunk + 1) + blockIdx.x) * A.nodes + t] = make_float2(mn, sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// shares
+
+// B operands of step 2 for the node of this lane's column: 16 bits' worth of
+// 0/1 in bf16, bits 16 s + 8 h + [0, 8) of `mask`
+__device__ __forceinline__ u32x4 bits_frag(uint32_t mask, int s, int h) {
+  const uint32_t b = mask >> (16 * s + 8 * h);
+  u32x4 f;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) f[t] = (b >> (2 * t) & 1 ? 0x3f80u : 0u) | (b >> (2 * t + 1) & 1 ? 0x3f800000u : 0u);
+  return f;
+}
+
+template <int D, int DT, int NT> constexpr int kApplyDV = D == 256 && NT == 2 ? 128 : D;
+
+template <int D, int DT, int NT>
+__global__ __launch_bounds__(kTreeThreads) void tree_apply(Tree A) {
+  using S = Shape<D, DT>;
+  constexpr int DV = kApplyDV<D, DT, NT>;
+  using V = ValueRows<DV, DT>;
+  constexpr int kParts = DT == DT_F32 ? 3 : 2;         // bf16 parts of a bid
+  const int64_t slice = A.slice0 + blockIdx.y;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, h = lane >> 5;
+  constexpr int kRedStride = DV + 1;
+  __shared__ union {
+    u32x4 q[NT * S::kPieces * 64];
+    struct {
+      float t[kTreeMaxNodes][kTreeMaxNodes + 1];
+      float sh[kTreeMaxNodes][kShareStride];
+    } draft;
+    float red[NT * kTileNodes][kRedStride];
+    float2 st[kTreeWaves][kTreeMaxNodes];
+  } s;
+  __shared__ uint64_t seen_s[kTreeMaxNodes];
+  __shared__ float lse_s[kTreeMaxNodes];
+  __shared__ float sum_s[kTreeWaves][NT * kTileNodes];
   const int32_t* parents = A.parents + slice / A.heads * A.parents_sb;
   if (wave == 0) seen_s[lane] = nodes_seen(parents, A.nodes, lane);
-  const int64_t j0 = static_cast<int64_t>(blockIdx.x) * kTreeKeys, j = j0 + t, end = A.length + A.nodes;
-  const int64_t row = (slice * A.cap + (j < end ? j : end - 1)) * D;
-  const float com = j < A.length ? A.committed[slice * A.cap + j] : 0.f;
-  const int64_t qbase = A.qv.slice(slice);
-  const int count = static_cast<int>(end - j0 < kTreeKeys ? end - j0 : kTreeKeys);
-  for (int i = 0; i < A.nodes; ++i) {
+  // the chunks' statistics joined: 64 nodes x 4 groups of entries
+  {
+    float m = -INFINITY, l = 0.f;
+    if (lane < A.nodes) {
+      const float2* part = A.part + slice * (A.nchunk + 1) * A.nodes + lane;
+#pragma unroll 4
+      for (int c = wave; c <= A.nchunk; c += kTreeWaves) {
+        const float2 e = part[static_cast<int64_t>(c) * A.nodes];
+        const float mn = fmaxf(m, e.x), mr = mn == -INFINITY ? 0.f : mn;
+        l = l * fast_exp2(m - mr) + e.y * fast_exp2(e.x - mr);
+        m = mn;
+      }
+    }
+    s.st[wave][lane] = make_float2(m, l);
+  }
+  __syncthreads();
+  if (wave == 0) {
+    float mn = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; ++w) mn = fmaxf(mn, s.st[w][lane].x);
+    const float mr = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; ++w) l += s.st[w][lane].y * fast_exp2(s.st[w][lane].x - mr);
+    // a row of -inf alone has no bids: NaN, as its softmax
+    const float lse = seen_s[lane] == 0 ? INFINITY : mn == -INFINITY ? NAN : mn + fast_log2(l);
+    lse_s[lane] = lse;
+    if (blockIdx.x == 0 && blockIdx.z == 0 && lane < A.nodes) A.lse[slice * A.nodes + lane] = lse;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    if (blockIdx.z == 0) draft_apply<D, DT>(A, slice, s.draft.t, s.draft.sh, seen_s, parents, lse_s);
+    return;
+  }
+  stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return r < A.nodes ? r : -1; });
+  const int64_t j0 = static_cast<int64_t>(blockIdx.x - 1) * A.chunk;
+  const int count = static_cast<int>(min(A.length - j0, static_cast<int64_t>(A.chunk)));
+  const int64_t row_base = (slice * A.cap + j0) * S::kRow, bytes = static_cast<int64_t>(count) * S::kRow;
+  const __amdgpu_buffer_rsrc_t kr = make_rsrc(static_cast<const char*>(A.k) + row_base, bytes);
+  const __amdgpu_buffer_rsrc_t vr = make_rsrc(static_cast<const char*>(A.v) + row_base, bytes);
+  const float* com = A.committed + slice * A.cap + j0;
+  KeyRows<D, DT> cur;
+  cur.load(kr, wave * 32, lane);
+
+  // step 2's operands and the row statistics of step 1's nodes (register i of
+  // half h: node perm_row(i, h))
+  u32x4 anc[NT][NT][2], one[2];
+  float lse[NT][16];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const uint64_t above = seen_s[u * kTileNodes + l32] & ~(uint64_t{1} << (u * kTileNodes + l32));
+#pragma unroll
+    for (int w = 0; w <= u; ++w)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) anc[u][w][st] = bits_frag(static_cast<uint32_t>(above >> (w * kTileNodes)), st, h);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) lse[u][i] = lse_s[u * kTileNodes + perm_row(i, h)];
+  }
+#pragma unroll
+  for (int st = 0; st < 2; ++st) one[st] = bits_frag(uint32_t{1} << l32, st, h);
+  __syncthreads();
+
+  floatx16 acc[NT][V::E];
+  float ssum[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    ssum[u] = 0.f;
+#pragma unroll
+    for (int e = 0; e < V::E; ++e) acc[u][e] = floatx16{};
+  }
+  for (int row = wave * 32; row < count; row += kTreeWaves * 32) {
+    const int left = count - row;
+    V val;
+    val.load(vr, row, lane, S::kRow, static_cast<int>(blockIdx.z) * DV * S::kElt);
+    // committed + eps of this lane's keys in step 2's layout
+    floatx16 c0;
+    if (left >= 32) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c0[4 * g + e] = com[row + 8 * g + 4 * h + e];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) c0[i] = com[min(row + acc_row(i, h), count - 1)];
+    }
+    // step 1
+    u32x4 p[NT][kParts][2];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      floatx16 x = {};
+#pragma unroll
+      for (int g = 0; g < S::kPieces; ++g)
+        x = mma_piece<DT>(s.q[(u * S::kPieces + g) * 64 + h * 32 + rho(l32)], cur.p[g], x);
+      if (left < 32 && l32 >= left) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = -INFINITY;
+      }
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        v[i] = __builtin_amdgcn_fmed3f(fast_exp2(fmaf(x[i], A.scale, -lse[u][i])), 0.f, 1.f);   // NaN becomes 0
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 8 * st + 2 * e;
+            const uint32_t b = pack_bf16(v[i], v[i + 1]);
+            p[u][part][st][e] = b;
+            if (part + 1 < kParts) {
+              v[i] -= __uint_as_float(b << 16);
+              v[i + 1] -= __uint_as_float(b & 0xffff0000u);
+            }
+          }
+      }
+    }
+    cur.load(kr, row + kTreeWaves * 32, lane);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c0[i] += kEps;
+    // steps 2 and 3
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      floatx16 tot = c0, bid = {};
+#pragma unroll
+      for (int part = kParts - 1; part >= 0; --part)
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          bid = mma_piece<DT_BF16>(p[u][part][st], one[st], bid);
+#pragma unroll
+          for (int w = 0; w <= u; ++w) tot = mma_piece<DT_BF16>(p[w][part][st], anc[u][w][st], tot);
+        }
+      float sh[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        sh[i] = bid[i] * fast_rcp(tot[i] + bid[i]);
+        if (left < 32 && acc_row(i, h) >= left) sh[i] = 0.f;
+        ssum[u] += sh[i];
+      }
+      if constexpr (DT == DT_F32) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int e = 0; e < V::E; ++e)
+            acc[u][e] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(val.w[i][e]), sh[i], acc[u][e], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          u32x4 b;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = sh[8 * st + 2 * e], y = sh[8 * st + 2 * e + 1];
+            b[e] = DT == DT_BF16 ? pack_bf16(x, y) : pack_f16(x * kShareScale<DT>, y * kShareScale<DT>);
+          }
+#pragma unroll
+          for (int e = 0; e < V::E; ++e) acc[u][e] = mma_piece<DT>(val.frag(e, st), b, acc[u][e]);
+        }
+      }
+    }
+  }
+  // the waves' sums, in order
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const float o = ssum[u] + __shfl_xor(ssum[u], 32, 64);
+    if (h == 0) sum_s[wave][u * kTileNodes + l32] = o;
+  }
+  for (int w = 0; w < kTreeWaves; ++w) {
     __syncthreads();
-    for (int d = t; d < D; d += kTreeThreads) q_s[d] = elem<DT>(A.q, qbase + i * A.qv.sr + d) * A.scale;
-    __syncthreads();
-    const uint64_t seen = seen_s[i];
-    float* po = A.part_out + ((slice * A.nchunk + blockIdx.x) * A.nodes + i) * (D + 1);
-    if (seen == 0) continue;                       // the whole workgroup: an absent node
-    const bool on = j < end && (j < A.length || (seen >> (j - A.length) & 1));
-    const float p = on ? exp2f(score<D, DT>(q_s, A.k, row) - A.lse[slice * A.nodes + i]) : 0.f;
-    const int par = parents[i];
-    const float tot = (par < 0 ? com : t_s[par][t]) + p;
-    t_s[i][t] = tot;
-    const float sh = on ? p / (tot + kEps) : 0.f;
-    sh_s[t] = on ? sh : -1.f;                      // -1: a key that the node does not see
-    const float s = wave_sum(sh);
-    if (lane == 0) ss[wave] = s;
-    __syncthreads();
-    for (int d = t; d < D; d += kTreeThreads) {
+    if (wave != w) continue;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int e = 0; e < V::E; ++e)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int d = V::E * acc_row(i, h) + e;
+          if (DV >= 32 || d < DV) {
+            float* dst = &s.red[u * kTileNodes + l32][d];
+            *dst = (w == 0 ? 0.f : *dst) + acc[u][e][i];
+          }
+        }
+  }
+  __syncthreads();
+  const int64_t p0 = (slice * (A.nchunk + 1) + blockIdx.x) * A.nodes;
+  constexpr float kUnscale = 1.f / kShareScale<DT>;
+  for (int o = t; o < A.nodes * DV; o += kTreeThreads)
+    A.part_out[(p0 + o / DV) * D + blockIdx.z * DV + o % DV] = s.red[o / DV][o % DV] * kUnscale;
+  if (blockIdx.z == 0 && t < A.nodes) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; ++w) x += sum_s[w][t];
+    A.part_sum[p0 + t] = x;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the chunks' sums joined: one workgroup per node and slice
+
+template <int D, int DT>
+__global__ __launch_bounds__(kTreeThreads) void tree_finish(Tree A) {
+  constexpr int kGroups = kTreeThreads / D;
+  const int64_t slice = A.slice0 + blockIdx.y;
+  const int i = blockIdx.x, t = threadIdx.x, lane = t & 63, d = t % D, g = t / D;
+  __shared__ float red[kGroups][D + 1];
+  const uint64_t seen = shfl64(nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, lane), i);
+  const float own = lane < A.nodes ? A.lse[slice * A.nodes + lane] : 0.f;
+  const bool spoilt = (__ballot(own != own) & seen) != 0;
+  const int64_t p0 = slice * (A.nchunk + 1) * A.nodes + i;
+  float x = 0.f, sum = 0.f;
+  if (seen != 0) {
+#pragma unroll 4
+    for (int c = g; c <= A.nchunk; c += kGroups) {
+      const int64_t at = p0 + static_cast<int64_t>(c) * A.nodes;
+      x += A.part_out[at * D + d];
+      sum += A.part_sum[at];
+    }
+  }
+  red[g][d] = x;
+  if (d == 0) red[g][D] = sum;
+  __syncthreads();
+  if (t >= D) return;
+  x = sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kGroups; ++w) {
+    x += red[w][d];
+    sum += red[w][D];
+  }
+  store_as(A.out, A.ov.slice(slice) + i * A.ov.sr + d, DT, seen == 0 ? 0.f : spoilt ? NAN : x / (sum + kEps));
+}
+
+// ---------------------------------------------------------------------------
+// acceptance: one pass over K with step 1's product alone (a lane holds a key); the
+// first workgroup of a slice sets the accepted positions' demand and moves their
+// rows, all of them into LDS before the first is written.
+
+template <int D, int DT, int NT>
+__global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
+  using S = Shape<D, DT>;
+  constexpr int kUnits = S::kRow / 16;
+  const int64_t slice = A.slice0 + blockIdx.y;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, h = lane >> 5;
+  __shared__ union {
+    u32x4 q[NT * S::kPieces * 64];
+    u32x4 rows[NT * kTileNodes * kUnits];
+    float p[kTreeMaxNodes][kTreeMaxNodes + 1];
+  } s;
+  __shared__ float lse_s[kTreeMaxNodes];
+  __shared__ int node_s[kTreeMaxNodes];
+  if (t < kTreeMaxNodes) {
+    const int a = t < A.count ? A.path[slice / A.heads * A.path_sb + t] : -1;
+    const bool ok = a >= 0 && a < A.nodes;
+    node_s[t] = ok ? a : -1;
+    lse_s[t] = ok ? A.lse[slice * A.nodes + a] : INFINITY;
+  }
+  __syncthreads();
+  float* crow = A.demand + slice * A.cap;
+  if (blockIdx.x == 0) {
+    const int64_t qbase = A.qv.slice(slice), kbase = (slice * A.cap + A.length) * D;
+    for (int o = t; o < A.count * A.count; o += kTreeThreads) {
+      const int r = o / A.count, c = o % A.count;
+      if (c > r) continue;
+      const int i = node_s[r], a = node_s[c];
       float x = 0.f;
-      for (int c = 0; c < count; ++c)
-        if (!(sh_s[c] < 0.f)) x = fmaf(sh_s[c], elem<DT>(A.v, (slice * A.cap + j0 + c) * D + d), x);
-      po[d] = x;
-    }
-    if (t == 0) po[D] = ss[0] + ss[1] + ss[2] + ss[3];
-  }
-}
-
-template <int D, int DT>
-__global__ void tree_finish(Tree A) {
-  const int64_t slice = A.slice0 + blockIdx.y;
-  const int i = blockIdx.x, d = threadIdx.x;
-  const uint64_t seen = nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, d & 63);
-  const int here = __shfl(seen != 0, i, 64);
-  if (d >= D) return;
-  float x = 0.f, s = 0.f;
-  if (here) {
-    for (int c = 0; c < A.nchunk; ++c) {
-      const float* po = A.part_out + ((slice * A.nchunk + c) * A.nodes + i) * (D + 1);
-      x += po[d];
-      s += po[D];
-    }
-    x /= s + kEps;
-  }
-  store_as(A.out, A.ov.slice(slice) + i * A.ov.sr + d, DT, x);
-}
-
-template <int D, int DT>
-__global__ __launch_bounds__(kTreeThreads) void tree_accept_kernel(Tree A, float* committed, void* kc, void* vc,
-                                                                   const int32_t* path, int64_t path_sb, int count) {
-  const int64_t slice = A.slice0 + blockIdx.y;
-  const int t = threadIdx.x;
-  __shared__ float q_s[D];
-  const int32_t* pr = path + slice / A.heads * path_sb;
-  const int64_t qbase = A.qv.slice(slice);
-  float* crow = committed + slice * A.cap;
-  auto stage = [&](int a) {
-    __syncthreads();
-    for (int d = t; d < D; d += kTreeThreads) q_s[d] = elem<DT>(A.q, qbase + a * A.qv.sr + d) * A.scale;
-    __syncthreads();
-  };
-  const bool tail = blockIdx.x == static_cast<unsigned>(A.nchunk);
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * kTreeKeys + t;
-  const int mine = tail && t < count ? pr[t] : -1;
-  const bool drafted = mine >= 0 && mine < A.nodes, cached = !tail && j < A.length;
-  const int64_t row = (slice * A.cap + (tail ? A.length + (drafted ? mine : 0) : (cached ? j : A.length))) * D;
-  float sum = cached ? crow[j] : 0.f;
-  for (int r = 0; r < count; ++r) {
-    const int a = pr[r];
-    if (a < 0 || a >= A.nodes) continue;
-    stage(a);
-    if (cached || (drafted && r >= t)) sum += exp2f(score<D, DT>(q_s, A.k, row) - A.lse[slice * A.nodes + a]);
-  }
-  if (cached) crow[j] = sum;
-  if (!tail) return;
-  if (t < count) crow[A.length + t] = sum;
-  // the rows: all into LDS, then to their places
-  __shared__ uint32_t rows_s[kTreeMaxNodes * 32];
-  constexpr int kWords = D * (DT == DT_F32 ? 4 : 2) / 4, kStep = kWords < 32 ? kWords : 32;
-  for (int w0 = 0; w0 < kWords; w0 += kStep) {
-    for (void* cache : {kc, vc}) {
-      uint32_t* base = static_cast<uint32_t*>(cache) + (slice * A.cap + A.length) * kWords + w0;
-      __syncthreads();
-      for (int u = t; u < count * kStep; u += kTreeThreads) {
-        const int a = pr[u / kStep];
-        if (a >= 0 && a < A.nodes) rows_s[u] = base[static_cast<int64_t>(a) * kWords + u % kStep];
+      if (i >= 0 && a >= 0) {
+        for (int d = 0; d < D; d += 8) {
+          float q[8], k[8];
+          load8_f32(A.q, qbase + i * A.qv.sr + d, DT, q);
+          load8_f32(A.k, kbase + static_cast<int64_t>(a) * D + d, DT, k);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x = fmaf(q[e], k[e], x);
+        }
+        x = fast_exp2(fmaf(x, A.scale, -lse_s[r]));
       }
+      s.p[r][c] = x;
+    }
+    __syncthreads();
+    if (t < A.count) {
+      float x = 0.f;
+      for (int r = t; r < A.count; ++r) x += s.p[r][t];
+      crow[A.length + t] = x;
+    }
+    for (void* cache : {A.k_move, A.v_move}) {
+      u32x4* rows = reinterpret_cast<u32x4*>(static_cast<char*>(cache) + (slice * A.cap + A.length) * S::kRow);
       __syncthreads();
-      for (int u = t; u < count * kStep; u += kTreeThreads) {
-        const int a = pr[u / kStep];
-        if (a >= 0 && a < A.nodes) base[static_cast<int64_t>(u / kStep) * kWords + u % kStep] = rows_s[u];
+      for (int u = t; u < A.count * kUnits; u += kTreeThreads)
+        if (node_s[u / kUnits] >= 0) s.rows[u] = rows[node_s[u / kUnits] * kUnits + u % kUnits];
+      __syncthreads();
+      for (int u = t; u < A.count * kUnits; u += kTreeThreads)
+        if (node_s[u / kUnits] >= 0) rows[u] = s.rows[u];
+    }
+    return;
+  }
+  stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return node_s[r]; });
+  const int64_t j0 = static_cast<int64_t>(blockIdx.x - 1) * A.chunk;
+  const int count = static_cast<int>(min(A.length - j0, static_cast<int64_t>(A.chunk)));
+  const __amdgpu_buffer_rsrc_t kr =
+      make_rsrc(static_cast<const char*>(A.k) + (slice * A.cap + j0) * S::kRow, static_cast<int64_t>(count) * S::kRow);
+  KeyRows<D, DT> cur, nxt;
+  cur.load(kr, wave * 32, lane);
+  float lse[NT][16];
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) lse[u][i] = lse_s[u * kTileNodes + acc_row(i, h)];
+  __syncthreads();
+  for (int row = wave * 32; row < count; row += kTreeWaves * 32) {
+    const int j = row + l32;
+    const float c = j < count ? crow[j0 + j] : 0.f;
+    nxt.load(kr, row + kTreeWaves * 32, lane);
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      floatx16 x = {};
+#pragma unroll
+      for (int g = 0; g < S::kPieces; ++g) x = mma_piece<DT>(s.q[(u * S::kPieces + g) * 64 + lane], cur.p[g], x);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        // rows that are no node have zero queries and lse +inf, and count for nothing whatever k holds
+        const float p = fast_exp2(fmaf(x[i], A.scale, -lse[u][i]));
+        sum += lse[u][i] == INFINITY ? 0.f : p;
       }
     }
+    sum += __shfl_xor(sum, 32, 64);
+    if (h == 0 && j < count) crow[j0 + j] = c + sum;
+    cur = nxt;
   }
 }
 
-int64_t tree_chunks(int64_t length, int64_t nodes) { return (length + nodes + kTreeKeys - 1) / kTreeKeys; }
+// ---------------------------------------------------------------------------
+// launches
+
+// Cached keys of a workgroup.
+int tree_chunk(int64_t n, int64_t length) {
+  constexpr int64_t kTarget = 2048, kMin = 256, kMax = 4096;
+  int64_t per = (kTarget + n - 1) / n;                 // workgroups of a slice
+  int64_t chunk = (length + per - 1) / per;
+  chunk = (chunk + 127) / 128 * 128;
+  return static_cast<int>(chunk < kMin ? kMin : chunk > kMax ? kMax : chunk);
+}
+int64_t tree_chunks(int64_t n, int64_t length) {
+  const int64_t chunk = tree_chunk(n, length);
+  return (length + chunk - 1) / chunk;
+}
 
 Tree tree_of(const TreeArgs& a) {
   Tree A{};
@@ -257,49 +774,74 @@ Tree tree_of(const TreeArgs& a) {
   A.out = a.out;
   A.ov = a.ov;
   A.lse = a.lse;
+  A.chunk = tree_chunk(a.n, a.length);
+  A.nchunk = static_cast<int>(tree_chunks(a.n, a.length));
   A.scale = kLog2e / sqrtf(static_cast<float>(a.head_dim));
   return A;
 }
 
-template <int D, int DT>
+struct TreeScratch {
+  size_t part, out, sum, aff, total;
+  TreeScratch(int64_t n, int64_t length, int64_t nodes, int head_dim) {
+    const size_t rows = static_cast<size_t>(n * (tree_chunks(n, length) + 1) * nodes);
+    part = 0;
+    out = part + align_up(sizeof(float2) * rows);
+    sum = out + align_up(sizeof(float) * rows * head_dim);
+    aff = sum + align_up(sizeof(float) * rows);
+    total = aff + align_up(sizeof(float) * n * nodes * nodes);
+  }
+};
+
+template <int D, int DT, int NT>
 int launch_step(const TreeArgs& a) {
   Tree A = tree_of(a);
-  A.nchunk = static_cast<int>(tree_chunks(a.length, a.nodes));
-  A.part = static_cast<float2*>(a.workspace);
-  A.part_out = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + align_up(sizeof(float2) * a.n * A.nchunk * a.nodes));
+  const TreeScratch w(a.n, a.length, a.nodes, a.head_dim);
+  char* ws = static_cast<char*>(a.workspace);
+  A.part = reinterpret_cast<float2*>(ws + w.part);
+  A.part_out = reinterpret_cast<float*>(ws + w.out);
+  A.part_sum = reinterpret_cast<float*>(ws + w.sum);
+  A.aff = reinterpret_cast<float*>(ws + w.aff);
   hipStream_t st = static_cast<hipStream_t>(a.stream);
+  const unsigned chunks = static_cast<unsigned>(A.nchunk + 1);
   slice_batches(a.n, [&](int64_t s0, unsigned ns) {
     A.slice0 = s0;
-    DIL_TIMED("tree_stats", st, (tree_stats<D, DT><<<dim3(A.nchunk, ns), kTreeThreads, 0, st>>>(A)));
-    DIL_TIMED("tree_lse", st, (tree_lse<<<dim3(ns), 64, 0, st>>>(A)));
-    DIL_TIMED("tree_apply", st, (tree_apply<D, DT><<<dim3(A.nchunk, ns), kTreeThreads, 0, st>>>(A)));
-    DIL_TIMED("tree_finish", st, (tree_finish<D, DT><<<dim3(A.nodes, ns), D < 64 ? 64 : D, 0, st>>>(A)));
+    DIL_TIMED("tree_stats", st, (tree_stats<D, DT, NT><<<dim3(chunks, ns), kTreeThreads, 0, st>>>(A)));
+    DIL_TIMED("tree_apply", st,
+              (tree_apply<D, DT, NT><<<dim3(chunks, ns, D / kApplyDV<D, DT, NT>), kTreeThreads, 0, st>>>(A)));
+    DIL_TIMED("tree_finish", st, (tree_finish<D, DT><<<dim3(A.nodes, ns), kTreeThreads, 0, st>>>(A)));
   });
   return static_cast<int>(hipGetLastError());
 }
 
-template <int D, int DT>
+template <int D, int DT, int NT>
 int launch_accept(const TreeArgs& a) {
   Tree A = tree_of(a);
-  A.nchunk = static_cast<int>((a.length + kTreeKeys - 1) / kTreeKeys);
+  A.demand = a.committed;
+  A.k_move = a.k_cache;
+  A.v_move = a.v_cache;
+  A.path = a.path;
+  A.path_sb = a.path_sb;
+  A.count = a.count;
   hipStream_t st = static_cast<hipStream_t>(a.stream);
   slice_batches(a.n, [&](int64_t s0, unsigned ns) {
     A.slice0 = s0;
-    DIL_TIMED("tree_accept", st,
-              (tree_accept_kernel<D, DT><<<dim3(A.nchunk + 1, ns), kTreeThreads, 0, st>>>(A, a.committed, a.k_cache, a.v_cache,
-                                                                                a.path, a.path_sb, a.count)));
+    DIL_TIMED("tree_demand", st,
+              (tree_demand<D, DT, NT><<<dim3(static_cast<unsigned>(A.nchunk + 1), ns), kTreeThreads, 0, st>>>(A)));
   });
   return static_cast<int>(hipGetLastError());
 }
 
-// f(head dim, dtype) as integral constants
+// f(head dim, dtype, node tiles) as integral constants
 template <typename F>
-int with_shape(int head_dim, int dtype, F&& f) {
+int with_shape(int head_dim, int dtype, int nodes, F&& f) {
+  auto by_nodes = [&](auto d, auto t) {
+    return nodes <= kTileNodes ? f(d, t, std::integral_constant<int, 1>{}) : f(d, t, std::integral_constant<int, 2>{});
+  };
   auto by_dtype = [&](auto d) {
     switch (dtype) {
-      case DT_F32: return f(d, std::integral_constant<int, DT_F32>{});
-      case DT_BF16: return f(d, std::integral_constant<int, DT_BF16>{});
-      case DT_F16: return f(d, std::integral_constant<int, DT_F16>{});
+      case DT_F32: return by_nodes(d, std::integral_constant<int, DT_F32>{});
+      case DT_BF16: return by_nodes(d, std::integral_constant<int, DT_BF16>{});
+      case DT_F16: return by_nodes(d, std::integral_constant<int, DT_F16>{});
       default: return kErrDtype;
     }
   };
@@ -316,17 +858,17 @@ int with_shape(int head_dim, int dtype, F&& f) {
 }  // namespace
 
 int64_t tree_workspace_bytes(int64_t n, int64_t length, int64_t nodes, int head_dim, int dtype) {
-  const int64_t nchunk = tree_chunks(length, nodes);
-  return static_cast<int64_t>(align_up(sizeof(float2) * n * nchunk * nodes) +
-                              align_up(sizeof(float) * n * nchunk * nodes * (head_dim + 1)));
+  (void)dtype;
+  if (n < 1) return 0;
+  return static_cast<int64_t>(TreeScratch(n, length < 0 ? 0 : length, nodes, head_dim).total);
 }
 
 int tree_step(const TreeArgs& a) {
-  return with_shape(a.head_dim, a.dtype, [&](auto d, auto t) { return launch_step<d(), t()>(a); });
+  return with_shape(a.head_dim, a.dtype, a.nodes, [&](auto d, auto t, auto nt) { return launch_step<d(), t(), nt()>(a); });
 }
 
 int tree_accept(const TreeArgs& a) {
-  return with_shape(a.head_dim, a.dtype, [&](auto d, auto t) { return launch_accept<d(), t()>(a); });
+  return with_shape(a.head_dim, a.dtype, a.count, [&](auto d, auto t, auto nt) { return launch_accept<d(), t(), nt()>(a); });
 }
 
 }  // namespace dil
