@@ -18,18 +18,17 @@
 // the queries.  tree_apply's chain keeps every intermediate in the accumulators:
 //   1  S = Q K^T with the nodes as rows, permuted so that a lane (one key) holds
 //      runs of 8 consecutive nodes: p = 2^(S - lse) is then the A operand of
-//   2  t^T = P^T seen^T and p^T = P^T 1 (seen: the 0/1 matrix of the ancestors),
-//      which sum the demand down the tree for all nodes at once and leave a lane
-//      one node and 16 keys.  committed + eps is the accumulator's start value.
-//      p enters as two bf16 parts (16 bits of it, 2^-17), three for fp32 caches.
+//   2  t^T = P^T seen^T and p^T = P^T 1 (seen: the 0/1 matrix of a node's ancestors
+//      and itself), which sum the demand down the tree for all nodes at once and
+//      leave a lane one node and 16 keys.  committed + eps is the accumulator's
+//      start value.
 //   3  the shares, in place, are the B operand of out^T += V^T share^T, whose A
 //      operand takes V rows as loaded, two head dims a register, regrouped by
 //      byte permutes.
 // The drafted keys (at most 64) are a workgroup of their own in plain fp32: there
 // the masks are, and what a node does not see it must not touch (NaN included).
 // A node whose own row statistics are NaN would spoil the others in step 2: its
-// bids are taken as 0 there (the clamp of p to [0, 1] does that), and tree_finish
-// makes it and the nodes below it NaN.
+// bids are taken as 0 there, and tree_finish makes it and the nodes below it NaN.
 #include "dil_tiles.hpp"
 
 namespace dil {
@@ -332,6 +331,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
     l[u] = 0.f;
   }
   for (int row = wave * 32; row < count; row += kTreeWaves * 32) {
+    asm volatile("" ::: "memory");                     // the queries stay in LDS (tree_apply)
     nxt.load(kr, row + kTreeWaves * 32, lane);
     const int left = count - row;
 #pragma unroll
@@ -379,8 +379,14 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
 // ---------------------------------------------------------------------------
 // shares
 
-// B operands of step 2 for the node of this lane's column: 16 bits' worth of
-// 0/1 in bf16, bits 16 s + 8 h + [0, 8) of `mask`
+// How step 2 takes the bids: 16-bit caches two bf16 parts, 16 bits (2^-17, where the
+// shares' rounding makes 2^-9 or 2^-12 next), fp32 caches three, all 24.  bf16 for
+// its range: where no demand has gone yet a share is p / (p + 1e-9), so bids of
+// 1e-9 count, which one fp16 part loses at any scale that holds 1.
+template <int DT> constexpr int kBidParts = DT == DT_F32 ? 3 : 2;
+
+// B operands of step 2 for the node of this lane's column: 0/1 by the bits
+// 16 s + 8 h + [0, 8) of `mask`
 __device__ __forceinline__ u32x4 bits_frag(uint32_t mask, int s, int h) {
   const uint32_t b = mask >> (16 * s + 8 * h);
   u32x4 f;
@@ -391,12 +397,16 @@ __device__ __forceinline__ u32x4 bits_frag(uint32_t mask, int s, int h) {
 
 template <int D, int DT, int NT> constexpr int kApplyDV = D == 256 && NT == 2 ? 128 : D;
 
+// Waves per SIMD that the registers are held to.
 template <int D, int DT, int NT>
-__global__ __launch_bounds__(kTreeThreads) void tree_apply(Tree A) {
+constexpr int kApplyWaves = DT == DT_F32 || D > 128 ? 1 : D == 128 ? 3 - NT : NT == 1 ? 3 : 2;
+
+template <int D, int DT, int NT>
+__global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_apply(Tree A) {
   using S = Shape<D, DT>;
   constexpr int DV = kApplyDV<D, DT, NT>;
   using V = ValueRows<DV, DT>;
-  constexpr int kParts = DT == DT_F32 ? 3 : 2;         // bf16 parts of a bid
+  constexpr int kParts = kBidParts<DT>;
   const int64_t slice = A.slice0 + blockIdx.y;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, h = lane >> 5;
   constexpr int kRedStride = DV + 1;
@@ -410,7 +420,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_apply(Tree A) {
     float2 st[kTreeWaves][kTreeMaxNodes];
   } s;
   __shared__ uint64_t seen_s[kTreeMaxNodes];
-  __shared__ float lse_s[kTreeMaxNodes];
+  __shared__ __attribute__((aligned(16))) float lse_s[kTreeMaxNodes];
   __shared__ float sum_s[kTreeWaves][NT * kTileNodes];
   const int32_t* parents = A.parents + slice / A.heads * A.parents_sb;
   if (wave == 0) seen_s[lane] = nodes_seen(parents, A.nodes, lane);
@@ -457,19 +467,15 @@ __global__ __launch_bounds__(kTreeThreads) void tree_apply(Tree A) {
   KeyRows<D, DT> cur;
   cur.load(kr, wave * 32, lane);
 
-  // step 2's operands and the row statistics of step 1's nodes (register i of
-  // half h: node perm_row(i, h))
+  // step 2's operands (a node sees itself: the sums include its own bid)
   u32x4 anc[NT][NT][2], one[2];
-  float lse[NT][16];
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
-    const uint64_t above = seen_s[u * kTileNodes + l32] & ~(uint64_t{1} << (u * kTileNodes + l32));
+    const uint64_t seen = seen_s[u * kTileNodes + l32];
 #pragma unroll
     for (int w = 0; w <= u; ++w)
 #pragma unroll
-      for (int st = 0; st < 2; ++st) anc[u][w][st] = bits_frag(static_cast<uint32_t>(above >> (w * kTileNodes)), st, h);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) lse[u][i] = lse_s[u * kTileNodes + perm_row(i, h)];
+      for (int st = 0; st < 2; ++st) anc[u][w][st] = bits_frag(static_cast<uint32_t>(seen >> (w * kTileNodes)), st, h);
   }
 #pragma unroll
   for (int st = 0; st < 2; ++st) one[st] = bits_frag(uint32_t{1} << l32, st, h);
@@ -484,6 +490,9 @@ __global__ __launch_bounds__(kTreeThreads) void tree_apply(Tree A) {
     for (int e = 0; e < V::E; ++e) acc[u][e] = floatx16{};
   }
   for (int row = wave * 32; row < count; row += kTreeWaves * 32) {
+    // the queries and row statistics stay in LDS: hoisted out of the loop they cost
+    // a wave per SIMD
+    asm volatile("" ::: "memory");
     const int left = count - row;
     V val;
     val.load(vr, row, lane, S::kRow, static_cast<int>(blockIdx.z) * DV * S::kElt);
@@ -512,9 +521,14 @@ __global__ __launch_bounds__(kTreeThreads) void tree_apply(Tree A) {
         for (int i = 0; i < 16; ++i) x[i] = -INFINITY;
       }
       float v[16];
+      // register i of half h: node perm_row(i, h), two runs of 8
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        v[i] = __builtin_amdgcn_fmed3f(fast_exp2(fmaf(x[i], A.scale, -lse[u][i])), 0.f, 1.f);   // NaN becomes 0
+      for (int g = 0; g < 4; ++g) {
+        const floatx4 lse = *reinterpret_cast<const floatx4*>(&lse_s[u * kTileNodes + 16 * (g >> 1) + 8 * h + 4 * (g & 1)]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)          // NaN (a node without statistics) becomes 0
+          v[4 * g + e] = __builtin_amdgcn_fmed3f(fast_exp2(fmaf(x[4 * g + e], A.scale, -lse[e])), 0.f, 1.f);
+      }
 #pragma unroll
       for (int part = 0; part < kParts; ++part) {
 #pragma unroll
@@ -549,7 +563,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_apply(Tree A) {
       float sh[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        sh[i] = bid[i] * fast_rcp(tot[i] + bid[i]);
+        sh[i] = bid[i] * fast_rcp(tot[i]);
         if (left < 32 && acc_row(i, h) >= left) sh[i] = 0.f;
         ssum[u] += sh[i];
       }
@@ -720,6 +734,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
     for (int i = 0; i < 16; ++i) lse[u][i] = lse_s[u * kTileNodes + acc_row(i, h)];
   __syncthreads();
   for (int row = wave * 32; row < count; row += kTreeWaves * 32) {
+    asm volatile("" ::: "memory");                     // the queries stay in LDS (tree_apply)
     const int j = row + l32;
     const float c = j < count ? crow[j0 + j] : 0.f;
     nxt.load(kr, row + kTreeWaves * 32, lane);
