@@ -2,7 +2,15 @@
 // cached keys the first `first`, the last `recent` and the most demanded of those
 // between move to a new cache, in their order.
 //
-//   evict_select  (slices)              the positions kept
+// The want-th largest demand of a slice is found digit by digit (11, 11 and 10 bits
+// of an integer that orders as the demand does): the counts of the keys that share
+// the digits found so far, summed from the top digit down.  Above it every key stays,
+// and of its equals the first that are wanted.
+//
+//   evict_select  (slices)              up to 32768 keys between: the slice in one
+//                                       workgroup, its keys in registers
+//   evict_digit   (chunks x slices)     longer: four launches, each of them reads the
+//                                       demand once; a chunk's counts go through memory
 //   evict_move    (row blocks x slices) K, V and demand rows to their places, zero
 //                                       past the last
 #include "dil_common.hpp"
@@ -22,119 +30,349 @@ __device__ __forceinline__ uint32_t demand_key(float x) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// The w-th largest key of [j0, j1) is found a byte at a time (the counts of the
-// keys that share the bytes found so far), then the kept positions are written in
-// order: all above it, and as many of its equals, lowest first, as are wanted.
-__global__ __launch_bounds__(kSelThreads) void evict_select(const float* __restrict__ committed, int64_t cap, int64_t length,
-                                                            int64_t keep, int64_t first, int64_t recent,
-                                                            int32_t* __restrict__ index) {
+constexpr int kWaves = kSelThreads / 64;
+constexpr int kBins = 2048;
+// digit `level` of a key: bits [shift, shift + width)
+__host__ __device__ constexpr int digit_shift(int level) { return level == 0 ? 21 : level == 1 ? 10 : 0; }
+__host__ __device__ constexpr uint32_t digit_mask(int level) { return level == 2 ? 1023u : 2047u; }
+
+// One bin's place: the counts of thread t's two bins (2 t and 2 t + 1), with the
+// counts of the higher bins before them.
+struct Found {
+  int bin, left;                  // the bin that holds the want-th largest, and how many of it are wanted
+};
+// Every thread of the workgroup calls.
+__device__ __forceinline__ Found find_bin(int h0, int h1, int want, int* scratch) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const float* row = committed + static_cast<int64_t>(blockIdx.x) * cap;
-  int32_t* dst = index + static_cast<int64_t>(blockIdx.x) * keep;
-  const int64_t j1 = length - recent;
-  __shared__ int hist[256];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_want;
-  __shared__ int cnt[2][kSelThreads / 64];
-  uint32_t prefix = 0, mask = 0;
-  int want = static_cast<int>(keep - first - recent);
-  for (int64_t j = t; j < first; j += kSelThreads) dst[j] = static_cast<int32_t>(j);
-  for (int64_t j = t; j < recent; j += kSelThreads) dst[keep - recent + j] = static_cast<int32_t>(j1 + j);
-  if (want == 0) return;                        // the same in every thread
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (t < 256) hist[t] = 0;
-    __syncthreads();
-    for (int64_t j = first + t; j < j1; j += kSelThreads) {
-      const uint32_t k = demand_key(row[j]);
-      if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & 255], 1);
-    }
-    __syncthreads();
-    if (t == 0) {
-      int left = want, b = 255;
-      while (b > 0 && hist[b] < left) left -= hist[b--];
-      s_prefix = prefix | static_cast<uint32_t>(b) << shift;
-      s_want = left;
-    }
-    __syncthreads();
-    prefix = s_prefix;
-    want = s_want;
-    mask |= 0xffu << shift;
+  int suffix = h0 + h1;           // over the lanes from this one on
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_down(suffix, o, 64);
+    if (lane + o < 64) suffix += x;
   }
-  // want: how many keys equal to the threshold `prefix` stay
-  int ties = 0;
-  int64_t at = first;
-  for (int64_t b = first; b < j1; b += kSelThreads) {
-    const int64_t j = b + t;
-    const uint32_t k = j < j1 ? demand_key(row[j]) : 0;
-    const bool above = j < j1 && k > prefix, equal = j < j1 && k == prefix;
-    const uint64_t ma = __ballot(above), me = __ballot(equal);
-    const uint64_t below = (uint64_t{1} << lane) - 1;
-    __syncthreads();                            // the counts of the round before are read
-    if (lane == 0) {
-      cnt[0][wave] = __popcll(ma);
-      cnt[1][wave] = __popcll(me);
-    }
-    __syncthreads();
-    int a0 = 0, e0 = 0, at_all = 0, e_all = 0;
-    for (int w = 0; w < kSelThreads / 64; ++w) {
-      if (w < wave) {
-        a0 += cnt[0][w];
-        e0 += cnt[1][w];
+  __syncthreads();
+  if (lane == 0) scratch[wave] = suffix;
+  __syncthreads();
+  int above = suffix - h0 - h1;
+  for (int w = wave + 1; w < kWaves; ++w) above += scratch[w];
+  if (above < want && want <= above + h1) {
+    scratch[kWaves] = 2 * t + 1;
+    scratch[kWaves + 1] = want - above;
+  } else if (above + h1 < want && want <= above + h1 + h0) {
+    scratch[kWaves] = 2 * t;
+    scratch[kWaves + 1] = want - above - h1;
+  }
+  __syncthreads();
+  return {scratch[kWaves], scratch[kWaves + 1]};
+}
+
+// The kept positions of one block of keys, in order.  Key e of thread t is position
+// j0 + e * 1024 + t; `ties` equals came before the block, and its first kept
+// position is number `at`.  Both move past the block.
+template <int E>
+__device__ __forceinline__ void emit_kept(const uint32_t (&key)[E], int64_t j0, int64_t j1, uint32_t least, int want,
+                                          int& ties, int64_t& at, int32_t* dst, int2 (*cnt)[kWaves], int2* total) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const uint64_t below = (uint64_t{1} << lane) - 1;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool in = j0 + e * kSelThreads + t < j1;
+    const uint64_t ma = __ballot(in && key[e] > least), me = __ballot(in && key[e] == least);
+    if (lane == 0) cnt[e][wave] = make_int2(__popcll(ma), __popcll(me));
+  }
+  __syncthreads();
+  if (wave == 0) {                 // exclusive sums over the (e, wave) runs, in order
+    int2 run = make_int2(0, 0);
+    for (int b = 0; b < E * kWaves; b += 64) {
+      int2* c = &cnt[0][0] + b + lane;
+      const bool in = b + lane < E * kWaves;
+      const int2 mine = in ? *c : make_int2(0, 0);
+      int2 x = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int xa = __shfl_up(x.x, o, 64), xe = __shfl_up(x.y, o, 64);
+        if (lane >= o) {
+          x.x += xa;
+          x.y += xe;
+        }
       }
-      at_all += cnt[0][w];
-      e_all += cnt[1][w];
+      if (in) *c = make_int2(run.x + x.x - mine.x, run.y + x.y - mine.y);
+      run.x += __shfl(x.x, 63, 64);
+      run.y += __shfl(x.y, 63, 64);
     }
-    const int eq_before = ties + e0 + __popcll(me & below);   // equals at lower positions
-    const int64_t place = at + a0 + __popcll(ma & below) + (min(eq_before, want) - min(ties, want));
-    if (above || (equal && eq_before < want)) dst[place] = static_cast<int32_t>(j);
-    at += at_all + min(ties + e_all, want) - min(ties, want);
-    ties += e_all;
+    if (lane == 0) *total = run;
+  }
+  __syncthreads();
+  const int taken = min(ties, want);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int64_t j = j0 + e * kSelThreads + t;
+    const bool in = j < j1, above = in && key[e] > least, equal = in && key[e] == least;
+    const uint64_t ma = __ballot(above), me = __ballot(equal);
+    const int2 c = cnt[e][wave];
+    const int rank = ties + c.y + __popcll(me & below);          // equals at lower positions
+    if (above || (equal && rank < want)) dst[at + c.x + __popcll(ma & below) + min(rank, want) - taken] = static_cast<int32_t>(j);
+  }
+  at += total->x + min(ties + total->y, want) - taken;
+  ties += total->y;
+}
+
+// The positions that stay whatever they carry.
+__device__ __forceinline__ void emit_ends(int32_t* dst, int64_t length, int64_t keep, int64_t first, int64_t recent) {
+  for (int64_t j = threadIdx.x; j < first; j += kSelThreads) dst[j] = static_cast<int32_t>(j);
+  for (int64_t j = threadIdx.x; j < recent; j += kSelThreads) dst[keep - recent + j] = static_cast<int32_t>(length - recent + j);
+}
+
+struct Select {
+  const float* committed;
+  int64_t cap, length, keep, first, recent;
+  int32_t* index;
+  int64_t slice0;
+  // the chunked form
+  int64_t chunk;
+  int chunks;
+  int* hist;                       // (3 levels, n, chunks, kBins)
+  int64_t level_stride;
+  int4* state;                     // (n): after level k the digits found so far, and how many equals are wanted
+  int* before;                     // (n, chunks): keys above the digits found so far in the chunks before
+};
+
+template <int E>
+__device__ __forceinline__ void load_keys(uint32_t (&key)[E], const float* row, int64_t j0, int64_t j1) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int64_t j = j0 + e * kSelThreads + threadIdx.x;
+    key[e] = demand_key(row[j < j1 ? j : j1 - 1]);
   }
 }
+
+// The slice in one workgroup: 1024 E keys at most.
+template <int E>
+__global__ __launch_bounds__(kSelThreads) void evict_select(Select A) {
+  __shared__ int hist[kBins];
+  __shared__ int scratch[kWaves + 2];
+  __shared__ int2 cnt[E][kWaves], total;
+  const int t = threadIdx.x;
+  const int64_t slice = A.slice0 + blockIdx.x;
+  int32_t* dst = A.index + slice * A.keep;
+  const int64_t j0 = A.first, j1 = A.length - A.recent;
+  int want = static_cast<int>(A.keep - A.first - A.recent);
+  emit_ends(dst, A.length, A.keep, A.first, A.recent);
+  if (want == 0) return;                        // the same in every thread
+  uint32_t key[E];
+  load_keys(key, A.committed + slice * A.cap, j0, j1);
+  uint32_t digits = 0, mask = 0;
+#pragma unroll
+  for (int level = 0; level < 3; ++level) {
+    hist[t] = hist[t + kSelThreads] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (j0 + e * kSelThreads + t < j1 && (key[e] & mask) == digits)
+        atomicAdd(&hist[key[e] >> digit_shift(level) & digit_mask(level)], 1);
+    __syncthreads();
+    const Found f = find_bin(hist[2 * t], hist[2 * t + 1], want, scratch);
+    digits |= static_cast<uint32_t>(f.bin) << digit_shift(level);
+    mask |= digit_mask(level) << digit_shift(level);
+    want = f.left;
+  }
+  int ties = 0;
+  int64_t at = A.first;
+  emit_kept<E>(key, j0, j1, digits, want, ties, at, dst, cnt, &total);
+}
+
+constexpr int kChunkKeys = 16;     // per thread and block
+
+// Level LEVEL of the chunked form: the digit of level LEVEL - 1 from its counts, then
+// the counts of the next digit; the last writes the positions.
+template <int LEVEL>
+__global__ __launch_bounds__(kSelThreads) void evict_digit(Select A) {
+  __shared__ int hist[kBins];
+  __shared__ int scratch[kWaves + 2];
+  __shared__ int2 cnt[kChunkKeys][kWaves], total;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int c = blockIdx.x;
+  const int64_t slice = A.slice0 + blockIdx.y;
+  const int64_t end = A.length - A.recent;
+  const int64_t j0 = A.first + c * A.chunk, j1 = min(j0 + A.chunk, end);
+  uint32_t digits = 0;
+  int want = static_cast<int>(A.keep - A.first - A.recent);
+  int before = 0, ties = 0;                     // keys above the threshold, and equal to it, in the chunks before
+  if constexpr (LEVEL > 0) {
+    if constexpr (LEVEL > 1) {
+      const int4 s = A.state[slice * 2 + (LEVEL - 2)];
+      digits = static_cast<uint32_t>(s.x);
+      want = s.y;
+      before = A.before[(slice * 2 + LEVEL - 2) * A.chunks + c];
+    }
+    const int* h = A.hist + (LEVEL - 1) * A.level_stride + slice * A.chunks * kBins + 2 * t;
+    int all0 = 0, all1 = 0, pre0 = 0, pre1 = 0;
+#pragma unroll 4
+    for (int i = 0; i < A.chunks; ++i) {
+      const int2 x = *reinterpret_cast<const int2*>(h + static_cast<int64_t>(i) * kBins);
+      all0 += x.x;
+      all1 += x.y;
+      pre0 += i < c ? x.x : 0;
+      pre1 += i < c ? x.y : 0;
+    }
+    const Found f = find_bin(all0, all1, want, scratch);
+    digits |= static_cast<uint32_t>(f.bin) << digit_shift(LEVEL - 1);
+    want = f.left;
+    int up = (2 * t > f.bin ? pre0 : 0) + (2 * t + 1 > f.bin ? pre1 : 0);
+    int eq = (2 * t == f.bin ? pre0 : 0) + (2 * t + 1 == f.bin ? pre1 : 0);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      up += __shfl_xor(up, o, 64);
+      eq += __shfl_xor(eq, o, 64);
+    }
+    if (lane == 0) cnt[0][wave] = make_int2(up, eq);
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) {
+      before += cnt[0][w].x;
+      ties += cnt[0][w].y;
+    }
+    if (LEVEL < 3 && t == 0) {
+      A.before[(slice * 2 + LEVEL - 1) * A.chunks + c] = before;
+      if (c == 0) A.state[slice * 2 + LEVEL - 1] = make_int4(static_cast<int>(digits), want, 0, 0);
+    }
+  }
+  const float* row = A.committed + slice * A.cap;
+  if constexpr (LEVEL < 3) {
+    constexpr uint32_t kFoundMask = LEVEL == 0 ? 0u : LEVEL == 1 ? ~0u << 21 : ~0u << 10;
+    hist[t] = hist[t + kSelThreads] = 0;
+    __syncthreads();
+    for (int64_t b = j0; b < j1; b += kChunkKeys * kSelThreads) {
+      uint32_t key[kChunkKeys];
+      load_keys(key, row, b, j1);
+#pragma unroll
+      for (int e = 0; e < kChunkKeys; ++e)
+        if (b + e * kSelThreads + t < j1 && (key[e] & kFoundMask) == digits)
+          atomicAdd(&hist[key[e] >> digit_shift(LEVEL) & digit_mask(LEVEL)], 1);
+    }
+    __syncthreads();
+    int* h = A.hist + LEVEL * A.level_stride + (slice * A.chunks + c) * kBins;
+    h[t] = hist[t];
+    h[t + kSelThreads] = hist[t + kSelThreads];
+  } else {
+    int32_t* dst = A.index + slice * A.keep;
+    if (c == 0) emit_ends(dst, A.length, A.keep, A.first, A.recent);
+    int64_t at = A.first + before + min(ties, want);
+    for (int64_t b = j0; b < j1; b += kChunkKeys * kSelThreads) {
+      uint32_t key[kChunkKeys];
+      load_keys(key, row, b, j1);
+      emit_kept<kChunkKeys>(key, b, j1, digits, want, ties, at, dst, cnt, &total);
+    }
+  }
+}
+
+// 16-byte units of the output slice, kMoveUnits a thread (K and V of all of them in
+// flight); a row is 2^shift units.
+constexpr int kMoveUnits = 4;
 
 __global__ __launch_bounds__(kMoveThreads) void evict_move(const u32x4* __restrict__ k, const u32x4* __restrict__ v,
                                                            const float* __restrict__ committed, int64_t cap,
                                                            const int32_t* __restrict__ index, int64_t keep, int64_t out_cap,
-                                                           int units, u32x4* __restrict__ ko, u32x4* __restrict__ vo,
+                                                           int shift, u32x4* __restrict__ ko, u32x4* __restrict__ vo,
                                                            float* __restrict__ co, int64_t slice0) {
-  const int64_t slice = slice0 + blockIdx.y;
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * kMoveThreads + threadIdx.x;   // 16-byte unit of the output slice
-  const int64_t r = u / units;
-  if (r >= out_cap) return;
-  const int64_t c = u - r * units;
-  const int64_t to = (slice * out_cap + r) * units + c;
-  if (r < keep) {
-    const int64_t src = slice * cap + index[slice * keep + r];
-    ko[to] = k[src * units + c];
-    vo[to] = v[src * units + c];
-    if (c == 0) co[slice * out_cap + r] = committed[src];
-  } else {
-    ko[to] = vo[to] = u32x4{0, 0, 0, 0};
-    if (c == 0) co[slice * out_cap + r] = 0.f;
+  const int64_t slice = slice0 + blockIdx.y, units = out_cap << shift;
+  const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (kMoveThreads * kMoveUnits) + threadIdx.x;
+  const int part = (1 << shift) - 1;
+  u32x4 x[kMoveUnits], y[kMoveUnits];
+  float c[kMoveUnits];
+#pragma unroll
+  for (int i = 0; i < kMoveUnits; ++i) {
+    const int64_t u = u0 + i * kMoveThreads, r = u >> shift;
+    x[i] = y[i] = u32x4{0, 0, 0, 0};
+    c[i] = 0.f;
+    if (r < keep) {
+      const int64_t row = slice * cap + index[slice * keep + r], src = (row << shift) + (u & part);
+      x[i] = k[src];
+      y[i] = v[src];
+      if ((u & part) == 0) c[i] = committed[row];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kMoveUnits; ++i) {
+    const int64_t u = u0 + i * kMoveThreads;
+    if (u >= units) return;
+    const int64_t to = slice * units + u;
+    ko[to] = x[i];
+    vo[to] = y[i];
+    if ((u & part) == 0) co[slice * out_cap + (u >> shift)] = c[i];
   }
 }
 
 }  // namespace
 
+namespace {
+
+constexpr int64_t kOneMax = 32 * kSelThreads;            // keys that one workgroup holds
+constexpr int64_t kMaxChunks = 64;
+
+// The chunked form's chunks: of 16384 keys, longer ones where that makes more than 64.
+int64_t chunk_of(int64_t keys) {
+  const int64_t block = kChunkKeys * kSelThreads, per = (keys + kMaxChunks - 1) / kMaxChunks;
+  return (per + block - 1) / block * block;
+}
+// Places for the most chunks that any first and recent leave of `length` keys: by the
+// length alone, as the workspace's size.
+struct EvictScratch {
+  size_t hist, state, before, total;
+  EvictScratch(int64_t n, int64_t length) {
+    const int64_t blocks = (length + kChunkKeys * kSelThreads - 1) / (kChunkKeys * kSelThreads);
+    const int64_t chunks = length <= kOneMax ? 0 : blocks < kMaxChunks ? blocks : kMaxChunks;
+    hist = 0;
+    state = hist + align_up(sizeof(int) * 3 * n * chunks * kBins);
+    before = state + align_up(sizeof(int4) * 2 * n * (chunks != 0));
+    total = before + align_up(sizeof(int) * 2 * n * chunks);
+  }
+};
+
+}  // namespace
+
 int64_t evict_workspace_bytes(int64_t n, int64_t length, int64_t keep) {
-  (void)n;
-  (void)length;
   (void)keep;
-  return 256;
+  return n < 1 || length < 1 ? 0 : static_cast<int64_t>(EvictScratch(n, length).total) + 256;
 }
 
 int evict(const EvictArgs& a) {
   hipStream_t st = static_cast<hipStream_t>(a.stream);
-  DIL_TIMED("evict_select", st,
-            (evict_select<<<dim3(static_cast<unsigned>(a.n)), kSelThreads, 0, st>>>(a.committed, a.cap, a.length, a.keep, a.first,
-                                                                           a.recent, a.index)));
-  const int units = a.head_dim * (a.dtype == DT_F32 ? 4 : 2) / 16;
-  const int64_t blocks = (a.out_cap * units + kMoveThreads - 1) / kMoveThreads;
+  const int64_t keys = a.length - a.first - a.recent;
+  Select S{a.committed, a.cap, a.length, a.keep, a.first, a.recent, a.index, 0, 0, 0, nullptr, 0, nullptr, nullptr};
+  if (keys <= kOneMax || a.keep == a.first + a.recent) {
+    const unsigned n = static_cast<unsigned>(a.n);
+    auto one = [&](auto e) { DIL_TIMED("evict_select", st, (evict_select<e()><<<dim3(n), kSelThreads, 0, st>>>(S))); };
+    if (keys <= 4 * kSelThreads || a.keep == a.first + a.recent) one(std::integral_constant<int, 4>{});
+    else if (keys <= 8 * kSelThreads) one(std::integral_constant<int, 8>{});
+    else if (keys <= 16 * kSelThreads) one(std::integral_constant<int, 16>{});
+    else one(std::integral_constant<int, 32>{});
+  } else {
+    const EvictScratch w(a.n, a.length);
+    char* ws = static_cast<char*>(a.workspace);
+    S.chunk = chunk_of(keys);
+    S.chunks = static_cast<int>((keys + S.chunk - 1) / S.chunk);
+    S.hist = reinterpret_cast<int*>(ws + w.hist);
+    S.level_stride = a.n * S.chunks * kBins;
+    S.state = reinterpret_cast<int4*>(ws + w.state);
+    S.before = reinterpret_cast<int*>(ws + w.before);
+    slice_batches(a.n, [&](int64_t s0, unsigned ns) {
+      S.slice0 = s0;
+      const dim3 grid(static_cast<unsigned>(S.chunks), ns);
+      DIL_TIMED("evict_digit0", st, (evict_digit<0><<<grid, kSelThreads, 0, st>>>(S)));
+      DIL_TIMED("evict_digit1", st, (evict_digit<1><<<grid, kSelThreads, 0, st>>>(S)));
+      DIL_TIMED("evict_digit2", st, (evict_digit<2><<<grid, kSelThreads, 0, st>>>(S)));
+      DIL_TIMED("evict_digit3", st, (evict_digit<3><<<grid, kSelThreads, 0, st>>>(S)));
+    });
+  }
+  int shift = 0;                                           // head_dim is a power of two
+  while (16 << shift < a.head_dim * (a.dtype == DT_F32 ? 4 : 2)) ++shift;
+  const int64_t blocks = ((a.out_cap << shift) + kMoveThreads * kMoveUnits - 1) / (kMoveThreads * kMoveUnits);
   slice_batches(a.n, [&](int64_t s0, unsigned ns) {
     DIL_TIMED("evict_move", st,
               (evict_move<<<dim3(static_cast<unsigned>(blocks), ns), kMoveThreads, 0, st>>>(
                   static_cast<const u32x4*>(a.k_cache), static_cast<const u32x4*>(a.v_cache), a.committed, a.cap, a.index, a.keep,
-                  a.out_cap, units, static_cast<u32x4*>(a.k_out), static_cast<u32x4*>(a.v_out), a.committed_out, s0)));
+                  a.out_cap, shift, static_cast<u32x4*>(a.k_out), static_cast<u32x4*>(a.v_out), a.committed_out, s0)));
   });
   return static_cast<int>(hipGetLastError());
 }

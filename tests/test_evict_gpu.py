@@ -58,6 +58,12 @@ SHAPES = [
     (2, 1, 20000, 16385, 16384, 0, 0, None, 256, F32),
     (1, 2, 70000, 66001, 30007, 5, 1003, 30100, 64, BF16),
     (1, 1, 200003, 200003, 100001, 7, 0, None, 16, BF16),
+    (1, 2, 32768, 32768, 9000, 0, 0, None, 16, BF16),          # the most keys of one workgroup, and one more
+    (1, 2, 32769, 32769, 9000, 0, 0, None, 16, BF16),
+    (1, 1, 1048600, 1048600, 400000, 6, 18, None, 16, BF16),   # 64 full chunks between, of a length that takes fewer
+    (1, 1, 1100000, 1100000, 700001, 0, 0, None, 16, BF16),    # chunks of two blocks
+    (1, 2, 50000, 50000, 50000, 0, 0, None, 16, BF16),
+    (1, 2, 50000, 50000, 40, 20, 20, None, 16, BF16),
     (16, 16, 3000, 2999, 1000, 4, 100, 1064, 64, BF16),
 ]
 
