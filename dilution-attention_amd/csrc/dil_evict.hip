@@ -66,6 +66,22 @@ __device__ __forceinline__ Found find_bin(int h0, int h1, int want, int* scratch
   return {scratch[kWaves], scratch[kWaves + 1]};
 }
 
+// Counts a key's digit.  The lanes that have the first counting lane's digit count
+// as one: demands crowd into few digits (all of them where many keys hold none), and
+// equal addresses of a wave's atomics take turns.
+__device__ __forceinline__ void count_digit(int* hist, uint32_t digit, bool on) {
+  const uint64_t active = __ballot(on);
+  if (active == 0) return;
+  const int lead = __ffsll(static_cast<unsigned long long>(active)) - 1;
+  const bool same = on && digit == static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(digit), lead));
+  const uint64_t with = __ballot(same);
+  if (same) {
+    if ((threadIdx.x & 63) == lead) atomicAdd(&hist[digit], __popcll(with));
+  } else if (on) {
+    atomicAdd(&hist[digit], 1);
+  }
+}
+
 // The kept positions of one block of keys, in order.  Key e of thread t is position
 // j0 + e * 1024 + t; `ties` equals came before the block, and its first kept
 // position is number `at`.  Both move past the block.
@@ -169,8 +185,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select(Select A) {
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (j0 + e * kSelThreads + t < j1 && (key[e] & mask) == digits)
-        atomicAdd(&hist[key[e] >> digit_shift(level) & digit_mask(level)], 1);
+      count_digit(hist, key[e] >> digit_shift(level) & digit_mask(level),
+                  j0 + e * kSelThreads + t < j1 && (key[e] & mask) == digits);
     __syncthreads();
     const Found f = find_bin(hist[2 * t], hist[2 * t + 1], want, scratch);
     digits |= static_cast<uint32_t>(f.bin) << digit_shift(level);
@@ -247,8 +263,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_digit(Select A) {
       load_keys(key, row, b, j1);
 #pragma unroll
       for (int e = 0; e < kChunkKeys; ++e)
-        if (b + e * kSelThreads + t < j1 && (key[e] & kFoundMask) == digits)
-          atomicAdd(&hist[key[e] >> digit_shift(LEVEL) & digit_mask(LEVEL)], 1);
+        count_digit(hist, key[e] >> digit_shift(LEVEL) & digit_mask(LEVEL),
+                    b + e * kSelThreads + t < j1 && (key[e] & kFoundMask) == digits);
     }
     __syncthreads();
     int* h = A.hist + LEVEL * A.level_stride + (slice * A.chunks + c) * kBins;

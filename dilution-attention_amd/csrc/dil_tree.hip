@@ -107,12 +107,12 @@ struct Tree {
   void* out;
   RowsView ov;
   float* lse;
-  float2* part;              // (n, nchunk + 1, nodes): entry 0 of a slice is the drafted keys'
+  float2* part;              // (n, nstat + 1, nodes): entry 0 of a slice is the drafted keys'
   float* part_out;           // (n, nchunk + 1, nodes, D)
   float* part_sum;           // (n, nchunk + 1, nodes)
   float* aff;                // (n, nodes, nodes): the drafted keys' affinities
-  int nchunk;
-  int chunk;                 // cached keys of a workgroup, a multiple of 32
+  uint64_t* seen;            // (n, 64): nodes_seen, for the launches after the first
+  int nstat, nchunk;         // workgroups of a slice over its cached keys: the statistics, and the shares (or the acceptance)
   float scale;
   int64_t slice0;
   // the acceptance
@@ -146,14 +146,36 @@ __device__ __forceinline__ void stage_queries(u32x4* q_s, const Tree& A, int64_t
   }
 }
 
-// 32 rows of a chunk, one per lane (l & 31): rows past the resource's end read 0.
-// The row offset is part of the per-lane offset: the range check of a buffer load
-// covers that one.
+// Workgroup c of a slice's `chunks` takes the blocks of 128 rows c, c + chunks, ...,
+// its waves 32 rows each: the GPU reads one stretch of every slice at a time.  (With
+// a stretch of its own for every workgroup the statistics of 128 slices of 65536 keys
+// took 193 to 235 us by the stretch's length.)  All uniform in a wave.
+constexpr int kBlockRows = kTreeWaves * 32;
+
+// The resource over the 32 rows from `row` on, as far as they exist: rows past the end
+// read 0.  Offsets within it are per lane alone, which the range check covers.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char* base, int64_t row, int64_t length, int rowbytes) {
+  const int64_t left = length - row;
+  const int n = left < 0 ? 0 : left < 32 ? static_cast<int>(left) : 32;
+  const uint64_t a = reinterpret_cast<uint64_t>(base) + static_cast<uint64_t>(row) * static_cast<uint32_t>(rowbytes);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((static_cast<uint64_t>(hi) << 32) | lo), 0,
+                                           __builtin_amdgcn_readfirstlane(n * rowbytes), 0x00020000);
+}
+
+// The constants that a load adds to `off` stay with the load, as its immediate offset:
+// hoisted out of the loop over `row` each of them is a register.
+__device__ __forceinline__ void keep_in_loop(uint32_t& off, int64_t row) { asm("" : "+v"(off) : "s"(row)); }
+
+// 32 rows, one per lane (l & 31).
 template <int D, int DT>
 struct KeyRows {
   u32x4 p[Shape<D, DT>::kPieces];
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int row0, int lane) {
-    const uint32_t off = static_cast<uint32_t>(row0 + (lane & 31)) * Shape<D, DT>::kRow + (lane >> 5) * 16u;
+  __device__ __forceinline__ void load(const char* base, int64_t row, int64_t length, int lane) {
+    const __amdgpu_buffer_rsrc_t r = rows_at(base, row, length, Shape<D, DT>::kRow);
+    uint32_t off = static_cast<uint32_t>(lane & 31) * Shape<D, DT>::kRow + (lane >> 5) * 16u;
+    keep_in_loop(off, row);
 #pragma unroll
     for (int g = 0; g < Shape<D, DT>::kPieces; ++g)
       p[g] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 32u * g, 0, 0));
@@ -163,34 +185,38 @@ struct KeyRows {
 // 32 V rows as A operands of V^T: lane (d, h) of instruction step s, slot t holds key
 // 16 s + 8 (t >> 2) + 4 h + (t & 3) (fp32: register i, key acc_row(i, h)).  A lane
 // loads E = DV / 32 consecutive head dims of a row: row u of operand tile e is head
-// dim E * u + e.
+// dim E * u + e.  Read once, past the caches (the K rows of the pass before stay there:
+// 8% of tree_apply at 128 slices of 16384 keys).
+constexpr int kOnce = 2;                               // the non-temporal hint of a buffer load
 template <int DV, int DT>
 struct ValueRows {
   static constexpr int E = DV < 32 ? 1 : DV / 32;
   static constexpr int kBytes = E * (DT == DT_F32 ? 4 : 2);   // per lane and row: 2 to 32
   static constexpr int kWords = kBytes < 4 ? 1 : kBytes / 4;
   uint32_t w[16][kWords];
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int row0, int lane, int rowbytes, int d0bytes) {
+  __device__ __forceinline__ void load(const char* base, int64_t row, int64_t length, int lane, int rowbytes, int d0bytes) {
+    const __amdgpu_buffer_rsrc_t r = rows_at(base, row, length, rowbytes);
     const int l32 = lane & 31, h = lane >> 5;
-    uint32_t off = static_cast<uint32_t>(row0 + 4 * h) * rowbytes + d0bytes + l32 * kBytes;
+    uint32_t off = static_cast<uint32_t>(4 * h) * rowbytes + d0bytes + l32 * kBytes;
     if constexpr (DV < 32) {
       if (l32 >= DV) off = 0xf0000000u;              // past the end: zeros
     }
+    keep_in_loop(off, row);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const uint32_t o = off + static_cast<uint32_t>(8 * (i >> 2) + (i & 3)) * rowbytes;
       if constexpr (kBytes == 2) {
-        w[i][0] = __builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0);
+        w[i][0] = __builtin_amdgcn_raw_buffer_load_b16(r, o, 0, kOnce);
       } else if constexpr (kBytes == 4) {
-        w[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+        w[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, kOnce);
       } else if constexpr (kBytes == 8) {
-        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0));
+        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, kOnce));
         w[i][0] = x[0];
         w[i][1] = x[1];
       } else {
 #pragma unroll
         for (int c = 0; c < kBytes / 16; ++c) {
-          const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o + 16u * c, 0, 0));
+          const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, o + 16u * c, 0, kOnce));
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[i][4 * c + e] = x[e];
         }
@@ -241,54 +267,70 @@ __device__ void draft_stats(const Tree& A, int64_t slice, float (*a_s)[kTreeMaxN
   const float mr = m == -INFINITY ? 0.f : m;
   for (int a = 0; a <= t; ++a)
     if (seen_s[t] >> a & 1) l += fast_exp2(a_s[t][a] - mr);
-  A.part[slice * (A.nchunk + 1) * n + t] = make_float2(m, l);
+  A.part[slice * (A.nstat + 1) * n + t] = make_float2(m, l);
 }
 
 constexpr int kShareStride = kTreeMaxNodes + 4;         // floats: 16-byte rows, a column on 16 banks
 
-// Shares of the drafted keys and their part of the outputs.  sh_s[a][i]: -1 where
-// node i does not see key a (shares are not negative there: the drafted keys start
-// without demand).
+// Shares of the drafted keys and their part of the outputs.  p_s[i][a]: node i's bid
+// for key a, 0 where it does not see it, so that the demand of a pair is a plain sum
+// down i's chain; sh_s[a][i]: the share, -1 where i does not see a (shares are not
+// negative there: the drafted keys start without demand).
 template <int D, int DT>
-__device__ void draft_apply(const Tree& A, int64_t slice, float (*t_s)[kTreeMaxNodes + 1], float (*sh_s)[kShareStride],
-                            const uint64_t* seen_s, const int32_t* parents, const float* lse_s) {
+__device__ void draft_apply(const Tree& A, int64_t slice, float (*p_s)[kTreeMaxNodes + 1], float (*sh_s)[kShareStride],
+                            const uint64_t* seen_s, const float* lse_s) {
   const int t = threadIdx.x, n = A.nodes;
   const int64_t p0 = slice * (A.nchunk + 1) * n;
-  if (t < 64) {                                        // one wave: lane = key
-    for (int i = 0; i < kTreeMaxNodes; ++i) {
-      const bool on = i < n && (seen_s[i] >> t & 1);
-      float sh = -1.f;
-      if (on) {
-        const float p = fast_exp2(A.aff[(slice * n + i) * n + t] - lse_s[i]);
-        const int par = parents[i];
-        // the parent does not see a node's own key: it starts at 0
-        const float tot = (par >= 0 && t != i ? t_s[par][t] : 0.f) + p;
-        t_s[i][t] = tot;
-        sh = p * fast_rcp(tot + kEps);
-      }
-      sh_s[t][i] = sh;
-      const float s = wave_sum(on ? sh : 0.f);
-      if (t == 0 && i < n) A.part_sum[p0 + i] = s;
-    }
+  for (int o = t; o < n * n; o += kTreeThreads) {
+    const int i = o / n, a = o % n;
+    p_s[i][a] = seen_s[i] >> a & 1 ? fast_exp2(A.aff[slice * n * n + o] - lse_s[i]) : 0.f;
   }
   __syncthreads();
+  const int padded = (n + 15) & ~15;                    // the nodes that the loads below take
+  for (int o = t; o < padded * n; o += kTreeThreads) {
+    const int i = o / n, a = o % n;
+    const uint64_t seen = i < n ? seen_s[i] : 0;
+    float sh = -1.f;
+    if (seen >> a & 1) {
+      float tot = 0.f;
+      for (int c = a; c <= i; ++c)
+        if (seen >> c & 1) tot += p_s[c][a];
+      sh = p_s[i][a] * fast_rcp(tot + kEps);
+    }
+    sh_s[a][i] = sh;
+  }
+  __syncthreads();
+  if (t < n) {
+    float s = 0.f;
+    for (int a = 0; a <= t; ++a) s += sh_s[a][t] < 0.f ? 0.f : sh_s[a][t];
+    A.part_sum[p0 + t] = s;
+  }
   constexpr int kPer = D * kTreeMaxNodes / kTreeThreads;        // nodes of a thread
+  constexpr int kAhead = 8;                             // V rows in flight
   const int d = t % D, i0 = t / D * kPer;
   if (i0 >= n) return;
   const int64_t vbase = (slice * A.cap + A.length) * D + d;
   float x[kPer];
 #pragma unroll
   for (int u = 0; u < kPer; ++u) x[u] = 0.f;
-  for (int a = 0; a < n; ++a) {
-    const int64_t at = vbase + static_cast<int64_t>(a) * D;
-    float v;
-    if constexpr (DT == DT_F32) v = static_cast<const float*>(A.v)[at];
-    else if constexpr (DT == DT_BF16) v = bf16_bits_to_f32(static_cast<const uint16_t*>(A.v)[at]);
-    else v = f16_bits_to_f32(static_cast<const uint16_t*>(A.v)[at]);
+  for (int a0 = 0; a0 < n; a0 += kAhead) {
+    float v[kAhead];
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      const float w = sh_s[a][i0 + u];
-      x[u] = w < 0.f ? x[u] : fmaf(w, v, x[u]);
+    for (int b = 0; b < kAhead; ++b) {
+      const int64_t at = vbase + static_cast<int64_t>(min(a0 + b, n - 1)) * D;
+      if constexpr (DT == DT_F32) v[b] = static_cast<const float*>(A.v)[at];
+      else if constexpr (DT == DT_BF16) v[b] = bf16_bits_to_f32(static_cast<const uint16_t*>(A.v)[at]);
+      else v[b] = f16_bits_to_f32(static_cast<const uint16_t*>(A.v)[at]);
+    }
+#pragma unroll
+    for (int b = 0; b < kAhead; ++b) {
+      if (a0 + b >= n) break;
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        if (kPer > 16 && i0 + u >= padded) break;
+        const float w = sh_s[a0 + b][i0 + u];
+        x[u] = w < 0.f ? x[u] : fmaf(w, v[b], x[u]);
+      }
     }
   }
 #pragma unroll
@@ -303,7 +345,7 @@ template <int D, int DT, int NT>
 __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
   using S = Shape<D, DT>;
   const int64_t slice = A.slice0 + blockIdx.y;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, h = lane >> 5;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), l32 = lane & 31, h = lane >> 5;
   __shared__ union {
     u32x4 q[NT * S::kPieces * 64];
     float a[kTreeMaxNodes][kTreeMaxNodes + 1];
@@ -311,18 +353,21 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
   __shared__ uint64_t seen_s[kTreeMaxNodes];
   __shared__ float2 red[kTreeWaves][NT * kTileNodes];
   if (blockIdx.x == 0) {
-    if (wave == 0) seen_s[lane] = nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, lane);
+    if (wave == 0) {
+      const uint64_t seen = nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, lane);
+      seen_s[lane] = seen;
+      A.seen[slice * kTreeMaxNodes + lane] = seen;
+    }
     __syncthreads();
     draft_stats<D, DT>(A, slice, s.a, seen_s);
     return;
   }
   stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return r < A.nodes ? r : -1; });
-  const int64_t j0 = static_cast<int64_t>(blockIdx.x - 1) * A.chunk;
-  const int count = static_cast<int>(min(A.length - j0, static_cast<int64_t>(A.chunk)));
-  const __amdgpu_buffer_rsrc_t kr =
-      make_rsrc(static_cast<const char*>(A.k) + (slice * A.cap + j0) * S::kRow, static_cast<int64_t>(count) * S::kRow);
+  const char* keys = static_cast<const char*>(A.k) + slice * A.cap * S::kRow;
+  int64_t row = static_cast<int64_t>(blockIdx.x - 1) * kBlockRows + wave * 32;
+  const int64_t step = static_cast<int64_t>(A.nstat) * kBlockRows;
   KeyRows<D, DT> cur, nxt;
-  cur.load(kr, wave * 32, lane);
+  cur.load(keys, row, A.length, lane);
   __syncthreads();
   float m[NT], l[NT];
 #pragma unroll
@@ -330,16 +375,17 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
     m[u] = -INFINITY;
     l[u] = 0.f;
   }
-  for (int row = wave * 32; row < count; row += kTreeWaves * 32) {
+  auto tile = [&](auto last) {                           // as in tree_apply
+    constexpr bool kLast = decltype(last)::value;
     asm volatile("" ::: "memory");                     // the queries stay in LDS (tree_apply)
-    nxt.load(kr, row + kTreeWaves * 32, lane);
-    const int left = count - row;
+    nxt.load(keys, row + step, A.length, lane);
+    const int left = kLast ? static_cast<int>(A.length - row) : 32;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       floatx16 x = {};
 #pragma unroll
       for (int g = 0; g < S::kPieces; ++g) x = mma_piece<DT>(cur.p[g], s.q[(u * S::kPieces + g) * 64 + lane], x);
-      if (left < 32) {
+      if constexpr (kLast) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (acc_row(i, h) >= left) x[i] = -INFINITY;
@@ -356,7 +402,9 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
       m[u] = mn;
     }
     cur = nxt;
-  }
+  };
+  for (; row + 32 <= A.length; row += step) tile(std::false_type{});
+  if (row < A.length) tile(std::true_type{});
   // the lane halves hold different keys of the same node; then the waves
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
@@ -372,7 +420,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
     const float mr = mn == -INFINITY ? 0.f : mn;
 #pragma unroll
     for (int w = 0; w < kTreeWaves; ++w) sum += red[w][t].y * fast_exp2(red[w][t].x - mr);
-    A.part[(slice * (A.nchunk + 1) + blockIdx.x) * A.nodes + t] = make_float2(mn, sum);
+    A.part[(slice * (A.nstat + 1) + blockIdx.x) * A.nodes + t] = make_float2(mn, sum);
   }
 }
 
@@ -399,7 +447,7 @@ template <int D, int DT, int NT> constexpr int kApplyDV = D == 256 && NT == 2 ? 
 
 // Waves per SIMD that the registers are held to.
 template <int D, int DT, int NT>
-constexpr int kApplyWaves = DT == DT_F32 || D > 128 ? 1 : D == 128 ? 3 - NT : NT == 1 ? 3 : 2;
+constexpr int kApplyWaves = NT == 2 ? (DT != DT_F32 && D <= 64 ? 2 : 1) : D <= 64 ? 4 : D == 256 ? 1 : DT == DT_F32 ? 2 : 3;
 
 template <int D, int DT, int NT>
 __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_apply(Tree A) {
@@ -408,12 +456,12 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
   using V = ValueRows<DV, DT>;
   constexpr int kParts = kBidParts<DT>;
   const int64_t slice = A.slice0 + blockIdx.y;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, h = lane >> 5;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), l32 = lane & 31, h = lane >> 5;
   constexpr int kRedStride = DV + 1;
   __shared__ union {
     u32x4 q[NT * S::kPieces * 64];
     struct {
-      float t[kTreeMaxNodes][kTreeMaxNodes + 1];
+      float p[kTreeMaxNodes][kTreeMaxNodes + 1];
       float sh[kTreeMaxNodes][kShareStride];
     } draft;
     float red[NT * kTileNodes][kRedStride];
@@ -422,15 +470,14 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
   __shared__ uint64_t seen_s[kTreeMaxNodes];
   __shared__ __attribute__((aligned(16))) float lse_s[kTreeMaxNodes];
   __shared__ float sum_s[kTreeWaves][NT * kTileNodes];
-  const int32_t* parents = A.parents + slice / A.heads * A.parents_sb;
-  if (wave == 0) seen_s[lane] = nodes_seen(parents, A.nodes, lane);
+  if (wave == 0) seen_s[lane] = A.seen[slice * kTreeMaxNodes + lane];
   // the chunks' statistics joined: 64 nodes x 4 groups of entries
   {
     float m = -INFINITY, l = 0.f;
     if (lane < A.nodes) {
-      const float2* part = A.part + slice * (A.nchunk + 1) * A.nodes + lane;
+      const float2* part = A.part + slice * (A.nstat + 1) * A.nodes + lane;
 #pragma unroll 4
-      for (int c = wave; c <= A.nchunk; c += kTreeWaves) {
+      for (int c = wave; c <= A.nstat; c += kTreeWaves) {
         const float2 e = part[static_cast<int64_t>(c) * A.nodes];
         const float mn = fmaxf(m, e.x), mr = mn == -INFINITY ? 0.f : mn;
         l = l * fast_exp2(m - mr) + e.y * fast_exp2(e.x - mr);
@@ -454,18 +501,17 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
   }
   __syncthreads();
   if (blockIdx.x == 0) {
-    if (blockIdx.z == 0) draft_apply<D, DT>(A, slice, s.draft.t, s.draft.sh, seen_s, parents, lse_s);
+    if (blockIdx.z == 0) draft_apply<D, DT>(A, slice, s.draft.p, s.draft.sh, seen_s, lse_s);
     return;
   }
   stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return r < A.nodes ? r : -1; });
-  const int64_t j0 = static_cast<int64_t>(blockIdx.x - 1) * A.chunk;
-  const int count = static_cast<int>(min(A.length - j0, static_cast<int64_t>(A.chunk)));
-  const int64_t row_base = (slice * A.cap + j0) * S::kRow, bytes = static_cast<int64_t>(count) * S::kRow;
-  const __amdgpu_buffer_rsrc_t kr = make_rsrc(static_cast<const char*>(A.k) + row_base, bytes);
-  const __amdgpu_buffer_rsrc_t vr = make_rsrc(static_cast<const char*>(A.v) + row_base, bytes);
-  const float* com = A.committed + slice * A.cap + j0;
+  const char* keys = static_cast<const char*>(A.k) + slice * A.cap * S::kRow;
+  const char* values = static_cast<const char*>(A.v) + slice * A.cap * S::kRow;
+  int64_t row = static_cast<int64_t>(blockIdx.x - 1) * kBlockRows + wave * 32;
+  const int64_t step = static_cast<int64_t>(A.nchunk) * kBlockRows;
+  const float* com0 = A.committed + slice * A.cap;
   KeyRows<D, DT> cur;
-  cur.load(kr, wave * 32, lane);
+  cur.load(keys, row, A.length, lane);
 
   // step 2's operands (a node sees itself: the sums include its own bid)
   u32x4 anc[NT][NT][2], one[2];
@@ -489,24 +535,31 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
 #pragma unroll
     for (int e = 0; e < V::E; ++e) acc[u][e] = floatx16{};
   }
-  for (int row = wave * 32; row < count; row += kTreeWaves * 32) {
+  // One tile.  The last one of a slice may be partly past the end: a form of its own,
+  // so that the others are straight code.
+  auto tile = [&](auto last) {
+    constexpr bool kLast = decltype(last)::value;
     // the queries and row statistics stay in LDS: hoisted out of the loop they cost
     // a wave per SIMD
     asm volatile("" ::: "memory");
-    const int left = count - row;
+    const int left = kLast ? static_cast<int>(A.length - row) : 32;
+    const float* com = com0 + row + 4 * h;
     V val;
-    val.load(vr, row, lane, S::kRow, static_cast<int>(blockIdx.z) * DV * S::kElt);
+    val.load(values, row, A.length, lane, S::kRow, static_cast<int>(blockIdx.z) * DV * S::kElt);
     // committed + eps of this lane's keys in step 2's layout
     floatx16 c0;
-    if (left >= 32) {
+    if constexpr (!kLast) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c0[4 * g + e] = com[row + 8 * g + 4 * h + e];
+        for (int e = 0; e < 4; ++e) c0[4 * g + e] = com[8 * g + e];
       }
-    } else {
+    } else {                                            // keys past the end have no demand and (below) no bids
 #pragma unroll
-      for (int i = 0; i < 16; ++i) c0[i] = com[min(row + acc_row(i, h), count - 1)];
+      for (int i = 0; i < 16; ++i) {
+        const float x = com0[row + min(acc_row(i, h), left - 1)];
+        c0[i] = acc_row(i, h) < left ? x : 0.f;
+      }
     }
     // step 1
     u32x4 p[NT][kParts][2];
@@ -516,9 +569,9 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
 #pragma unroll
       for (int g = 0; g < S::kPieces; ++g)
         x = mma_piece<DT>(s.q[(u * S::kPieces + g) * 64 + h * 32 + rho(l32)], cur.p[g], x);
-      if (left < 32 && l32 >= left) {
+      if constexpr (kLast) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = -INFINITY;
+        for (int i = 0; i < 16; ++i) x[i] = l32 < left ? x[i] : -INFINITY;
       }
       float v[16];
       // register i of half h: node perm_row(i, h), two runs of 8
@@ -545,7 +598,7 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
           }
       }
     }
-    cur.load(kr, row + kTreeWaves * 32, lane);
+    cur.load(keys, row + step, A.length, lane);
 #pragma unroll
     for (int i = 0; i < 16; ++i) c0[i] += kEps;
     // steps 2 and 3
@@ -564,7 +617,6 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         sh[i] = bid[i] * fast_rcp(tot[i]);
-        if (left < 32 && acc_row(i, h) >= left) sh[i] = 0.f;
         ssum[u] += sh[i];
       }
       if constexpr (DT == DT_F32) {
@@ -587,7 +639,9 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
         }
       }
     }
-  }
+  };
+  for (; row + 32 <= A.length; row += step) tile(std::false_type{});
+  if (row < A.length) tile(std::true_type{});
   // the waves' sums, in order
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
@@ -632,7 +686,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_finish(Tree A) {
   const int64_t slice = A.slice0 + blockIdx.y;
   const int i = blockIdx.x, t = threadIdx.x, lane = t & 63, d = t % D, g = t / D;
   __shared__ float red[kGroups][D + 1];
-  const uint64_t seen = shfl64(nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, lane), i);
+  const uint64_t seen = A.seen[slice * kTreeMaxNodes + i];
   const float own = lane < A.nodes ? A.lse[slice * A.nodes + lane] : 0.f;
   const bool spoilt = (__ballot(own != own) & seen) != 0;
   const int64_t p0 = slice * (A.nchunk + 1) * A.nodes + i;
@@ -668,7 +722,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
   using S = Shape<D, DT>;
   constexpr int kUnits = S::kRow / 16;
   const int64_t slice = A.slice0 + blockIdx.y;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, l32 = lane & 31, h = lane >> 5;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), l32 = lane & 31, h = lane >> 5;
   __shared__ union {
     u32x4 q[NT * S::kPieces * 64];
     u32x4 rows[NT * kTileNodes * kUnits];
@@ -721,23 +775,22 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
     return;
   }
   stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return node_s[r]; });
-  const int64_t j0 = static_cast<int64_t>(blockIdx.x - 1) * A.chunk;
-  const int count = static_cast<int>(min(A.length - j0, static_cast<int64_t>(A.chunk)));
-  const __amdgpu_buffer_rsrc_t kr =
-      make_rsrc(static_cast<const char*>(A.k) + (slice * A.cap + j0) * S::kRow, static_cast<int64_t>(count) * S::kRow);
+  const char* keys = static_cast<const char*>(A.k) + slice * A.cap * S::kRow;
+  int64_t row = static_cast<int64_t>(blockIdx.x - 1) * kBlockRows + wave * 32;
+  const int64_t step = static_cast<int64_t>(A.nchunk) * kBlockRows;
   KeyRows<D, DT> cur, nxt;
-  cur.load(kr, wave * 32, lane);
+  cur.load(keys, row, A.length, lane);
   float lse[NT][16];
 #pragma unroll
   for (int u = 0; u < NT; ++u)
 #pragma unroll
     for (int i = 0; i < 16; ++i) lse[u][i] = lse_s[u * kTileNodes + acc_row(i, h)];
   __syncthreads();
-  for (int row = wave * 32; row < count; row += kTreeWaves * 32) {
+  for (; row < A.length; row += step) {
     asm volatile("" ::: "memory");                     // the queries stay in LDS (tree_apply)
-    const int j = row + l32;
-    const float c = j < count ? crow[j0 + j] : 0.f;
-    nxt.load(kr, row + kTreeWaves * 32, lane);
+    const int64_t j = row + l32;
+    const float c = j < A.length ? crow[j] : 0.f;
+    nxt.load(keys, row + step, A.length, lane);
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
@@ -752,7 +805,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
       }
     }
     sum += __shfl_xor(sum, 32, 64);
-    if (h == 0 && j < count) crow[j0 + j] = c + sum;
+    if (h == 0 && j < A.length) crow[j] = c + sum;
     cur = nxt;
   }
 }
@@ -760,18 +813,24 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
 // ---------------------------------------------------------------------------
 // launches
 
-// Cached keys of a workgroup.
-int tree_chunk(int64_t n, int64_t length) {
-  constexpr int64_t kTarget = 2048, kMin = 256, kMax = 4096;
-  int64_t per = (kTarget + n - 1) / n;                 // workgroups of a slice
-  int64_t chunk = (length + per - 1) / per;
-  chunk = (chunk + 127) / 128 * 128;
-  return static_cast<int>(chunk < kMin ? kMin : chunk > kMax ? kMax : chunk);
+// The workgroups of a slice over its cached keys: those of all slices (one more each,
+// for the drafted keys) fill whole rounds of the `slots` that the GPU holds at once,
+// as few rounds as fill 15/16 of their places (of 4 rounds the best).  At least 256
+// keys each.
+int tree_split(int64_t n, int64_t length, int64_t slots) {
+  if (length < 1) return 0;
+  int64_t best = 1, best_fill = -1;
+  for (int64_t rounds = (2 * n + slots - 1) / slots, i = 0; i < 4 && best_fill < 960; ++rounds, ++i) {
+    const int64_t c = rounds * slots / n - 1, fill = n * (c + 1) * 1024 / (rounds * slots);
+    if (fill > best_fill) {
+      best = c;
+      best_fill = fill;
+    }
+  }
+  const int64_t most = (length + 2 * kBlockRows - 1) / (2 * kBlockRows);
+  return static_cast<int>(best < most ? best : most);
 }
-int64_t tree_chunks(int64_t n, int64_t length) {
-  const int64_t chunk = tree_chunk(n, length);
-  return (length + chunk - 1) / chunk;
-}
+constexpr int64_t kCUs = 256;
 
 Tree tree_of(const TreeArgs& a) {
   Tree A{};
@@ -789,38 +848,50 @@ Tree tree_of(const TreeArgs& a) {
   A.out = a.out;
   A.ov = a.ov;
   A.lse = a.lse;
-  A.chunk = tree_chunk(a.n, a.length);
-  A.nchunk = static_cast<int>(tree_chunks(a.n, a.length));
   A.scale = kLog2e / sqrtf(static_cast<float>(a.head_dim));
   return A;
 }
 
-struct TreeScratch {
-  size_t part, out, sum, aff, total;
-  TreeScratch(int64_t n, int64_t length, int64_t nodes, int head_dim) {
-    const size_t rows = static_cast<size_t>(n * (tree_chunks(n, length) + 1) * nodes);
+// One step's chunks and the places in its workspace.
+struct TreePlan {
+  int nstat, nchunk;
+  size_t part, out, sum, aff, seen, total;
+  TreePlan(int64_t n, int64_t length, int64_t nodes, int head_dim, int apply_waves) {
+    // The places to fill are the CUs times the workgroups that each holds, or a
+    // multiple: several short rounds hide one another's start and end.  us for 128
+    // slices of 65536 keys, 64 nodes: statistics with 512, 768, 1024, 2048 places 203,
+    // 196, 238, 198 (768 at once); shares with 512, 768, 1024, 2048 476, 462, 426, 439
+    // (512 at once).  128 slices of 16384 keys, 32 nodes: statistics 55, 55, 56, 52
+    // (2048 at once), shares 128, 105, 101, 104 (1024 at once).
+    nstat = tree_split(n, length, kCUs * (nodes > kTileNodes ? 3 : 8));
+    nchunk = tree_split(n, length, kCUs * (nodes > kTileNodes && apply_waves == 2 ? 4 : apply_waves));
+    const size_t rows = static_cast<size_t>(n * (nchunk + 1) * nodes);
     part = 0;
-    out = part + align_up(sizeof(float2) * rows);
+    out = part + align_up(sizeof(float2) * n * (nstat + 1) * nodes);
     sum = out + align_up(sizeof(float) * rows * head_dim);
     aff = sum + align_up(sizeof(float) * rows);
-    total = aff + align_up(sizeof(float) * n * nodes * nodes);
+    seen = aff + align_up(sizeof(float) * n * nodes * nodes);
+    total = seen + align_up(sizeof(uint64_t) * n * kTreeMaxNodes);
   }
 };
 
 template <int D, int DT, int NT>
 int launch_step(const TreeArgs& a) {
   Tree A = tree_of(a);
-  const TreeScratch w(a.n, a.length, a.nodes, a.head_dim);
+  const TreePlan w(a.n, a.length, a.nodes, D, kApplyWaves<D, DT, NT>);
+  A.nstat = w.nstat;
+  A.nchunk = w.nchunk;
   char* ws = static_cast<char*>(a.workspace);
   A.part = reinterpret_cast<float2*>(ws + w.part);
   A.part_out = reinterpret_cast<float*>(ws + w.out);
   A.part_sum = reinterpret_cast<float*>(ws + w.sum);
   A.aff = reinterpret_cast<float*>(ws + w.aff);
+  A.seen = reinterpret_cast<uint64_t*>(ws + w.seen);
   hipStream_t st = static_cast<hipStream_t>(a.stream);
   const unsigned chunks = static_cast<unsigned>(A.nchunk + 1);
   slice_batches(a.n, [&](int64_t s0, unsigned ns) {
     A.slice0 = s0;
-    DIL_TIMED("tree_stats", st, (tree_stats<D, DT, NT><<<dim3(chunks, ns), kTreeThreads, 0, st>>>(A)));
+    DIL_TIMED("tree_stats", st, (tree_stats<D, DT, NT><<<dim3(A.nstat + 1, ns), kTreeThreads, 0, st>>>(A)));
     DIL_TIMED("tree_apply", st,
               (tree_apply<D, DT, NT><<<dim3(chunks, ns, D / kApplyDV<D, DT, NT>), kTreeThreads, 0, st>>>(A)));
     DIL_TIMED("tree_finish", st, (tree_finish<D, DT><<<dim3(A.nodes, ns), kTreeThreads, 0, st>>>(A)));
@@ -831,6 +902,8 @@ int launch_step(const TreeArgs& a) {
 template <int D, int DT, int NT>
 int launch_accept(const TreeArgs& a) {
   Tree A = tree_of(a);
+  // 128 slices of 65536 keys with 512, 768, 1024, 2048, 4096 places: 296, 258, 236, 238, 230 us
+  A.nchunk = tree_split(a.n, a.length, kCUs * 8);
   A.demand = a.committed;
   A.k_move = a.k_cache;
   A.v_move = a.v_cache;
@@ -873,9 +946,13 @@ int with_shape(int head_dim, int dtype, int nodes, F&& f) {
 }  // namespace
 
 int64_t tree_workspace_bytes(int64_t n, int64_t length, int64_t nodes, int head_dim, int dtype) {
-  (void)dtype;
-  if (n < 1) return 0;
-  return static_cast<int64_t>(TreeScratch(n, length < 0 ? 0 : length, nodes, head_dim).total);
+  if (n < 1 || length < 0 || nodes < 1 || nodes > kTreeMaxNodes) return 0;
+  int64_t bytes = 0;
+  with_shape(head_dim, dtype, static_cast<int>(nodes), [&](auto d, auto t, auto nt) {
+    bytes = static_cast<int64_t>(TreePlan(n, length, nodes, d(), kApplyWaves<d(), t(), nt()>).total);
+    return 0;
+  });
+  return bytes;
 }
 
 int tree_step(const TreeArgs& a) {
