@@ -25,8 +25,9 @@
 //   3  the shares, in place, are the B operand of out^T += V^T share^T, whose A
 //      operand takes V rows as loaded, two head dims a register, regrouped by
 //      byte permutes.
-// The drafted keys (at most 64) are a workgroup of their own in plain fp32: there
-// the masks are, and what a node does not see it must not touch (NaN included).
+// The drafted keys (at most 64) are a workgroup of their own: there the masks are, and
+// what a node does not see it must not touch (NaN included), so their shares are
+// summed in plain fp32.
 // A node whose own row statistics are NaN would spoil the others in step 2: its
 // bids are taken as 0 there, and tree_finish makes it and the nodes below it NaN.
 #include "dil_tiles.hpp"
@@ -152,15 +153,20 @@ __device__ __forceinline__ void stage_queries(u32x4* q_s, const Tree& A, int64_t
 // took 193 to 235 us by the stretch's length.)  All uniform in a wave.
 constexpr int kBlockRows = kTreeWaves * 32;
 
+// An address that is the same in every lane, in scalar registers.
+__device__ __forceinline__ void* uniform(const void* p) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
+  return reinterpret_cast<void*>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+
 // The resource over the 32 rows from `row` on, as far as they exist: rows past the end
 // read 0.  Offsets within it are per lane alone, which the range check covers.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char* base, int64_t row, int64_t length, int rowbytes) {
   const int64_t left = length - row;
   const int n = left < 0 ? 0 : left < 32 ? static_cast<int>(left) : 32;
-  const uint64_t a = reinterpret_cast<uint64_t>(base) + static_cast<uint64_t>(row) * static_cast<uint32_t>(rowbytes);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
-  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((static_cast<uint64_t>(hi) << 32) | lo), 0,
+  return __builtin_amdgcn_make_buffer_rsrc(uniform(base + row * rowbytes), 0,
                                            __builtin_amdgcn_readfirstlane(n * rowbytes), 0x00020000);
 }
 
@@ -173,8 +179,14 @@ template <int D, int DT>
 struct KeyRows {
   u32x4 p[Shape<D, DT>::kPieces];
   __device__ __forceinline__ void load(const char* base, int64_t row, int64_t length, int lane) {
-    const __amdgpu_buffer_rsrc_t r = rows_at(base, row, length, Shape<D, DT>::kRow);
-    uint32_t off = static_cast<uint32_t>(lane & 31) * Shape<D, DT>::kRow + (lane >> 5) * 16u;
+    load(rows_at(base, row, length, Shape<D, DT>::kRow), row, lane, lane & 31);
+  }
+  // the rows `mine` of the lanes among `rows` (at most 64) at base; none where negative
+  __device__ __forceinline__ void gather(const char* base, int rows, int lane, int mine) {
+    load(__builtin_amdgcn_make_buffer_rsrc(uniform(base), 0, rows * Shape<D, DT>::kRow, 0x00020000), 0, lane, mine);
+  }
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int64_t row, int lane, int mine) {
+    uint32_t off = mine < 0 ? 0xf0000000u : static_cast<uint32_t>(mine) * Shape<D, DT>::kRow + (lane >> 5) * 16u;
     keep_in_loop(off, row);
 #pragma unroll
     for (int g = 0; g < Shape<D, DT>::kPieces; ++g)
@@ -238,104 +250,122 @@ struct ValueRows {
 // ---------------------------------------------------------------------------
 // the drafted keys
 
-// Affinities of every node for the drafted keys that it sees; the maxima and sums
-// of 2^(a - max) over them as the slice's entry 0.
-template <int D, int DT>
-__device__ void draft_stats(const Tree& A, int64_t slice, float (*a_s)[kTreeMaxNodes + 1], const uint64_t* seen_s) {
-  const int t = threadIdx.x, n = A.nodes;
-  const int64_t qbase = A.qv.slice(slice), kbase = (slice * A.cap + A.length) * D;
-  for (int p = t; p < n * n; p += kTreeThreads) {
-    const int i = p / n, a = p % n;
-    if (!(seen_s[i] >> a & 1)) continue;
-    float s = 0.f;
-    for (int d = 0; d < D; d += 8) {
-      float x[8], y[8];
-      load8_f32(A.q, qbase + i * A.qv.sr + d, DT, x);
-      load8_f32(A.k, kbase + static_cast<int64_t>(a) * D + d, DT, y);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
-    }
-    s *= A.scale;
-    a_s[i][a] = s;
-    A.aff[(slice * n + i) * n + a] = s;
-  }
-  __syncthreads();
-  if (t >= n) return;
-  float m = -INFINITY, l = 0.f;
-  for (int a = 0; a <= t; ++a)
-    if (seen_s[t] >> a & 1) m = fmaxf(m, a_s[t][a]);
-  const float mr = m == -INFINITY ? 0.f : m;
-  for (int a = 0; a <= t; ++a)
-    if (seen_s[t] >> a & 1) l += fast_exp2(a_s[t][a] - mr);
-  A.part[slice * (A.nstat + 1) * n + t] = make_float2(m, l);
-}
-
 constexpr int kShareStride = kTreeMaxNodes + 4;         // floats: 16-byte rows, a column on 16 banks
 
-// Shares of the drafted keys and their part of the outputs.  p_s[i][a]: node i's bid
-// for key a, 0 where it does not see it, so that the demand of a pair is a plain sum
-// down i's chain; sh_s[a][i]: the share, -1 where i does not see a (shares are not
-// negative there: the drafted keys start without demand).
+// Sum over the wave in every lane, by lane moves of the vector unit (a shuffle through
+// LDS takes about ten times as long).
+__device__ __forceinline__ float wave_sum_dpp(float x) {
+  auto moved = [](float v, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  x += moved(x, std::integral_constant<int, 0xB1>{});    // quad_perm [1, 0, 3, 2]
+  x += moved(x, std::integral_constant<int, 0x4E>{});    // quad_perm [2, 3, 0, 1]
+  x += moved(x, std::integral_constant<int, 0x141>{});   // row_half_mirror
+  x += moved(x, std::integral_constant<int, 0x140>{});   // row_mirror
+  const int b = __float_as_int(x);
+  return (__int_as_float(__builtin_amdgcn_readlane(b, 0)) + __int_as_float(__builtin_amdgcn_readlane(b, 16))) +
+         (__int_as_float(__builtin_amdgcn_readlane(b, 32)) + __int_as_float(__builtin_amdgcn_readlane(b, 48)));
+}
+
+// Shares of the drafted keys and their part of the outputs, from the affinities that
+// tree_stats left.  Wave w holds the nodes i = w + 4 u in registers, a lane one key;
+// the demand goes down the chains by doubling (after k rounds a pair holds the bids
+// of 2^k nodes of the chain).  What a node does not see enters as 0, and where a V row
+// is not finite not at all.
 template <int D, int DT>
-__device__ void draft_apply(const Tree& A, int64_t slice, float (*p_s)[kTreeMaxNodes + 1], float (*sh_s)[kShareStride],
+__device__ void draft_apply(const Tree& A, int64_t slice, float (*t_s)[kTreeMaxNodes], float (*sh_s)[kShareStride],
                             const uint64_t* seen_s, const float* lse_s) {
-  const int t = threadIdx.x, n = A.nodes;
+  constexpr int kRows = kTreeMaxNodes / kTreeWaves;
+  const int t = threadIdx.x, n = A.nodes, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int64_t p0 = slice * (A.nchunk + 1) * n;
-  for (int o = t; o < n * n; o += kTreeThreads) {
-    const int i = o / n, a = o % n;
-    p_s[i][a] = seen_s[i] >> a & 1 ? fast_exp2(A.aff[slice * n * n + o] - lse_s[i]) : 0.f;
+  const uint64_t above = seen_s[lane] & ~(uint64_t{1} << lane);
+  int jump = above ? 63 - __clzll(static_cast<long long>(above)) : -1;    // node `lane`'s parent
+  float p[kRows], tot[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int i = wave + kTreeWaves * u;
+    p[u] = 0.f;
+    if (i < n && (seen_s[i] >> lane & 1)) p[u] = fast_exp2(A.aff[(slice * n + i) * n + lane] - lse_s[i]);
+    tot[u] = p[u];
   }
-  __syncthreads();
-  const int padded = (n + 15) & ~15;                    // the nodes that the loads below take
-  for (int o = t; o < padded * n; o += kTreeThreads) {
-    const int i = o / n, a = o % n;
-    const uint64_t seen = i < n ? seen_s[i] : 0;
-    float sh = -1.f;
-    if (seen >> a & 1) {
-      float tot = 0.f;
-      for (int c = a; c <= i; ++c)
-        if (seen >> c & 1) tot += p_s[c][a];
-      sh = p_s[i][a] * fast_rcp(tot + kEps);
+  for (int span = 1; span < n; span *= 2) {
+#pragma unroll
+    for (int u = 0; u < kRows; ++u)
+      if (wave + kTreeWaves * u < n) t_s[wave + kTreeWaves * u][lane] = tot[u];
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      if (wave + kTreeWaves * u >= n) break;
+      const int j = __builtin_amdgcn_readlane(jump, wave + kTreeWaves * u);
+      if (j >= 0) tot[u] += t_s[j][lane];
     }
-    sh_s[a][i] = sh;
+    const int next = __shfl(jump, max(jump, 0), 64);
+    jump = jump < 0 ? -1 : next;
+    __syncthreads();
+  }
+  const int n4 = n <= 16 ? (n + 3) & ~3 : kTreeMaxNodes;    // the products below take at least 4 nodes at a time, or a block's
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int i = wave + kTreeWaves * u;
+    if (i >= n4) break;
+    const float sh = seen_s[i] >> lane & 1 ? p[u] * fast_rcp(tot[u] + kEps) : 0.f;
+    sh_s[lane][i] = sh;
+    const float sum = wave_sum_dpp(sh);
+    if (lane == 0 && i < n) A.part_sum[p0 + i] = sum;
   }
   __syncthreads();
-  if (t < n) {
-    float s = 0.f;
-    for (int a = 0; a <= t; ++a) s += sh_s[a][t] < 0.f ? 0.f : sh_s[a][t];
-    A.part_sum[p0 + t] = s;
-  }
-  constexpr int kPer = D * kTreeMaxNodes / kTreeThreads;        // nodes of a thread
-  constexpr int kAhead = 8;                             // V rows in flight
-  const int d = t % D, i0 = t / D * kPer;
-  if (i0 >= n) return;
+  constexpr int kPer = D < 64 ? D / 4 : 16;             // nodes of a thread at a time
+  constexpr int kAhead = 16;                            // V rows in flight
+  const int d = t % D;
   const int64_t vbase = (slice * A.cap + A.length) * D + d;
-  float x[kPer];
+  auto value = [&](int a) {
+    const int64_t at = vbase + static_cast<int64_t>(a) * D;
+    if constexpr (DT == DT_F32) return static_cast<const float*>(A.v)[at];
+    else if constexpr (DT == DT_BF16) return bf16_bits_to_f32(static_cast<const uint16_t*>(A.v)[at]);
+    else return f16_bits_to_f32(static_cast<const uint16_t*>(A.v)[at]);
+  };
+  for (int i0 = t / D * kPer; i0 < n; i0 += kTreeThreads / D * kPer) {
+    float x[kPer];
 #pragma unroll
-  for (int u = 0; u < kPer; ++u) x[u] = 0.f;
-  for (int a0 = 0; a0 < n; a0 += kAhead) {
-    float v[kAhead];
+    for (int u = 0; u < kPer; ++u) x[u] = 0.f;
+    // `keys` V rows from a0 on: a whole block in straight code, or the fewer of the last
+    auto block = [&](auto whole, int a0, int keys) {
+      constexpr bool kWhole = decltype(whole)::value;
+      float v[kAhead], odd = 0.f;
 #pragma unroll
-    for (int b = 0; b < kAhead; ++b) {
-      const int64_t at = vbase + static_cast<int64_t>(min(a0 + b, n - 1)) * D;
-      if constexpr (DT == DT_F32) v[b] = static_cast<const float*>(A.v)[at];
-      else if constexpr (DT == DT_BF16) v[b] = bf16_bits_to_f32(static_cast<const uint16_t*>(A.v)[at]);
-      else v[b] = f16_bits_to_f32(static_cast<const uint16_t*>(A.v)[at]);
-    }
+      for (int b = 0; b < kAhead; ++b) v[b] = kWhole || b < keys ? value(a0 + b) : 0.f;
 #pragma unroll
-    for (int b = 0; b < kAhead; ++b) {
-      if (a0 + b >= n) break;
+      for (int b = 0; b < kAhead; ++b) odd += v[b] - v[b];        // 0, or NaN where a value is not finite
+      if (__ballot(odd != 0.f) == 0) {
 #pragma unroll
-      for (int u = 0; u < kPer; ++u) {
-        if (kPer > 16 && i0 + u >= padded) break;
-        const float w = sh_s[a0 + b][i0 + u];
-        x[u] = w < 0.f ? x[u] : fmaf(w, v[b], x[u]);
+        for (int b = 0; b < kAhead; ++b) {
+          if (!kWhole && b >= keys) break;
+#pragma unroll
+          for (int u = 0; u < kPer; u += 4) {
+            if (!kWhole && i0 + u >= n) break;
+            const floatx4 sh = *reinterpret_cast<const floatx4*>(&sh_s[a0 + b][i0 + u]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[u + e] = fmaf(sh[e], v[b], x[u + e]);
+          }
+        }
+      } else {
+        for (int b = 0; b < keys; ++b) {
+          float vb = v[0];
+#pragma unroll
+          for (int c = 1; c < kAhead; ++c) vb = c == b ? v[c] : vb;
+#pragma unroll
+          for (int u = 0; u < kPer; ++u)
+            if (seen_s[i0 + u] >> (a0 + b) & 1) x[u] = fmaf(sh_s[a0 + b][i0 + u], vb, x[u]);
+        }
       }
-    }
-  }
+    };
+    int a0 = 0;
+    for (; a0 + kAhead <= n; a0 += kAhead) block(std::true_type{}, a0, kAhead);
+    if (a0 < n) block(std::false_type{}, a0, n - a0);
 #pragma unroll
-  for (int u = 0; u < kPer; ++u)
-    if (i0 + u < n) A.part_out[(p0 + i0 + u) * D + d] = x[u];
+    for (int u = 0; u < kPer; ++u)
+      if (i0 + u < n) A.part_out[(p0 + i0 + u) * D + d] = x[u];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -346,28 +376,23 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
   using S = Shape<D, DT>;
   const int64_t slice = A.slice0 + blockIdx.y;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), l32 = lane & 31, h = lane >> 5;
-  __shared__ union {
-    u32x4 q[NT * S::kPieces * 64];
-    float a[kTreeMaxNodes][kTreeMaxNodes + 1];
-  } s;
+  __shared__ u32x4 q_s[NT * S::kPieces * 64];
   __shared__ uint64_t seen_s[kTreeMaxNodes];
   __shared__ float2 red[kTreeWaves][NT * kTileNodes];
-  if (blockIdx.x == 0) {
-    if (wave == 0) {
-      const uint64_t seen = nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, lane);
-      seen_s[lane] = seen;
-      A.seen[slice * kTreeMaxNodes + lane] = seen;
-    }
-    __syncthreads();
-    draft_stats<D, DT>(A, slice, s.a, seen_s);
-    return;
+  // the first workgroup of a slice takes the drafted keys, wave w the 32 from 32 w on
+  const bool drafted = blockIdx.x == 0;
+  if (drafted && wave == 0) {
+    const uint64_t seen = nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, lane);
+    seen_s[lane] = seen;
+    A.seen[slice * kTreeMaxNodes + lane] = seen;
   }
-  stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return r < A.nodes ? r : -1; });
+  stage_queries<D, DT, NT>(q_s, A, slice, [&](int r) { return r < A.nodes ? r : -1; });
   const char* keys = static_cast<const char*>(A.k) + slice * A.cap * S::kRow;
-  int64_t row = static_cast<int64_t>(blockIdx.x - 1) * kBlockRows + wave * 32;
+  const int64_t end = drafted ? A.length + A.nodes : A.length;
+  int64_t row = (drafted ? A.length : static_cast<int64_t>(blockIdx.x - 1) * kBlockRows) + wave * 32;
   const int64_t step = static_cast<int64_t>(A.nstat) * kBlockRows;
   KeyRows<D, DT> cur, nxt;
-  cur.load(keys, row, A.length, lane);
+  cur.load(keys, row, end, lane);
   __syncthreads();
   float m[NT], l[NT];
 #pragma unroll
@@ -375,20 +400,31 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
     m[u] = -INFINITY;
     l[u] = 0.f;
   }
-  auto tile = [&](auto last) {                           // as in tree_apply
-    constexpr bool kLast = decltype(last)::value;
+  // kind 0: 32 cached keys; 1: the last ones of a slice, fewer; 2: drafted keys, masked
+  auto tile = [&](auto kind) {
+    constexpr int kKind = decltype(kind)::value;
     asm volatile("" ::: "memory");                     // the queries stay in LDS (tree_apply)
-    nxt.load(keys, row + step, A.length, lane);
-    const int left = kLast ? static_cast<int>(A.length - row) : 32;
+    nxt.load(keys, row + step, end, lane);
+    const int left = kKind == 0 ? 32 : static_cast<int>(end - row);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       floatx16 x = {};
 #pragma unroll
-      for (int g = 0; g < S::kPieces; ++g) x = mma_piece<DT>(cur.p[g], s.q[(u * S::kPieces + g) * 64 + lane], x);
-      if constexpr (kLast) {
+      for (int g = 0; g < S::kPieces; ++g) x = mma_piece<DT>(cur.p[g], q_s[(u * S::kPieces + g) * 64 + lane], x);
+      if constexpr (kKind == 1) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (acc_row(i, h) >= left) x[i] = -INFINITY;
+      }
+      if constexpr (kKind == 2) {
+        const int node = u * kTileNodes + l32, key0 = static_cast<int>(row - A.length);
+        const uint64_t seen = seen_s[node];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = key0 + acc_row(i, h);
+          if (seen >> key & 1) A.aff[(slice * A.nodes + node) * A.nodes + key] = x[i] * A.scale;
+          else x[i] = -INFINITY;
+        }
       }
       float big = x[0];
 #pragma unroll
@@ -403,8 +439,12 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
     }
     cur = nxt;
   };
-  for (; row + 32 <= A.length; row += step) tile(std::false_type{});
-  if (row < A.length) tile(std::true_type{});
+  if (drafted) {
+    if (row < end) tile(std::integral_constant<int, 2>{});
+  } else {
+    for (; row + 32 <= end; row += step) tile(std::integral_constant<int, 0>{});
+    if (row < end) tile(std::integral_constant<int, 1>{});
+  }
   // the lane halves hold different keys of the same node; then the waves
 #pragma unroll
   for (int u = 0; u < NT; ++u) {
@@ -461,7 +501,7 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
   __shared__ union {
     u32x4 q[NT * S::kPieces * 64];
     struct {
-      float p[kTreeMaxNodes][kTreeMaxNodes + 1];
+      float p[kTreeMaxNodes][kTreeMaxNodes];
       float sh[kTreeMaxNodes][kShareStride];
     } draft;
     float red[NT * kTileNodes][kRedStride];
@@ -726,7 +766,6 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
   __shared__ union {
     u32x4 q[NT * S::kPieces * 64];
     u32x4 rows[NT * kTileNodes * kUnits];
-    float p[kTreeMaxNodes][kTreeMaxNodes + 1];
   } s;
   __shared__ float lse_s[kTreeMaxNodes];
   __shared__ int node_s[kTreeMaxNodes];
@@ -738,30 +777,31 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
   }
   __syncthreads();
   float* crow = A.demand + slice * A.cap;
+  stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return node_s[r]; });
+  const char* keys = static_cast<const char*>(A.k) + slice * A.cap * S::kRow;
   if (blockIdx.x == 0) {
-    const int64_t qbase = A.qv.slice(slice), kbase = (slice * A.cap + A.length) * D;
-    for (int o = t; o < A.count * A.count; o += kTreeThreads) {
-      const int r = o / A.count, c = o % A.count;
-      if (c > r) continue;
-      const int i = node_s[r], a = node_s[c];
-      float x = 0.f;
-      if (i >= 0 && a >= 0) {
-        for (int d = 0; d < D; d += 8) {
-          float q[8], k[8];
-          load8_f32(A.q, qbase + i * A.qv.sr + d, DT, q);
-          load8_f32(A.k, kbase + static_cast<int64_t>(a) * D + d, DT, k);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x = fmaf(q[e], k[e], x);
-        }
-        x = fast_exp2(fmaf(x, A.scale, -lse_s[r]));
-      }
-      s.p[r][c] = x;
-    }
+    // wave w: the accepted positions 32 w + [0, 32), one per lane, and the bids of the
+    // accepted nodes from that one on
     __syncthreads();
-    if (t < A.count) {
-      float x = 0.f;
-      for (int r = t; r < A.count; ++r) x += s.p[r][t];
-      crow[A.length + t] = x;
+    if (wave < NT) {
+      const int c = wave * kTileNodes + l32, node = node_s[c];
+      KeyRows<D, DT> k;
+      k.gather(keys + A.length * S::kRow, A.nodes, lane, node);
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        floatx16 x = {};
+#pragma unroll
+        for (int g = 0; g < S::kPieces; ++g) x = mma_piece<DT>(s.q[(u * S::kPieces + g) * 64 + lane], k.p[g], x);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = u * kTileNodes + acc_row(i, h);
+          const float p = fast_exp2(fmaf(x[i], A.scale, -lse_s[r]));
+          if (r >= c && node_s[r] >= 0) sum += p;
+        }
+      }
+      sum += __shfl_xor(sum, 32, 64);
+      if (h == 0 && c < A.count) crow[A.length + c] = node < 0 ? 0.f : sum;
     }
     for (void* cache : {A.k_move, A.v_move}) {
       u32x4* rows = reinterpret_cast<u32x4*>(static_cast<char*>(cache) + (slice * A.cap + A.length) * S::kRow);
@@ -774,8 +814,6 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
     }
     return;
   }
-  stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return node_s[r]; });
-  const char* keys = static_cast<const char*>(A.k) + slice * A.cap * S::kRow;
   int64_t row = static_cast<int64_t>(blockIdx.x - 1) * kBlockRows + wave * 32;
   const int64_t step = static_cast<int64_t>(A.nchunk) * kBlockRows;
   KeyRows<D, DT> cur, nxt;
