@@ -39,7 +39,7 @@ __host__ __device__ constexpr uint32_t digit_mask(int level) { return level == 2
 // One bin's place: the counts of thread t's two bins (2 t and 2 t + 1), with the
 // counts of the higher bins before them.
 struct Found {
-  int bin, left;                  // the bin that holds the want-th largest, and how many of it are wanted
+  int bin, left, count;           // the bin that holds the want-th largest, how many of it are wanted, and how many it has
 };
 // Every thread of the workgroup calls.
 __device__ __forceinline__ Found find_bin(int h0, int h1, int want, int* scratch) {
@@ -58,12 +58,14 @@ __device__ __forceinline__ Found find_bin(int h0, int h1, int want, int* scratch
   if (above < want && want <= above + h1) {
     scratch[kWaves] = 2 * t + 1;
     scratch[kWaves + 1] = want - above;
+    scratch[kWaves + 2] = h1;
   } else if (above + h1 < want && want <= above + h1 + h0) {
     scratch[kWaves] = 2 * t;
     scratch[kWaves + 1] = want - above - h1;
+    scratch[kWaves + 2] = h0;
   }
   __syncthreads();
-  return {scratch[kWaves], scratch[kWaves + 1]};
+  return {scratch[kWaves], scratch[kWaves + 1], scratch[kWaves + 2]};
 }
 
 // Counts a key's digit.  The lanes that have the first counting lane's digit count
@@ -167,7 +169,7 @@ __device__ __forceinline__ void load_keys(uint32_t (&key)[E], const float* row, 
 template <int E>
 __global__ __launch_bounds__(kSelThreads) void evict_select(Select A) {
   __shared__ int hist[kBins];
-  __shared__ int scratch[kWaves + 2];
+  __shared__ int scratch[kWaves + 3];
   __shared__ int2 cnt[E][kWaves], total;
   const int t = threadIdx.x;
   const int64_t slice = A.slice0 + blockIdx.x;
@@ -192,7 +194,10 @@ __global__ __launch_bounds__(kSelThreads) void evict_select(Select A) {
     digits |= static_cast<uint32_t>(f.bin) << digit_shift(level);
     mask |= digit_mask(level) << digit_shift(level);
     want = f.left;
+    if (f.left == f.count) break;               // all that share these digits stay: the others need not be known
   }
+#pragma unroll
+  for (int e = 0; e < E; ++e) key[e] &= mask;
   int ties = 0;
   int64_t at = A.first;
   emit_kept<E>(key, j0, j1, digits, want, ties, at, dst, cnt, &total);
@@ -205,7 +210,7 @@ constexpr int kChunkKeys = 16;     // per thread and block
 template <int LEVEL>
 __global__ __launch_bounds__(kSelThreads) void evict_digit(Select A) {
   __shared__ int hist[kBins];
-  __shared__ int scratch[kWaves + 2];
+  __shared__ int scratch[kWaves + 3];
   __shared__ int2 cnt[kChunkKeys][kWaves], total;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int c = blockIdx.x;

@@ -174,6 +174,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char* base, int6
 // hoisted out of the loop over `row` each of them is a register.
 __device__ __forceinline__ void keep_in_loop(uint32_t& off, int64_t row) { asm("" : "+v"(off) : "s"(row)); }
 
+// Loads issued before this stay before it (everything but vector memory may cross):
+// the next tile's go out here, not where they are used.
+__device__ __forceinline__ void loads_go_out() { __builtin_amdgcn_sched_barrier(0x78F); }
+
 // 32 rows, one per lane (l & 31).
 template <int D, int DT>
 struct KeyRows {
@@ -371,8 +375,12 @@ __device__ void draft_apply(const Tree& A, int64_t slice, float (*t_s)[kTreeMaxN
 // ---------------------------------------------------------------------------
 // statistics
 
+// Waves per SIMD that the registers are held to, by the bytes of a row.
 template <int D, int DT, int NT>
-__global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
+constexpr int kStatWaves = Shape<D, DT>::kRow <= 128 ? 5 - NT : Shape<D, DT>::kRow <= 256 ? 4 - NT : 1;
+
+template <int D, int DT, int NT>
+__global__ __launch_bounds__(kTreeThreads, (kStatWaves<D, DT, NT>)) void tree_stats(Tree A) {
   using S = Shape<D, DT>;
   const int64_t slice = A.slice0 + blockIdx.y;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), l32 = lane & 31, h = lane >> 5;
@@ -405,6 +413,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stats(Tree A) {
     constexpr int kKind = decltype(kind)::value;
     asm volatile("" ::: "memory");                     // the queries stay in LDS (tree_apply)
     nxt.load(keys, row + step, end, lane);
+    loads_go_out();
     const int left = kKind == 0 ? 32 : static_cast<int>(end - row);
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
@@ -485,9 +494,12 @@ __device__ __forceinline__ u32x4 bits_frag(uint32_t mask, int s, int h) {
 
 template <int D, int DT, int NT> constexpr int kApplyDV = D == 256 && NT == 2 ? 128 : D;
 
-// Waves per SIMD that the registers are held to.
+// Waves per SIMD that the registers are held to.  One node tile at head_dim up to 64
+// takes V a tile ahead as K, at three waves: 128 slices of 16384 keys 97 -> 91 us, 16 of
+// 131072 91 -> 84 against four waves without; elsewhere the registers for it are a wave
+// (head_dim 128: 15 -> 18 us at 15 slices of 5003 keys).
 template <int D, int DT, int NT>
-constexpr int kApplyWaves = NT == 2 ? (DT != DT_F32 && D <= 64 ? 2 : 1) : D <= 64 ? 4 : D == 256 ? 1 : DT == DT_F32 ? 2 : 3;
+constexpr int kApplyWaves = NT == 2 ? (DT != DT_F32 && D <= 64 ? 2 : 1) : D <= 64 ? 3 : D == 256 ? 1 : DT == DT_F32 ? 2 : 3;
 
 template <int D, int DT, int NT>
 __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_apply(Tree A) {
@@ -495,6 +507,7 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
   constexpr int DV = kApplyDV<D, DT, NT>;
   using V = ValueRows<DV, DT>;
   constexpr int kParts = kBidParts<DT>;
+  constexpr bool kValuesAhead = D <= 64 && NT == 1;
   const int64_t slice = A.slice0 + blockIdx.y;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), l32 = lane & 31, h = lane >> 5;
   constexpr int kRedStride = DV + 1;
@@ -575,6 +588,9 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
 #pragma unroll
     for (int e = 0; e < V::E; ++e) acc[u][e] = floatx16{};
   }
+  const int d0 = static_cast<int>(blockIdx.z) * DV * S::kElt;
+  V val;
+  if constexpr (kValuesAhead) val.load(values, row, A.length, lane, S::kRow, d0);
   // One tile.  The last one of a slice may be partly past the end: a form of its own,
   // so that the others are straight code.
   auto tile = [&](auto last) {
@@ -584,8 +600,8 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
     asm volatile("" ::: "memory");
     const int left = kLast ? static_cast<int>(A.length - row) : 32;
     const float* com = com0 + row + 4 * h;
-    V val;
-    val.load(values, row, A.length, lane, S::kRow, static_cast<int>(blockIdx.z) * DV * S::kElt);
+    if constexpr (!kValuesAhead) val.load(values, row, A.length, lane, S::kRow, d0);
+    const V now = val;
     // committed + eps of this lane's keys in step 2's layout
     floatx16 c0;
     if constexpr (!kLast) {
@@ -639,6 +655,7 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
       }
     }
     cur.load(keys, row + step, A.length, lane);
+    if constexpr (kValuesAhead) val.load(values, row + step, A.length, lane, S::kRow, d0);
 #pragma unroll
     for (int i = 0; i < 16; ++i) c0[i] += kEps;
     // steps 2 and 3
@@ -664,7 +681,7 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
         for (int i = 0; i < 16; ++i)
 #pragma unroll
           for (int e = 0; e < V::E; ++e)
-            acc[u][e] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(val.w[i][e]), sh[i], acc[u][e], 0, 0, 0);
+            acc[u][e] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(now.w[i][e]), sh[i], acc[u][e], 0, 0, 0);
       } else {
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
@@ -675,7 +692,7 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
             b[e] = DT == DT_BF16 ? pack_bf16(x, y) : pack_f16(x * kShareScale<DT>, y * kShareScale<DT>);
           }
 #pragma unroll
-          for (int e = 0; e < V::E; ++e) acc[u][e] = mma_piece<DT>(val.frag(e, st), b, acc[u][e]);
+          for (int e = 0; e < V::E; ++e) acc[u][e] = mma_piece<DT>(now.frag(e, st), b, acc[u][e]);
         }
       }
     }
@@ -829,6 +846,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
     const int64_t j = row + l32;
     const float c = j < A.length ? crow[j] : 0.f;
     nxt.load(keys, row + step, A.length, lane);
+    loads_go_out();
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
@@ -896,12 +914,12 @@ struct TreePlan {
   size_t part, out, sum, aff, seen, total;
   TreePlan(int64_t n, int64_t length, int64_t nodes, int head_dim, int apply_waves) {
     // The places to fill are the CUs times the workgroups that each holds, or a
-    // multiple: several short rounds hide one another's start and end.  us for 128
-    // slices of 65536 keys, 64 nodes: statistics with 512, 768, 1024, 2048 places 203,
-    // 196, 238, 198 (768 at once); shares with 512, 768, 1024, 2048 476, 462, 426, 439
-    // (512 at once).  128 slices of 16384 keys, 32 nodes: statistics 55, 55, 56, 52
-    // (2048 at once), shares 128, 105, 101, 104 (1024 at once).
-    nstat = tree_split(n, length, kCUs * (nodes > kTileNodes ? 3 : 8));
+    // multiple: several short rounds hide one another's start and end.  us with 3, 4, 6,
+    // 8, 12, 16 places a CU, 128 slices of 65536 keys and 64 nodes (3 at once):
+    // statistics 201, 245, 185, 198, 188, 205; 128 of 16384, 32 nodes (6 at once): 55, 57,
+    // 53, 59, 51, 56.  Shares of the first with 2, 3, 4, 8 places (2 at once): 464, 462,
+    // 426, 439.
+    nstat = tree_split(n, length, kCUs * (nodes > kTileNodes ? 6 : 12));
     nchunk = tree_split(n, length, kCUs * (nodes > kTileNodes && apply_waves == 2 ? 4 : apply_waves));
     const size_t rows = static_cast<size_t>(n * (nchunk + 1) * nodes);
     part = 0;
@@ -940,8 +958,9 @@ int launch_step(const TreeArgs& a) {
 template <int D, int DT, int NT>
 int launch_accept(const TreeArgs& a) {
   Tree A = tree_of(a);
-  // 128 slices of 65536 keys with 512, 768, 1024, 2048, 4096 places: 296, 258, 236, 238, 230 us
-  A.nchunk = tree_split(a.n, a.length, kCUs * 8);
+  // us for 128 slices of 65536 keys with 3, 4, 8, 16, 24, 32 places a CU: 263, 245, 262,
+  // 244, 233, 230; 24 slices of 9001 keys 11 with any
+  A.nchunk = tree_split(a.n, a.length, kCUs * 24);
   A.demand = a.committed;
   A.k_move = a.k_cache;
   A.v_move = a.v_cache;
