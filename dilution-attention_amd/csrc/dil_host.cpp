@@ -421,9 +421,9 @@ int64_t check_nodes(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
     throw py::value_error("a tree holds 1 to 64 drafted nodes, got " + std::to_string(nodes));
   const int64_t capacity = check_cache(q, k, v, committed);
   check_head_dim(q.size(3), nullptr);
-  if (length < 0 || length + nodes > capacity)
-    throw py::value_error("drafted rows [" + std::to_string(length) + ", " + std::to_string(length + nodes) +
-                          ") outside cache capacity " + std::to_string(capacity));
+  if (length < 0 || length > capacity - nodes)
+    throw py::value_error(std::to_string(nodes) + " drafted rows from " + std::to_string(length) +
+                          " on outside cache capacity " + std::to_string(capacity));
   cache_type(k, v);
   if (q.scalar_type() != k.scalar_type()) throw py::value_error("q must have the caches' dtype");
   return capacity;

@@ -797,6 +797,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
   stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return node_s[r]; });
   const char* keys = static_cast<const char*>(A.k) + slice * A.cap * S::kRow;
   if (blockIdx.x == 0) {
+    bool moved = false;
     // wave w: the accepted positions 32 w + [0, 32), one per lane, and the bids of the
     // accepted nodes from that one on
     __syncthreads();
@@ -821,6 +822,8 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
       if (h == 0 && c < A.count) crow[A.length + c] = node < 0 ? 0.f : sum;
     }
     for (void* cache : {A.k_move, A.v_move}) {
+      if (moved && A.v_move == A.k_move) break;          // K and V in one buffer: once
+      moved = true;
       u32x4* rows = reinterpret_cast<u32x4*>(static_cast<char*>(cache) + (slice * A.cap + A.length) * S::kRow);
       __syncthreads();
       for (int u = t; u < A.count * kUnits; u += kTreeThreads)

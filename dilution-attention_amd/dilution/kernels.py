@@ -482,7 +482,9 @@ def dilution_tree_step(
     its ancestors add: its output is what ``dilution_decode_step`` gives after
     decoding its path token by token, up to rounding.  It does not depend on the
     nodes that it does not see.  Nothing in the cache changes:
-    ``dilution_tree_accept`` takes a path of the tree into it.
+    ``dilution_tree_accept`` takes a path of the tree into it.  The same call gives
+    the same bits; a slice's bits may differ in calls of another B * H, length or N,
+    which pick the order of its sums.
 
     With return_aux also returns dict(lse): the (B, H, N) fp32 row statistics,
     p_ij = 2^(log2(e) q_i.k_j / sqrt(D) - lse_i), +inf for absent nodes.

@@ -133,6 +133,16 @@ def test_evict_moves_every_bit():
     assert torch.equal(ko.view(torch.int16), want)
 
 
+def test_evict_of_many_slices():
+    """More slices than one grid's y takes."""
+    from dilution import kernels
+
+    k, v, com = _cache(9, 4400, 15, 6, 16, BF16)
+    got = kernels.dilution_evict(k, v, com, 6, 3, 1, 1, 4)
+    sel = [0, 2345, 4369, 4399]
+    _check(k[sel], v[sel], com[sel], 6, 3, 1, 1, 4, [t[sel] for t in got])
+
+
 def test_evict_empty_batch():
     from dilution import kernels
 

@@ -34,7 +34,7 @@ def test_tree_step_refusals():
         step(q, k, v, com, 36, torch.zeros(3, 4, dtype=torch.int32) - 1)
     with pytest.raises(ValueError, match="int32 or int64"):
         step(q, k, v, com, 36, torch.zeros(4) - 1)
-    for length in (37, -1, 1 << 40):
+    for length in (37, -1, 1 << 40, (1 << 63) - 1):
         with pytest.raises(ValueError, match="capacity"):
             step(q, k, v, com, length, PARENTS)
     with pytest.raises(ValueError, match="dtype"):

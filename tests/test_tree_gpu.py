@@ -335,6 +335,58 @@ def test_accept_of_an_absent_node_adds_nothing_to_the_cached_keys():
     assert torch.equal(com[:, :, :length], c0[:, :, :length])
 
 
+def test_accept_with_keys_and_values_in_one_buffer():
+    """A cache whose values are its keys: the rows move once."""
+    from dilution import kernels
+
+    length, n = 70, 8
+    q, k, _, com = _make(23, 1, 2, length, n, 64, BF16)
+    tree = [-1, 0, 0, 1, 2, 4, 5, 6]
+    _, aux = kernels.dilution_tree_step(q, k, k, com, length, tree, return_aux=True)
+    k0 = k.clone()
+    kernels.dilution_tree_accept(q, k, k, com, length, aux["lse"], [0, 2, 4, 5, 6])
+    for r, node in enumerate([0, 2, 4, 5, 6]):
+        assert torch.equal(k[:, :, length + r], k0[:, :, length + node])
+
+
+def test_a_row_without_bids_is_nan_as_its_softmax():
+    """Every score of node 1 is -inf: no bids; the others stay."""
+    from dilution import kernels
+
+    length, n = 40, 4
+    q, k, v, com = _make(24, 1, 1, length, n, 64, F32)
+    k[:, :, :, 0] = k[:, :, :, 0].abs() + 0.5
+    clean = kernels.dilution_tree_step(q, k, v, com, length, [-1, -1, 0, 1])
+    q[:, :, 1] = 0.0
+    q[:, :, 1, 0] = -float("inf")
+    out, aux = kernels.dilution_tree_step(q, k, v, com, length, [-1, -1, 0, 1], return_aux=True)
+    assert bool(torch.isnan(out[:, :, [1, 3]]).all())
+    assert torch.equal(out[:, :, [0, 2]], clean[:, :, [0, 2]])
+
+
+def test_many_slices_and_a_broadcast_query():
+    """More slices than one grid takes, and queries that the heads share (a stride of 0)."""
+    from dilution import kernels
+
+    b, h, length, n, d = 4400, 15, 3, 2, 16
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn(b, 1, n, d, generator=g, device="cuda").to(BF16).expand(b, h, n, d)
+    k = torch.randn(b, h, length + n, d, generator=g, device="cuda").to(BF16)
+    v = torch.randn(b, h, length + n, d, generator=g, device="cuda").to(BF16)
+    com = torch.rand(b, h, length + n, generator=g, device="cuda")
+    com[:, :, length:] = 0
+    out, aux = kernels.dilution_tree_step(q, k, v, com, length, [-1, 0], return_aux=True)
+    for i, j in ((0, 0), (2345, 7), (4369, 1), (4399, 14)):
+        one = slice(i, i + 1)
+        _check_step(q[one, j : j + 1], k[one, j : j + 1], v[one, j : j + 1], com[one, j : j + 1], length, [[-1, 0]],
+                    out[one, j : j + 1], aux["lse"][one, j : j + 1])
+    c0 = com.clone()
+    kernels.dilution_tree_accept(q, k, v, com, length, aux["lse"], [0, 1])
+    for i, j in ((0, 0), (4399, 14)):
+        want, _ = ref.accept_f64(q[i, j], k[i, j], c0[i, j], length, aux["lse"][i, j], [0, 1])
+        assert (com[i, j].double() - want).abs().max().item() < 1e-5
+
+
 # ---------------------------------------------------------------------------
 # streams, graphs, far offsets
 
