@@ -511,13 +511,16 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
   const int64_t slice = A.slice0 + blockIdx.y;
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), l32 = lane & 31, h = lane >> 5;
   constexpr int kRedStride = DV + 1;
+  // a region of LDS for every wave's sums where that takes no workgroup off the CU
+  constexpr int kRegionBytes = NT * kTileNodes * kRedStride * 4;
+  constexpr int kRegions = kTreeWaves * kRegionBytes * kApplyWaves<D, DT, NT> <= 144 * 1024 ? kTreeWaves : 2;
   __shared__ union {
     u32x4 q[NT * S::kPieces * 64];
     struct {
       float p[kTreeMaxNodes][kTreeMaxNodes];
       float sh[kTreeMaxNodes][kShareStride];
     } draft;
-    float red[NT * kTileNodes][kRedStride];
+    float red[kRegions][NT * kTileNodes][kRedStride];
     float2 st[kTreeWaves][kTreeMaxNodes];
   } s;
   __shared__ uint64_t seen_s[kTreeMaxNodes];
@@ -705,9 +708,10 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
     const float o = ssum[u] + __shfl_xor(ssum[u], 32, 64);
     if (h == 0) sum_s[wave][u * kTileNodes + l32] = o;
   }
-  for (int w = 0; w < kTreeWaves; ++w) {
+#pragma unroll
+  for (int w = 0; w < kTreeWaves; w += kRegions) {
     __syncthreads();
-    if (wave != w) continue;
+    if (wave < w || wave >= w + kRegions) continue;
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -716,16 +720,20 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
         for (int i = 0; i < 16; ++i) {
           const int d = V::E * acc_row(i, h) + e;
           if (DV >= 32 || d < DV) {
-            float* dst = &s.red[u * kTileNodes + l32][d];
-            *dst = (w == 0 ? 0.f : *dst) + acc[u][e][i];
+            float* dst = &s.red[wave - w][u * kTileNodes + l32][d];
+            *dst = w == 0 ? acc[u][e][i] : *dst + acc[u][e][i];
           }
         }
   }
   __syncthreads();
   const int64_t p0 = (slice * (A.nchunk + 1) + blockIdx.x) * A.nodes;
   constexpr float kUnscale = 1.f / kShareScale<DT>;
-  for (int o = t; o < A.nodes * DV; o += kTreeThreads)
-    A.part_out[(p0 + o / DV) * D + blockIdx.z * DV + o % DV] = s.red[o / DV][o % DV] * kUnscale;
+  for (int o = t; o < A.nodes * DV; o += kTreeThreads) {
+    float x = s.red[0][o / DV][o % DV];
+#pragma unroll
+    for (int w = 1; w < kRegions; ++w) x += s.red[w][o / DV][o % DV];
+    A.part_out[(p0 + o / DV) * D + blockIdx.z * DV + o % DV] = x * kUnscale;
+  }
   if (blockIdx.z == 0 && t < A.nodes) {
     float x = 0.f;
 #pragma unroll
@@ -874,9 +882,12 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
 
 // The workgroups of a slice over its cached keys: those of all slices (one more each,
 // for the drafted keys) fill whole rounds of the `slots` that the GPU holds at once,
-// as few rounds as fill 15/16 of their places (of 4 rounds the best).  At least 256
-// keys each.
-int tree_split(int64_t n, int64_t length, int64_t slots) {
+// as few rounds as fill 15/16 of their places (of 4 rounds the best).  At least
+// `least` keys each: 256 (16 slices of 1000 keys, 128, 256, 512, 1024 of them: shares
+// 7.2, 7.4, 10.2, 18.3 us; 15 of 5003 at head_dim 128 16, 15, 18, 27), of fp32 caches
+// 128, whose tiles take four times the matrix cycles (16 of 4096 keys 16, 19, 24, 41).
+constexpr int64_t least_keys(int dtype) { return dtype == DT_F32 ? kBlockRows : 2 * kBlockRows; }
+int tree_split(int64_t n, int64_t length, int64_t slots, int64_t least) {
   if (length < 1) return 0;
   int64_t best = 1, best_fill = -1;
   for (int64_t rounds = (2 * n + slots - 1) / slots, i = 0; i < 4 && best_fill < 960; ++rounds, ++i) {
@@ -886,7 +897,7 @@ int tree_split(int64_t n, int64_t length, int64_t slots) {
       best_fill = fill;
     }
   }
-  const int64_t most = (length + 2 * kBlockRows - 1) / (2 * kBlockRows);
+  const int64_t most = (length + least - 1) / least;
   return static_cast<int>(best < most ? best : most);
 }
 constexpr int64_t kCUs = 256;
@@ -915,15 +926,15 @@ Tree tree_of(const TreeArgs& a) {
 struct TreePlan {
   int nstat, nchunk;
   size_t part, out, sum, aff, seen, total;
-  TreePlan(int64_t n, int64_t length, int64_t nodes, int head_dim, int apply_waves) {
+  TreePlan(int64_t n, int64_t length, int64_t nodes, int head_dim, int dtype, int apply_waves) {
     // The places to fill are the CUs times the workgroups that each holds, or a
     // multiple: several short rounds hide one another's start and end.  us with 3, 4, 6,
     // 8, 12, 16 places a CU, 128 slices of 65536 keys and 64 nodes (3 at once):
     // statistics 201, 245, 185, 198, 188, 205; 128 of 16384, 32 nodes (6 at once): 55, 57,
     // 53, 59, 51, 56.  Shares of the first with 2, 3, 4, 8 places (2 at once): 464, 462,
     // 426, 439.
-    nstat = tree_split(n, length, kCUs * (nodes > kTileNodes ? 6 : 12));
-    nchunk = tree_split(n, length, kCUs * (nodes > kTileNodes && apply_waves == 2 ? 4 : apply_waves));
+    nstat = tree_split(n, length, kCUs * (nodes > kTileNodes ? 6 : 12), least_keys(dtype));
+    nchunk = tree_split(n, length, kCUs * (nodes > kTileNodes && apply_waves == 2 ? 4 : apply_waves), least_keys(dtype));
     const size_t rows = static_cast<size_t>(n * (nchunk + 1) * nodes);
     part = 0;
     out = part + align_up(sizeof(float2) * n * (nstat + 1) * nodes);
@@ -937,7 +948,7 @@ struct TreePlan {
 template <int D, int DT, int NT>
 int launch_step(const TreeArgs& a) {
   Tree A = tree_of(a);
-  const TreePlan w(a.n, a.length, a.nodes, D, kApplyWaves<D, DT, NT>);
+  const TreePlan w(a.n, a.length, a.nodes, D, DT, kApplyWaves<D, DT, NT>);
   A.nstat = w.nstat;
   A.nchunk = w.nchunk;
   char* ws = static_cast<char*>(a.workspace);
@@ -963,7 +974,7 @@ int launch_accept(const TreeArgs& a) {
   Tree A = tree_of(a);
   // us for 128 slices of 65536 keys with 3, 4, 8, 16, 24, 32 places a CU: 263, 245, 262,
   // 244, 233, 230; 24 slices of 9001 keys 11 with any
-  A.nchunk = tree_split(a.n, a.length, kCUs * 24);
+  A.nchunk = tree_split(a.n, a.length, kCUs * 24, 2 * kBlockRows);
   A.demand = a.committed;
   A.k_move = a.k_cache;
   A.v_move = a.v_cache;
@@ -1009,7 +1020,7 @@ int64_t tree_workspace_bytes(int64_t n, int64_t length, int64_t nodes, int head_
   if (n < 1 || length < 0 || nodes < 1 || nodes > kTreeMaxNodes) return 0;
   int64_t bytes = 0;
   with_shape(head_dim, dtype, static_cast<int>(nodes), [&](auto d, auto t, auto nt) {
-    bytes = static_cast<int64_t>(TreePlan(n, length, nodes, d(), kApplyWaves<d(), t(), nt()>).total);
+    bytes = static_cast<int64_t>(TreePlan(n, length, nodes, d(), t(), kApplyWaves<d(), t(), nt()>).total);
     return 0;
   });
   return bytes;
