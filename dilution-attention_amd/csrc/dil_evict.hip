@@ -8,7 +8,8 @@
 // and of its equals the first that are wanted.
 //
 //   evict_select  (slices)              up to 32768 keys between: the slice in one
-//                                       workgroup, its keys in registers
+//                                       workgroup, its keys in registers (and its rows
+//                                       moved there, where they are few)
 //   evict_digit   (chunks x slices)     longer: four launches, each of them reads the
 //                                       demand once; a chunk's counts go through memory
 //   evict_move    (row blocks x slices) K, V and demand rows to their places, zero
@@ -142,6 +143,18 @@ __device__ __forceinline__ void emit_ends(int32_t* dst, int64_t length, int64_t 
   for (int64_t j = threadIdx.x; j < recent; j += kSelThreads) dst[keep - recent + j] = static_cast<int32_t>(length - recent + j);
 }
 
+// Where the rows go; a row is 2^shift units of 16 bytes.
+struct Move {
+  const u32x4* k;
+  const u32x4* v;
+  u32x4* ko;
+  u32x4* vo;
+  float* co;
+  int64_t out_cap;
+  int shift;
+  bool here;                       // evict_select moves the rows itself
+};
+
 struct Select {
   const float* committed;
   int64_t cap, length, keep, first, recent;
@@ -154,7 +167,41 @@ struct Select {
   int64_t level_stride;
   int4* state;                     // (n): after level k the digits found so far, and how many equals are wanted
   int* before;                     // (n, chunks): keys above the digits found so far in the chunks before
+  Move m;
 };
+
+// Units u0, u0 + stride, ... (kMoveUnits of them, K and V of all in flight) of an
+// output slice.
+constexpr int kMoveUnits = 4;
+
+__device__ __forceinline__ void move_units(const Move& m, const float* committed, int64_t cap, const int32_t* index, int64_t keep,
+                                           int64_t slice, int64_t u0, int64_t stride) {
+  const int64_t units = m.out_cap << m.shift;
+  const int part = (1 << m.shift) - 1;
+  u32x4 x[kMoveUnits], y[kMoveUnits];
+  float c[kMoveUnits];
+#pragma unroll
+  for (int i = 0; i < kMoveUnits; ++i) {
+    const int64_t u = u0 + i * stride, r = u >> m.shift;
+    x[i] = y[i] = u32x4{0, 0, 0, 0};
+    c[i] = 0.f;
+    if (r < keep) {
+      const int64_t row = slice * cap + index[slice * keep + r], src = (row << m.shift) + (u & part);
+      x[i] = m.k[src];
+      y[i] = m.v[src];
+      if ((u & part) == 0) c[i] = committed[row];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kMoveUnits; ++i) {
+    const int64_t u = u0 + i * stride;
+    if (u >= units) return;
+    const int64_t to = slice * units + u;
+    m.ko[to] = x[i];
+    m.vo[to] = y[i];
+    if ((u & part) == 0) m.co[slice * m.out_cap + (u >> m.shift)] = c[i];
+  }
+}
 
 template <int E>
 __device__ __forceinline__ void load_keys(uint32_t (&key)[E], const float* row, int64_t j0, int64_t j1) {
@@ -177,7 +224,17 @@ __global__ __launch_bounds__(kSelThreads) void evict_select(Select A) {
   const int64_t j0 = A.first, j1 = A.length - A.recent;
   int want = static_cast<int>(A.keep - A.first - A.recent);
   emit_ends(dst, A.length, A.keep, A.first, A.recent);
-  if (want == 0) return;                        // the same in every thread
+  auto move = [&] {
+    if (!A.m.here) return;
+    __syncthreads();                            // the positions are written
+    const int64_t units = A.m.out_cap << A.m.shift;
+    for (int64_t u = t; u < units; u += kSelThreads * kMoveUnits)
+      move_units(A.m, A.committed, A.cap, A.index, A.keep, slice, u, kSelThreads);
+  };
+  if (want == 0) {                              // the same in every thread
+    move();
+    return;
+  }
   uint32_t key[E];
   load_keys(key, A.committed + slice * A.cap, j0, j1);
   uint32_t digits = 0, mask = 0;
@@ -201,6 +258,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select(Select A) {
   int ties = 0;
   int64_t at = A.first;
   emit_kept<E>(key, j0, j1, digits, want, ties, at, dst, cnt, &total);
+  move();
 }
 
 constexpr int kChunkKeys = 16;     // per thread and block
@@ -287,41 +345,10 @@ __global__ __launch_bounds__(kSelThreads) void evict_digit(Select A) {
   }
 }
 
-// 16-byte units of the output slice, kMoveUnits a thread (K and V of all of them in
-// flight); a row is 2^shift units.
-constexpr int kMoveUnits = 4;
-
-__global__ __launch_bounds__(kMoveThreads) void evict_move(const u32x4* __restrict__ k, const u32x4* __restrict__ v,
-                                                           const float* __restrict__ committed, int64_t cap,
-                                                           const int32_t* __restrict__ index, int64_t keep, int64_t out_cap,
-                                                           int shift, u32x4* __restrict__ ko, u32x4* __restrict__ vo,
-                                                           float* __restrict__ co, int64_t slice0) {
-  const int64_t slice = slice0 + blockIdx.y, units = out_cap << shift;
-  const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (kMoveThreads * kMoveUnits) + threadIdx.x;
-  const int part = (1 << shift) - 1;
-  u32x4 x[kMoveUnits], y[kMoveUnits];
-  float c[kMoveUnits];
-#pragma unroll
-  for (int i = 0; i < kMoveUnits; ++i) {
-    const int64_t u = u0 + i * kMoveThreads, r = u >> shift;
-    x[i] = y[i] = u32x4{0, 0, 0, 0};
-    c[i] = 0.f;
-    if (r < keep) {
-      const int64_t row = slice * cap + index[slice * keep + r], src = (row << shift) + (u & part);
-      x[i] = k[src];
-      y[i] = v[src];
-      if ((u & part) == 0) c[i] = committed[row];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kMoveUnits; ++i) {
-    const int64_t u = u0 + i * kMoveThreads;
-    if (u >= units) return;
-    const int64_t to = slice * units + u;
-    ko[to] = x[i];
-    vo[to] = y[i];
-    if ((u & part) == 0) co[slice * out_cap + (u >> shift)] = c[i];
-  }
+__global__ __launch_bounds__(kMoveThreads) void evict_move(Move m, const float* committed, int64_t cap, const int32_t* index,
+                                                           int64_t keep, int64_t slice0) {
+  move_units(m, committed, cap, index, keep, slice0 + blockIdx.y,
+             static_cast<int64_t>(blockIdx.x) * (kMoveThreads * kMoveUnits) + threadIdx.x, kMoveThreads);
 }
 
 }  // namespace
@@ -360,14 +387,26 @@ int64_t evict_workspace_bytes(int64_t n, int64_t length, int64_t keep) {
 int evict(const EvictArgs& a) {
   hipStream_t st = static_cast<hipStream_t>(a.stream);
   const int64_t keys = a.length - a.first - a.recent;
-  Select S{a.committed, a.cap, a.length, a.keep, a.first, a.recent, a.index, 0, 0, 0, nullptr, 0, nullptr, nullptr};
-  if (keys <= kOneMax || a.keep == a.first + a.recent) {
+  int shift = 0;                                           // head_dim is a power of two
+  while (16 << shift < a.head_dim * (a.dtype == DT_F32 ? 4 : 2)) ++shift;
+  const bool one = keys <= kOneMax || a.keep == a.first + a.recent;
+  // Up to 64 KB of K rows a slice the selecting workgroup moves them itself and saves
+  // the launch; above, a launch of its own has more workgroups for them.  us a call, own
+  // launch -> here: 16 slices of 16, 32, 64, 128 KB 10.7 -> 8.4, 10.6 -> 8.5, 10.6 -> 9.5, 12.1
+  // -> 13.2; 64 slices 10.6 -> 8.6, 10.7 -> 9.2, 11.7 -> 11.3, 15.4 -> 15.7; 256 slices 11.9 -> 9.3,
+  // 14.4 -> 11.5, 19.3 -> 16.8, 34.7 -> 33.1.
+  constexpr int64_t kHereUnits = 4096;
+  const bool here = one && (a.out_cap << shift) <= kHereUnits;
+  Select S{a.committed, a.cap, a.length, a.keep, a.first, a.recent, a.index, 0, 0, 0, nullptr, 0, nullptr, nullptr,
+           Move{static_cast<const u32x4*>(a.k_cache), static_cast<const u32x4*>(a.v_cache), static_cast<u32x4*>(a.k_out),
+                static_cast<u32x4*>(a.v_out), a.committed_out, a.out_cap, shift, here}};
+  if (one) {
     const unsigned n = static_cast<unsigned>(a.n);
-    auto one = [&](auto e) { DIL_TIMED("evict_select", st, (evict_select<e()><<<dim3(n), kSelThreads, 0, st>>>(S))); };
-    if (keys <= 4 * kSelThreads || a.keep == a.first + a.recent) one(std::integral_constant<int, 4>{});
-    else if (keys <= 8 * kSelThreads) one(std::integral_constant<int, 8>{});
-    else if (keys <= 16 * kSelThreads) one(std::integral_constant<int, 16>{});
-    else one(std::integral_constant<int, 32>{});
+    auto select = [&](auto e) { DIL_TIMED("evict_select", st, (evict_select<e()><<<dim3(n), kSelThreads, 0, st>>>(S))); };
+    if (keys <= 4 * kSelThreads || a.keep == a.first + a.recent) select(std::integral_constant<int, 4>{});
+    else if (keys <= 8 * kSelThreads) select(std::integral_constant<int, 8>{});
+    else if (keys <= 16 * kSelThreads) select(std::integral_constant<int, 16>{});
+    else select(std::integral_constant<int, 32>{});
   } else {
     const EvictScratch w(a.n, a.length);
     char* ws = static_cast<char*>(a.workspace);
@@ -386,15 +425,14 @@ int evict(const EvictArgs& a) {
       DIL_TIMED("evict_digit3", st, (evict_digit<3><<<grid, kSelThreads, 0, st>>>(S)));
     });
   }
-  int shift = 0;                                           // head_dim is a power of two
-  while (16 << shift < a.head_dim * (a.dtype == DT_F32 ? 4 : 2)) ++shift;
-  const int64_t blocks = ((a.out_cap << shift) + kMoveThreads * kMoveUnits - 1) / (kMoveThreads * kMoveUnits);
-  slice_batches(a.n, [&](int64_t s0, unsigned ns) {
-    DIL_TIMED("evict_move", st,
-              (evict_move<<<dim3(static_cast<unsigned>(blocks), ns), kMoveThreads, 0, st>>>(
-                  static_cast<const u32x4*>(a.k_cache), static_cast<const u32x4*>(a.v_cache), a.committed, a.cap, a.index, a.keep,
-                  a.out_cap, shift, static_cast<u32x4*>(a.k_out), static_cast<u32x4*>(a.v_out), a.committed_out, s0)));
-  });
+  if (!here) {
+    const int64_t blocks = ((a.out_cap << shift) + kMoveThreads * kMoveUnits - 1) / (kMoveThreads * kMoveUnits);
+    slice_batches(a.n, [&](int64_t s0, unsigned ns) {
+      DIL_TIMED("evict_move", st,
+                (evict_move<<<dim3(static_cast<unsigned>(blocks), ns), kMoveThreads, 0, st>>>(S.m, a.committed, a.cap, a.index,
+                                                                                    a.keep, s0)));
+    });
+  }
   return static_cast<int>(hipGetLastError());
 }
 

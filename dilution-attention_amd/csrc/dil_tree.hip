@@ -148,9 +148,9 @@ __device__ __forceinline__ void stage_queries(u32x4* q_s, const Tree& A, int64_t
 }
 
 // Workgroup c of a slice's `chunks` takes the blocks of 128 rows c, c + chunks, ...,
-// its waves 32 rows each: the GPU reads one stretch of every slice at a time.  (With
-// a stretch of its own for every workgroup the statistics of 128 slices of 65536 keys
-// took 193 to 235 us by the stretch's length.)  All uniform in a wave.
+// its waves 32 rows each, all uniform in a wave: the workgroups' shares differ by one
+// block at most, and no resource spans more than 32 rows, whatever the length.  (A
+// stretch of its own for every workgroup takes the same time.)
 constexpr int kBlockRows = kTreeWaves * 32;
 
 // An address that is the same in every lane, in scalar registers.

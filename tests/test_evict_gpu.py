@@ -63,6 +63,9 @@ SHAPES = [
     (1, 1, 1048600, 1048600, 400000, 6, 18, None, 16, BF16),   # 64 full chunks between, of a length that takes fewer
     (1, 1, 1100000, 1100000, 700001, 0, 0, None, 16, BF16),    # chunks of two blocks
     (1, 2, 50000, 50000, 50000, 0, 0, None, 16, BF16),
+    (2, 2, 1000, 900, 500, 4, 8, 512, 64, BF16),               # the most rows that the selection moves, and one more
+    (2, 2, 1000, 900, 500, 4, 8, 513, 64, BF16),
+    (2, 2, 1000, 900, 12, 4, 8, 512, 64, BF16),
     (1, 2, 50000, 50000, 40, 20, 20, None, 16, BF16),
     (16, 16, 3000, 2999, 1000, 4, 100, 1064, 64, BF16),
 ]
