@@ -11,6 +11,7 @@
 //   tree_apply   joins the chunks' statistics; per chunk and node: the sums of
 //                share and of share v
 //   tree_finish  joins the chunks' sums
+//                (short or many slices: tree_apply alone, a workgroup per slice)
 //   tree_demand  the acceptance: committed_j += sum of the accepted nodes' p_ij
 //
 // The cached keys go through matrix instructions in tiles of 32 keys x 32 nodes
@@ -375,6 +376,59 @@ __device__ void draft_apply(const Tree& A, int64_t slice, float (*t_s)[kTreeMaxN
 // ---------------------------------------------------------------------------
 // statistics
 
+// One tile of 32 keys (the rows k) against every node: the lane's running maximum and
+// sum, node u * 32 + (l & 31).  kind 0: 32 cached keys; 1: the last `left` ones of a
+// slice; 2: the drafted keys from key0 on, masked, their affinities kept.
+template <int D, int DT, int NT, int KIND>
+__device__ __forceinline__ void stat_tile(const KeyRows<D, DT>& k, const u32x4* q_s, const Tree& A, int64_t slice,
+                                          const uint64_t* seen_s, int key0, int left, int lane, float (&m)[NT], float (&l)[NT]) {
+  using S = Shape<D, DT>;
+  const int l32 = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    floatx16 x = {};
+#pragma unroll
+    for (int g = 0; g < S::kPieces; ++g) x = mma_piece<DT>(k.p[g], q_s[(u * S::kPieces + g) * 64 + lane], x);
+    if constexpr (KIND == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (acc_row(i, h) >= left) x[i] = -INFINITY;
+    }
+    if constexpr (KIND == 2) {
+      const int node = u * kTileNodes + l32;
+      const uint64_t seen = seen_s[node];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = key0 + acc_row(i, h);
+        if (seen >> key & 1) A.aff[(slice * A.nodes + node) * A.nodes + key] = x[i] * A.scale;
+        else x[i] = -INFINITY;
+      }
+    }
+    float big = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) big = fmaxf(big, x[i]);
+    const float mn = fmaxf(m[u], big * A.scale);
+    const float mr = mn == -INFINITY ? 0.f : mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += fast_exp2(fmaf(x[i], A.scale, -mr));
+    l[u] = fmaf(l[u], fast_exp2(m[u] - mr), sum);
+    m[u] = mn;
+  }
+}
+
+// A wave's statistics, its lane halves (different keys of the same nodes) joined.
+template <int NT>
+__device__ __forceinline__ void stat_halves(const float (&m)[NT], const float (&l)[NT], int lane, float2* dst) {
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const float mo = __shfl_xor(m[u], 32, 64), lo = __shfl_xor(l[u], 32, 64);
+    const float mn = fmaxf(m[u], mo), mr = mn == -INFINITY ? 0.f : mn;
+    if (lane < 32)
+      dst[u * kTileNodes + lane] = make_float2(mn, l[u] * fast_exp2(m[u] - mr) + lo * fast_exp2(mo - mr));
+  }
+}
+
 // Waves per SIMD that the registers are held to, by the bytes of a row.
 template <int D, int DT, int NT>
 constexpr int kStatWaves = Shape<D, DT>::kRow <= 128 ? 5 - NT : Shape<D, DT>::kRow <= 256 ? 4 - NT : 1;
@@ -383,7 +437,7 @@ template <int D, int DT, int NT>
 __global__ __launch_bounds__(kTreeThreads, (kStatWaves<D, DT, NT>)) void tree_stats(Tree A) {
   using S = Shape<D, DT>;
   const int64_t slice = A.slice0 + blockIdx.y;
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), l32 = lane & 31, h = lane >> 5;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   __shared__ u32x4 q_s[NT * S::kPieces * 64];
   __shared__ uint64_t seen_s[kTreeMaxNodes];
   __shared__ float2 red[kTreeWaves][NT * kTileNodes];
@@ -408,44 +462,13 @@ __global__ __launch_bounds__(kTreeThreads, (kStatWaves<D, DT, NT>)) void tree_st
     m[u] = -INFINITY;
     l[u] = 0.f;
   }
-  // kind 0: 32 cached keys; 1: the last ones of a slice, fewer; 2: drafted keys, masked
   auto tile = [&](auto kind) {
     constexpr int kKind = decltype(kind)::value;
     asm volatile("" ::: "memory");                     // the queries stay in LDS (tree_apply)
     nxt.load(keys, row + step, end, lane);
     loads_go_out();
-    const int left = kKind == 0 ? 32 : static_cast<int>(end - row);
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      floatx16 x = {};
-#pragma unroll
-      for (int g = 0; g < S::kPieces; ++g) x = mma_piece<DT>(cur.p[g], q_s[(u * S::kPieces + g) * 64 + lane], x);
-      if constexpr (kKind == 1) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (acc_row(i, h) >= left) x[i] = -INFINITY;
-      }
-      if constexpr (kKind == 2) {
-        const int node = u * kTileNodes + l32, key0 = static_cast<int>(row - A.length);
-        const uint64_t seen = seen_s[node];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = key0 + acc_row(i, h);
-          if (seen >> key & 1) A.aff[(slice * A.nodes + node) * A.nodes + key] = x[i] * A.scale;
-          else x[i] = -INFINITY;
-        }
-      }
-      float big = x[0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) big = fmaxf(big, x[i]);
-      const float mn = fmaxf(m[u], big * A.scale);
-      const float mr = mn == -INFINITY ? 0.f : mn;
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum += fast_exp2(fmaf(x[i], A.scale, -mr));
-      l[u] = fmaf(l[u], fast_exp2(m[u] - mr), sum);
-      m[u] = mn;
-    }
+    stat_tile<D, DT, NT, kKind>(cur, q_s, A, slice, seen_s, static_cast<int>(row - A.length), static_cast<int>(end - row), lane,
+                                m, l);
     cur = nxt;
   };
   if (drafted) {
@@ -454,13 +477,7 @@ __global__ __launch_bounds__(kTreeThreads, (kStatWaves<D, DT, NT>)) void tree_st
     for (; row + 32 <= end; row += step) tile(std::integral_constant<int, 0>{});
     if (row < end) tile(std::integral_constant<int, 1>{});
   }
-  // the lane halves hold different keys of the same node; then the waves
-#pragma unroll
-  for (int u = 0; u < NT; ++u) {
-    const float mo = __shfl_xor(m[u], 32, 64), lo = __shfl_xor(l[u], 32, 64);
-    const float mn = fmaxf(m[u], mo), mr = mn == -INFINITY ? 0.f : mn;
-    if (h == 0) red[wave][u * kTileNodes + l32] = make_float2(mn, l[u] * fast_exp2(m[u] - mr) + lo * fast_exp2(mo - mr));
-  }
+  stat_halves<NT>(m, l, lane, red[wave]);
   __syncthreads();
   if (t < A.nodes) {
     float mn = -INFINITY, sum = 0.f;
@@ -501,7 +518,9 @@ template <int D, int DT, int NT> constexpr int kApplyDV = D == 256 && NT == 2 ? 
 template <int D, int DT, int NT>
 constexpr int kApplyWaves = NT == 2 ? (DT != DT_F32 && D <= 64 ? 2 : 1) : D <= 64 ? 3 : D == 256 ? 1 : DT == DT_F32 ? 2 : 3;
 
-template <int D, int DT, int NT>
+// ONE: a short slice in one workgroup and one launch, its statistics first and its outputs
+// last (one node tile; with two the drafted keys' sums spill beside the walk's).
+template <int D, int DT, int NT, bool ONE>
 __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_apply(Tree A) {
   using S = Shape<D, DT>;
   constexpr int DV = kApplyDV<D, DT, NT>;
@@ -526,9 +545,36 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
   __shared__ uint64_t seen_s[kTreeMaxNodes];
   __shared__ __attribute__((aligned(16))) float lse_s[kTreeMaxNodes];
   __shared__ float sum_s[kTreeWaves][NT * kTileNodes];
-  if (wave == 0) seen_s[lane] = A.seen[slice * kTreeMaxNodes + lane];
-  // the chunks' statistics joined: 64 nodes x 4 groups of entries
-  {
+  __shared__ float2 one_st[ONE ? kTreeWaves : 1][NT * kTileNodes];
+  const char* keys = static_cast<const char*>(A.k) + slice * A.cap * S::kRow;
+  KeyRows<D, DT> cur;
+  if constexpr (ONE) {
+    if (wave == 0) seen_s[lane] = nodes_seen(A.parents + slice / A.heads * A.parents_sb, A.nodes, lane);
+    stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return r < A.nodes ? r : -1; });
+    __syncthreads();
+    float m[NT], l[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      m[u] = -INFINITY;
+      l[u] = 0.f;
+    }
+    int64_t row = wave * 32;
+    for (; row + 32 <= A.length; row += kBlockRows) {
+      cur.load(keys, row, A.length, lane);
+      stat_tile<D, DT, NT, 0>(cur, s.q, A, slice, seen_s, 0, 32, lane, m, l);
+    }
+    if (row < A.length) {
+      cur.load(keys, row, A.length, lane);
+      stat_tile<D, DT, NT, 1>(cur, s.q, A, slice, seen_s, 0, static_cast<int>(A.length - row), lane, m, l);
+    }
+    if (wave * 32 < A.nodes) {
+      cur.load(keys, A.length + wave * 32, A.length + A.nodes, lane);
+      stat_tile<D, DT, NT, 2>(cur, s.q, A, slice, seen_s, wave * 32, 0, lane, m, l);
+    }
+    stat_halves<NT>(m, l, lane, one_st[wave]);
+  } else {
+    if (wave == 0) seen_s[lane] = A.seen[slice * kTreeMaxNodes + lane];
+    // the chunks' statistics joined: 64 nodes x 4 groups of entries
     float m = -INFINITY, l = 0.f;
     if (lane < A.nodes) {
       const float2* part = A.part + slice * (A.nstat + 1) * A.nodes + lane;
@@ -544,12 +590,16 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
   }
   __syncthreads();
   if (wave == 0) {
+    auto st = [&](int w) {
+      if constexpr (ONE) return lane < NT * kTileNodes ? one_st[w][lane] : make_float2(-INFINITY, 0.f);
+      else return s.st[w][lane];
+    };
     float mn = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kTreeWaves; ++w) mn = fmaxf(mn, s.st[w][lane].x);
+    for (int w = 0; w < kTreeWaves; ++w) mn = fmaxf(mn, st(w).x);
     const float mr = mn == -INFINITY ? 0.f : mn;
 #pragma unroll
-    for (int w = 0; w < kTreeWaves; ++w) l += s.st[w][lane].y * fast_exp2(s.st[w][lane].x - mr);
+    for (int w = 0; w < kTreeWaves; ++w) l += st(w).y * fast_exp2(st(w).x - mr);
     // a row of -inf alone has no bids: NaN, as its softmax
     const float lse = seen_s[lane] == 0 ? INFINITY : mn == -INFINITY ? NAN : mn + fast_log2(l);
     lse_s[lane] = lse;
@@ -558,15 +608,14 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
   __syncthreads();
   if (blockIdx.x == 0) {
     if (blockIdx.z == 0) draft_apply<D, DT>(A, slice, s.draft.p, s.draft.sh, seen_s, lse_s);
-    return;
+    if constexpr (!ONE) return;
+    __syncthreads();
   }
   stage_queries<D, DT, NT>(s.q, A, slice, [&](int r) { return r < A.nodes ? r : -1; });
-  const char* keys = static_cast<const char*>(A.k) + slice * A.cap * S::kRow;
   const char* values = static_cast<const char*>(A.v) + slice * A.cap * S::kRow;
-  int64_t row = static_cast<int64_t>(blockIdx.x - 1) * kBlockRows + wave * 32;
-  const int64_t step = static_cast<int64_t>(A.nchunk) * kBlockRows;
+  int64_t row = (ONE ? 0 : static_cast<int64_t>(blockIdx.x - 1) * kBlockRows) + wave * 32;
+  const int64_t step = ONE ? kBlockRows : static_cast<int64_t>(A.nchunk) * kBlockRows;
   const float* com0 = A.committed + slice * A.cap;
-  KeyRows<D, DT> cur;
   cur.load(keys, row, A.length, lane);
 
   // step 2's operands (a node sees itself: the sums include its own bid)
@@ -726,19 +775,33 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
         }
   }
   __syncthreads();
-  const int64_t p0 = (slice * (A.nchunk + 1) + blockIdx.x) * A.nodes;
   constexpr float kUnscale = 1.f / kShareScale<DT>;
-  for (int o = t; o < A.nodes * DV; o += kTreeThreads) {
+  auto sum_of = [&](int o) {
     float x = s.red[0][o / DV][o % DV];
 #pragma unroll
     for (int w = 1; w < kRegions; ++w) x += s.red[w][o / DV][o % DV];
-    A.part_out[(p0 + o / DV) * D + blockIdx.z * DV + o % DV] = x * kUnscale;
-  }
-  if (blockIdx.z == 0 && t < A.nodes) {
+    return x * kUnscale;
+  };
+  auto shares_of = [&](int i) {
     float x = 0.f;
 #pragma unroll
-    for (int w = 0; w < kTreeWaves; ++w) x += sum_s[w][t];
-    A.part_sum[p0 + t] = x;
+    for (int w = 0; w < kTreeWaves; ++w) x += sum_s[w][i];
+    return x;
+  };
+  const int64_t p0 = (slice * (A.nchunk + 1) + blockIdx.x) * A.nodes;    // ONE: the drafted keys' entry
+  if constexpr (ONE) {
+    const uint64_t bad = __ballot(lse_s[lane] != lse_s[lane]);
+    for (int o = t; o < A.nodes * DV; o += kTreeThreads) {
+      const int i = o / DV, d = o % DV;
+      const uint64_t seen = seen_s[i];
+      float x = 0.f;
+      if (seen != 0) x = (sum_of(o) + A.part_out[(p0 + i) * D + d]) / (shares_of(i) + A.part_sum[p0 + i] + kEps);
+      store_as(A.out, A.ov.slice(slice) + i * A.ov.sr + d, DT, (bad & seen) != 0 ? NAN : x);
+    }
+  } else {
+    for (int o = t; o < A.nodes * DV; o += kTreeThreads)
+      A.part_out[(p0 + o / DV) * D + blockIdx.z * DV + o % DV] = sum_of(o);
+    if (blockIdx.z == 0 && t < A.nodes) A.part_sum[p0 + t] = shares_of(t);
   }
 }
 
@@ -945,6 +1008,33 @@ struct TreePlan {
   }
 };
 
+// Whether a slice's whole step runs in one workgroup (one node tile): little work, where
+// two launches less count, or slices that fill the places on the GPU by themselves.
+// us a call, three launches -> one, 8 nodes, bf16 64 where nothing else stands:
+//   16 slices of 32, 128, 256, 512 keys 13.3 -> 11.2, 13.3 -> 11.6, 13.4 -> 13.5, 13.6 -> 17.1 (1 node
+//   12.9 -> 8.5, 13.6 -> 8.9, 13.8 -> 10.5, 13.6 -> 13.6); head_dim 16, 512 and 768 keys 13.2 -> 12.6,
+//   13.3 -> 14.5; head_dim 128, 32 keys 13.1 -> 13.3; fp32, 32 keys 14.2 -> 14.5
+//   256 keys: 128, 192, 256, 384, 512, 768, 900 slices 13.2 -> 13.9, 15.5 -> 14.3, 16.0 -> 14.4,
+//   19.3 -> 18.4, 26.5 -> 19.8, 33.1 -> 23.8, 40.2 -> 37.9
+//   1024 keys: 256, 384, 512, 768, 900 slices 27.8 -> 31.3, 42.2 -> 38.4, 47.6 -> 41.9, 74.3 -> 55.3,
+//   81.4 -> 88.5 (fp32 54 -> 55, 109 -> 77, 104 -> 83, 193 -> 128, 202 -> 172)
+//   16384 keys: 384, 512, 640, 768, 900, 1100, 1300 slices 494 -> 509, 577 -> 562, 681 -> 722,
+//   992 -> 786, 980 -> 1135, 1422 -> 1260, 1376 -> 1435 (head_dim 128, 4096 keys: 271 -> 253, 325 -> 276,
+//   405 -> 360, 542 -> 398, 571 -> 592, 775 -> 682, 800 -> 715)
+//   head_dim 256 (256 places), 1024 keys: 256, 320, 512, 768, 900 slices 102 -> 80, 111 -> 159,
+//   201 -> 179, 320 -> 263, 310 -> 335
+template <int D, int DT>
+bool tree_in_one(int64_t n, int64_t length, int64_t places) {
+  constexpr int64_t kRow = Shape<D, DT>::kRow;
+  if (kRow <= 128 && length * kRow <= 16384) return true;
+  if (n < 192) return false;
+  if (length <= 256) return true;
+  if (2 * n < places) return false;
+  if (D <= 128 && length <= 1024) return true;
+  const int64_t rounds = (n + places - 1) / places;          // the share of the rounds' places that the slices fill
+  return 100 * n >= (D <= 128 ? 70 : 95) * rounds * places;
+}
+
 template <int D, int DT, int NT>
 int launch_step(const TreeArgs& a) {
   Tree A = tree_of(a);
@@ -958,12 +1048,21 @@ int launch_step(const TreeArgs& a) {
   A.aff = reinterpret_cast<float*>(ws + w.aff);
   A.seen = reinterpret_cast<uint64_t*>(ws + w.seen);
   hipStream_t st = static_cast<hipStream_t>(a.stream);
+  if constexpr (NT == 1) {
+    if (tree_in_one<D, DT>(a.n, a.length, kCUs * kApplyWaves<D, DT, NT>)) {
+      slice_batches(a.n, [&](int64_t s0, unsigned ns) {
+        A.slice0 = s0;
+        DIL_TIMED("tree_one", st, (tree_apply<D, DT, NT, true><<<dim3(1, ns), kTreeThreads, 0, st>>>(A)));
+      });
+      return static_cast<int>(hipGetLastError());
+    }
+  }
   const unsigned chunks = static_cast<unsigned>(A.nchunk + 1);
   slice_batches(a.n, [&](int64_t s0, unsigned ns) {
     A.slice0 = s0;
     DIL_TIMED("tree_stats", st, (tree_stats<D, DT, NT><<<dim3(A.nstat + 1, ns), kTreeThreads, 0, st>>>(A)));
     DIL_TIMED("tree_apply", st,
-              (tree_apply<D, DT, NT><<<dim3(chunks, ns, D / kApplyDV<D, DT, NT>), kTreeThreads, 0, st>>>(A)));
+              (tree_apply<D, DT, NT, false><<<dim3(chunks, ns, D / kApplyDV<D, DT, NT>), kTreeThreads, 0, st>>>(A)));
     DIL_TIMED("tree_finish", st, (tree_finish<D, DT><<<dim3(A.nodes, ns), kTreeThreads, 0, st>>>(A)));
   });
   return static_cast<int>(hipGetLastError());

@@ -143,12 +143,12 @@ def test_wild_device_parents_are_absent_nodes():
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("length,n", [(333, 40), (333, 30), (100, 30), (0, 20)])
 @pytest.mark.parametrize("bad", ["nan_q", "inf_q", "nan_v", "nan_k"])
-def test_a_broken_branch_stays_its_own(bad):
+def test_a_broken_branch_stays_its_own(bad, length, n):
     """A node that holds NaN spoils itself and the nodes below it, and no bit of the others."""
     from dilution import kernels
 
-    length, n = 333, 40
     q, k, v, com = _make(7, 1, 2, length, n, 64, BF16, strided=False)
     parents = _tree("bushy", n, 9)
     clean, aux = kernels.dilution_tree_step(q, k, v, com, length, parents, return_aux=True)
@@ -235,6 +235,36 @@ def test_empty_batch():
     out, aux = kernels.dilution_tree_step(q[:0], k[:0], v[:0], com[:0], 20, [-1, 0, 0, 0], return_aux=True)
     assert out.shape == (0, 2, 4, 32)
     assert kernels.dilution_tree_accept(q[:0], k[:0], v[:0], com[:0], 20, aux["lse"], [0, 1]) == 22
+
+
+@pytest.mark.parametrize("b,h,length,n,d,dtype", [
+    (48, 16, 1501, 20, 64, BF16),          # as many slices as the GPU holds: a workgroup each
+    (16, 12, 255, 32, 64, BF16),           # 192 slices of few keys
+    (16, 12, 257, 32, 64, F16),            # and of more
+    (32, 16, 900, 9, 128, F16),
+    (48, 16, 333, 17, 32, F32),
+    (24, 16, 1000, 3, 64, F32),
+    (16, 16, 500, 12, 256, BF16),
+    (16, 16, 300, 5, 256, F32),
+    (30, 30, 700, 8, 16, BF16),
+    (48, 16, 600, 40, 64, BF16),           # two node tiles: never one workgroup
+])
+def test_many_slices_match_float64(b, h, length, n, d, dtype):
+    from dilution import kernels
+
+    q, k, v, com = _make(length, b, h, length, n, d, dtype, extra=1)
+    com[:, :, length:] = float("nan")
+    k[:, :, length + n :] = v[:, :, length + n :] = float("nan")
+    parents = [_tree("bushy", n, i) for i in range(b)]
+    parents[1] = parents[1][: n - 1] + [-2]
+    k[1, :, length + n - 1] = v[1, :, length + n - 1] = q[1, :, n - 1] = float("nan")
+    out, aux = kernels.dilution_tree_step(q, k, v, com, length, parents, return_aux=True)
+    for i, j in ((0, 0), (1, 1), (b // 2, h - 1), (b - 1, h - 1)):
+        one = slice(i, i + 1)
+        _check_step(q[one, j : j + 1], k[one, j : j + 1], v[one, j : j + 1], com[one, j : j + 1], length, [parents[i]],
+                    out[one, j : j + 1], aux["lse"][one, j : j + 1])
+    again = kernels.dilution_tree_step(q, k, v, com, length, parents)
+    assert torch.equal(again, out)
 
 
 # ---------------------------------------------------------------------------
