@@ -886,7 +886,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
         for (int i = 0; i < 16; ++i) {
           const int r = u * kTileNodes + acc_row(i, h);
           const float p = fast_exp2(fmaf(x[i], A.scale, -lse_s[r]));
-          if (r >= c && node_s[r] >= 0) sum += p;
+          if (r >= c && lse_s[r] != INFINITY) sum += p;         // no node, or an absent one: whatever its query holds
         }
       }
       sum += __shfl_xor(sum, 32, 64);

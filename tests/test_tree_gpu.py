@@ -365,6 +365,25 @@ def test_accept_of_an_absent_node_adds_nothing_to_the_cached_keys():
     assert torch.equal(com[:, :, :length], c0[:, :, :length])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_an_accepted_absent_node_brings_no_nan(dtype):
+    """Its query may hold anything: the demand of every position takes the present nodes' bids alone."""
+    from dilution import kernels
+
+    length, n, d = 50, 3, 64
+    q, k, v, com = _make(25, 1, 2, length, n, d, dtype, strided=False)
+    q[:, :, 1] = float("nan")
+    _, aux = kernels.dilution_tree_step(q, k, v, com, length, [-1, -2, 0], return_aux=True)
+    k0, c0 = k.clone(), com.clone()
+    kernels.dilution_tree_accept(q, k, v, com, length, aux["lse"], [0, 1, 2])
+    for j in range(2):
+        lse = aux["lse"][0, j].clone()
+        q2 = q[0, j].clone()
+        q2[1] = 0                                     # bids of 0: 2^(0 - inf)
+        want, _ = ref.accept_f64(q2, k0[0, j], c0[0, j], length, lse, [0, 1, 2])
+        assert (com[0, j, : length + 3].double() - want).abs().max().item() < 1e-5
+
+
 def test_accept_with_keys_and_values_in_one_buffer():
     """A cache whose values are its keys: the rows move once."""
     from dilution import kernels
