@@ -23,9 +23,9 @@
 //      and itself), which sum the demand down the tree for all nodes at once and
 //      leave a lane one node and 16 keys.  committed + eps is the accumulator's
 //      start value.
-//   3  the shares, in place, are the B operand of out^T += V^T share^T, whose A
-//      operand takes V rows as loaded, two head dims a register, regrouped by
-//      byte permutes.
+//   3  the shares, in place, are the B operand of out^T += V^T share^T (of a 16-bit
+//      type in two parts), whose A operand takes V rows as loaded, two head dims a
+//      register, regrouped by byte permutes.
 // The drafted keys (at most 64) are a workgroup of their own: there the masks are, and
 // what a node does not see it must not touch (NaN included), so their shares are
 // summed in plain fp32.
@@ -70,6 +70,23 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{lo, hi}, f16x2));
+}
+
+// Two shares as the operands of step 3, each in two parts of the 16-bit type: with one
+// alone they would be rounded to 8 (bf16) or 11 bits before V, an error of the size of
+// the outputs' own rounding; with two it is 2^-17 or less.  A call of 128 slices of
+// 65536 keys and 64 nodes takes 688 us with two parts and 635 with one; with one node
+// tile the times are within 1%.
+template <int DT>
+__device__ __forceinline__ u32x2 split_shares(float x, float y) {
+  if constexpr (DT == DT_BF16) {
+    const uint32_t hi = pack_bf16(x, y);
+    return {hi, pack_bf16(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u))};
+  } else {
+    const uint32_t hi = pack_f16(x, y);
+    const f16x2 h = __builtin_bit_cast(f16x2, hi);
+    return {hi, pack_f16(x - static_cast<float>(h[0]), y - static_cast<float>(h[1]))};
+  }
 }
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t x, int lane) {
@@ -493,10 +510,10 @@ __global__ __launch_bounds__(kTreeThreads, (kStatWaves<D, DT, NT>)) void tree_st
 // ---------------------------------------------------------------------------
 // shares
 
-// How step 2 takes the bids: 16-bit caches two bf16 parts, 16 bits (2^-17, where the
-// shares' rounding makes 2^-9 or 2^-12 next), fp32 caches three, all 24.  bf16 for
-// its range: where no demand has gone yet a share is p / (p + 1e-9), so bids of
-// 1e-9 count, which one fp16 part loses at any scale that holds 1.
+// How step 2 takes the bids: 16-bit caches two bf16 parts, 16 bits (2^-17, as the shares'
+// two parts in step 3, where the outputs' own rounding makes 2^-9 or 2^-12 at the end),
+// fp32 caches three, all 24.  bf16 for its range: where no demand has gone yet a share is
+// p / (p + 1e-9), so bids of 1e-9 count, which one fp16 part loses at any scale that holds 1.
 template <int DT> constexpr int kBidParts = DT == DT_F32 ? 3 : 2;
 
 // B operands of step 2 for the node of this lane's column: 0/1 by the bits
@@ -737,14 +754,18 @@ __global__ __launch_bounds__(kTreeThreads, (kApplyWaves<D, DT, NT>)) void tree_a
       } else {
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          u32x4 b;
+          u32x4 hi, lo;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = sh[8 * st + 2 * e], y = sh[8 * st + 2 * e + 1];
-            b[e] = DT == DT_BF16 ? pack_bf16(x, y) : pack_f16(x * kShareScale<DT>, y * kShareScale<DT>);
+            const u32x2 b = split_shares<DT>(sh[8 * st + 2 * e] * kShareScale<DT>, sh[8 * st + 2 * e + 1] * kShareScale<DT>);
+            hi[e] = b[0];
+            lo[e] = b[1];
           }
 #pragma unroll
-          for (int e = 0; e < V::E; ++e) acc[u][e] = mma_piece<DT>(now.frag(e, st), b, acc[u][e]);
+          for (int e = 0; e < V::E; ++e) {
+            const u32x4 f = now.frag(e, st);
+            acc[u][e] = mma_piece<DT>(f, hi, mma_piece<DT>(f, lo, acc[u][e]));
+          }
         }
       }
     }
