@@ -393,9 +393,18 @@ class DilutionLM(nn.Module):
         return length
 
     def evict(self, caches, eviction: "Eviction", capacity: int | None = None) -> list:
-        """Every layer's cache shrunk by its own demand (``cache.evict_cache``)."""
+        """Every layer's cache shrunk by its own demand (``cache.evict_cache``); the
+        list given and its caches stay as they are."""
         self._need_production("evict")
-        return [dcache.evict_cache(c, eviction.keep, eviction.first, eviction.recent, capacity) for c in caches]
+        return self._shrink(list(caches), eviction, capacity)
+
+    @staticmethod
+    def _shrink(caches: list, eviction: "Eviction", capacity: int | None) -> list:
+        """``evict`` in the list itself: a layer's old buffers are released (where the list alone
+        holds them) before the next layer's new ones are made."""
+        for i in range(len(caches)):
+            caches[i] = dcache.evict_cache(caches[i], eviction.keep, eviction.first, eviction.recent, capacity)
+        return caches
 
     def _need_production(self, what: str) -> None:
         if not self.graph_decode_eligible():
@@ -461,8 +470,9 @@ class DilutionLM(nn.Module):
         new tokens below that id.  ``graph=True`` runs greedy decoding of an
         all-dilution production stack through ``GraphDecoder`` (the same
         tokens, one HIP graph replay per step).  ``eviction`` bounds the caches:
-        when they hold ``eviction.limit`` positions they shrink to its ``keep``
-        (not with ``graph``, whose captured step holds the caches' addresses)."""
+        when they hold ``eviction.limit`` positions they shrink to its ``keep``, in
+        buffers of at most ``limit`` positions, whatever the prompt's length (not
+        with ``graph``, whose captured step holds the caches' addresses)."""
         if vocab_limit is not None and not 0 < vocab_limit <= self.cfg.vocab_size:
             raise ValueError(f"vocab_limit must be in (0, {self.cfg.vocab_size}]")
         capacity = idx.shape[1] + max_new_tokens
@@ -470,7 +480,7 @@ class DilutionLM(nn.Module):
             if graph:
                 raise ValueError("a graph-replayed generation keeps its caches: eviction needs graph=False")
             self._need_production("eviction")
-            capacity = min(capacity, max(idx.shape[1], eviction.limit) + 1)
+            capacity = min(capacity, max(idx.shape[1], eviction.limit))
         logits, caches = self.prefill(idx, capacity=capacity)
         tokens = idx
         if graph and max_new_tokens > 0 and not (temperature and temperature > 0.0) and self.graph_decode_eligible():
@@ -501,7 +511,8 @@ class DilutionLM(nn.Module):
             tokens = torch.cat([tokens, nxt], dim=1)
             if step + 1 < max_new_tokens:
                 if eviction is not None and caches[0]["len"] >= eviction.limit:
-                    caches = self.evict(caches, eviction, capacity)
+                    left = max_new_tokens - 1 - step            # decode steps, this one included
+                    self._shrink(caches, eviction, min(eviction.keep + left, eviction.limit))
                 logits = self.decode_step(nxt, caches)
         return tokens
 
@@ -528,8 +539,8 @@ class DilutionLM(nn.Module):
             return idx
         room = kernels.MAX_TREE_NODES
         capacity = prompt + max_new_tokens + room
-        if eviction is not None:
-            capacity = min(capacity, max(prompt, eviction.limit) + room)
+        if eviction is not None:             # a prompt past the limit shrinks before the first tree
+            capacity = prompt if prompt >= eviction.limit else min(capacity, eviction.limit + room)
         logits, caches = self.prefill(idx, capacity=capacity)
 
         def pick(x):
@@ -538,10 +549,10 @@ class DilutionLM(nn.Module):
 
         tokens = torch.cat([idx, pick(logits[:, -1:])], dim=1)
         while tokens.shape[1] < prompt + max_new_tokens:
-            if eviction is not None and caches[0]["len"] >= eviction.limit:
-                caches = self.evict(caches, eviction, capacity)
-            drafted, parents = draft(tokens)
             left = prompt + max_new_tokens - tokens.shape[1]
+            if eviction is not None and caches[0]["len"] >= eviction.limit:
+                self._shrink(caches, eviction, min(eviction.keep + left, eviction.limit) + room)
+            drafted, parents = draft(tokens)
             tree = torch.cat([tokens[:, -1:], drafted.to(tokens)], dim=1)
             # node 0 is the last token, the drafted ones follow
             below = [-1] + [int(p) + 1 for p in parents]
