@@ -136,7 +136,8 @@ def accept_tree(cache: dict, draft: dict, path) -> int:
 
 def evict_cache(cache: dict, keep: int, first: int = 0, recent: int = 0, capacity: int | None = None) -> dict:
     """A cache of the ``keep`` positions that carry the demand (the first
-    ``first`` and the last ``recent`` stay whatever they carry), in new buffers of
+    ``first`` and the last ``recent`` stay whatever they carry: the newest keys
+    have had the fewest rows to gather demand from), in new buffers of
     ``max(capacity, keep)`` positions.  The keys hold no position, so decoding
     goes on over the kept ones.  A cache of at most ``keep`` positions is returned as it is."""
     if cache["len"] <= keep:

@@ -579,14 +579,18 @@ class DilutionLM(nn.Module):
 class Eviction:
     """When and how a generation's caches shrink: at ``limit`` positions to the
     ``keep`` that carry the demand, among them the ``first`` first and the
-    ``recent`` last."""
+    ``recent`` last.  By default half of what ``first`` leaves (rounded up) is
+    recent: a key's demand grows with the rows that have seen it, so the newest
+    keys hold the least and would go first."""
 
     limit: int
     keep: int
     first: int = 4
-    recent: int = 0
+    recent: int | None = None
 
     def __post_init__(self):
+        if self.recent is None:
+            self.recent = (self.keep - self.first + 1) // 2
         if self.first < 0 or self.recent < 0 or not 1 <= self.first + self.recent <= self.keep < self.limit:
             raise ValueError("an eviction needs 1 <= first + recent <= keep < limit")
 

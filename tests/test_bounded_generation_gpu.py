@@ -107,3 +107,18 @@ def test_evict_leaves_the_callers_caches():
     assert all(a is b for a, b in zip(caches, given)) and len(caches) == 3
     assert all(c["len"] == 100 and torch.equal(c["k"], s) for c, s in zip(caches, snap))
     assert all(c["len"] == 50 and c["k"].shape[2] == 70 for c in small)
+
+
+def test_an_eviction_by_default_keeps_the_newest_rows():
+    """The demand of a key grows with the rows that have seen it, so the newest hold the least of
+    it: a window of them stays all the same."""
+    from dilution.lm import Eviction
+
+    model = _model()
+    idx = torch.randint(0, 300, (2, 512), generator=torch.Generator().manual_seed(12)).cuda()
+    _, caches = model.prefill(idx)
+    small = model.evict(caches, Eviction(limit=512, keep=256))
+    for old, new in zip(caches, small):
+        for name in ("k", "v"):
+            assert torch.equal(new[name][:, :, :4], old[name][:, :, :4])
+            assert torch.equal(new[name][:, :, 256 - 126 :], old[name][:, :, 512 - 126 :])
