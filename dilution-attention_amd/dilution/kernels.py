@@ -423,36 +423,45 @@ MAX_TREE_NODES = 64
 """The most drafted nodes of one tree step."""
 
 
-def _node_numbers(x, device, low: int, high: int, name: str) -> torch.Tensor:
-    """Node numbers as int32 on ``device``.  Host values (sequences, CPU tensors)
-    come checked and are copied over; device tensors are taken as they are, int64
-    ones brought into [low, high] first, so that no value wraps into another."""
+def _node_numbers(x, name: str) -> torch.Tensor:
+    """Node numbers as a tensor of whole numbers, (N,) or (B, N), wherever they are."""
     if not torch.is_tensor(x):
-        x = torch.tensor(x, dtype=torch.int64)
+        x = torch.as_tensor(x)
+        # an empty sequence has no type of its own; numpy's narrow whole numbers hold the same values
+        if x.numel() == 0 or x.dtype in (torch.int8, torch.uint8, torch.int16):
+            x = x.to(torch.int64)
     if x.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be int32 or int64, got {x.dtype}")
+    if x.dim() not in (1, 2):
+        raise ValueError(f"{name} must be (N,) or (B, N) node numbers, got shape {tuple(x.shape)}")
+    return x
+
+
+def _to_device(x: torch.Tensor, device, low: int, high: int) -> torch.Tensor:
+    """Node numbers as contiguous int32 on ``device``; int64 ones are brought into
+    [low, high] first, so that no value wraps into another."""
     if x.dtype == torch.int64:
         x = x.clamp(low, high).to(torch.int32)
     return x.to(device).contiguous()
 
 
-def _check_parents(parents) -> None:
-    """ValueError unless every host value is -1, -2 (absent) or an earlier node."""
-    if torch.is_tensor(parents) and parents.is_cuda:
-        return
-    p = torch.as_tensor(parents)
-    if p.dtype in (torch.int32, torch.int64) and p.dim() in (1, 2):
-        if bool(((p < -2) | (p >= torch.arange(p.shape[-1]))).any()):
-            raise ValueError("each parent must be an earlier node, -1 (a child of the context) or -2 (absent)")
+def _parents_on(device, parents) -> torch.Tensor:
+    """A tree's parents for the kernels.  Host values (sequences, CPU tensors) are
+    checked: each is -1, -2 (absent) or an earlier node; device tensors are taken as they are."""
+    p = _node_numbers(parents, "parents")
+    if not p.is_cuda and bool(((p < -2) | (p >= torch.arange(p.shape[-1]))).any()):
+        raise ValueError("each parent must be an earlier node, -1 (a child of the context) or -2 (absent)")
+    return _to_device(p, device, -2, MAX_TREE_NODES)
 
 
-def _check_path(path, nodes: int) -> None:
-    if torch.is_tensor(path) and path.is_cuda:
-        return
-    p = torch.as_tensor(path)
-    if p.dtype in (torch.int32, torch.int64) and p.numel():
+def _path_on(device, path, nodes: int | None) -> torch.Tensor:
+    """An accepted path for the kernels, host values checked against the tree's nodes
+    (``None``: unknown here, for the native checks to refuse)."""
+    p = _node_numbers(path, "path")
+    if not p.is_cuda and nodes is not None and p.numel():
         if bool(((p < 0) | (p >= nodes)).any()) or bool((p.diff(dim=-1) <= 0).any()):
             raise ValueError(f"a path runs down the tree: ascending node numbers in [0, {nodes})")
+    return _to_device(p, device, -1, MAX_TREE_NODES)
 
 
 def dilution_tree_step(
@@ -489,8 +498,7 @@ def dilution_tree_step(
     With return_aux also returns dict(lse): the (B, H, N) fp32 row statistics,
     p_ij = 2^(log2(e) q_i.k_j / sqrt(D) - lse_i), +inf for absent nodes.
     """
-    _check_parents(parents)
-    parents = _node_numbers(parents, q.device, -2, MAX_TREE_NODES, "parents")
+    parents = _parents_on(q.device, parents)
     out, lse = _native().tree_step(q, k_cache, v_cache, committed, length, parents, _raw_stream(q))
     return (out, dict(lse=lse)) if return_aux else out
 
@@ -517,9 +525,7 @@ def dilution_tree_accept(
     as they are (zero demand stays zero).  A device path is not checked: an entry
     outside [0, N) counts for nothing and leaves its row.
     """
-    if q.dim() == 4:
-        _check_path(path, q.shape[2])
-    path = _node_numbers(path, q.device, -1, MAX_TREE_NODES, "path")
+    path = _path_on(q.device, path, q.shape[2] if q.dim() == 4 else None)
     _native().tree_accept(q, k_cache, v_cache, committed, length, lse, path, _raw_stream(q))
     return length + path.shape[-1]
 

@@ -383,11 +383,7 @@ class DilutionLM(nn.Module):
     def accept_tree(self, caches, drafts, path) -> int:
         """Take a path of the last ``tree_step``'s tree into every layer's cache
         (``cache.accept_tree``); returns the new length."""
-        if not torch.is_tensor(path):
-            path = torch.tensor(path, dtype=torch.int64)
-        if not path.is_cuda:
-            kernels._check_path(path, drafts[0]["q"].shape[2])
-            path = path.to(caches[0]["k"].device)       # once, not in every layer
+        path = kernels._path_on(caches[0]["k"].device, path, drafts[0]["q"].shape[2])       # once, not in every layer
         for cache, draft in zip(caches, drafts):
             length = dcache.accept_tree(cache, draft, path)
         return length

@@ -3,8 +3,11 @@ refuse around the kernels."""
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
+import torch
 
+from dilution import kernels
 from dilution.lm import Eviction
 
 
@@ -22,3 +25,36 @@ def test_an_eviction_has_room_for_the_first_ones():
                 dict(limit=10, keep=8, recent=5), dict(limit=10, keep=0, first=0)):
         with pytest.raises(ValueError, match="eviction"):
             Eviction(**bad)
+
+
+def _state(b=2, h=3, cap=40, n=4, d=64):
+    q = torch.zeros(b, h, n, d, dtype=torch.bfloat16)
+    k = torch.zeros(b, h, cap, d, dtype=torch.bfloat16)
+    return q, k, k.clone(), torch.zeros(b, h, cap)
+
+
+def test_host_node_numbers_are_whole_and_checked():
+    """Numbers that are not whole are refused, not cut; so are the shapes that no tree has."""
+    q, k, v, com = _state()
+    lse = torch.zeros(2, 3, 4)
+    for bad in ([-1, 0.0, 1.0, 5.7], [-1.0, 0.5, 1.0, 2.0], np.array([-1.0, 0, 1, 2]), [True, False, False, False]):
+        with pytest.raises(ValueError, match="parents must be int32 or int64"):
+            kernels.dilution_tree_step(q, k, v, com, 36, bad)
+    for bad in ([0.0, 1.5], np.array([0.5]), [False, True]):
+        with pytest.raises(ValueError, match="path must be int32 or int64"):
+            kernels.dilution_tree_accept(q, k, v, com, 36, lse, bad)
+    for bad in (0, torch.tensor(0), np.int64(0), [[[0, 1]]], torch.zeros(1, 1, 2, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="path"):
+            kernels.dilution_tree_accept(q, k, v, com, 36, lse, bad)
+    for bad in (0, torch.tensor(-1), [[[-1, 0, 1, 2]]]):
+        with pytest.raises(ValueError, match="parents"):
+            kernels.dilution_tree_step(q, k, v, com, 36, bad)
+    # what is whole passes these checks (and stops at the tensors, which are on the CPU)
+    for good in ([-1, 0, 1, 2], (-1, 0, 1, -2), np.array([-1, 0, 1, 2]), np.array([-1, 0, 1, 2], dtype=np.int32),
+                 np.array([-1, 0, 1, 2], dtype=np.int16),
+                 torch.tensor([[-1, 0, 1, 2]] * 2)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            kernels.dilution_tree_step(q, k, v, com, 36, good)
+    for good in ([], [[], []], [0, 3], np.array([1, 2])):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            kernels.dilution_tree_accept(q, k, v, com, 36, lse, good)
