@@ -374,6 +374,7 @@ class DilutionLM(nn.Module):
         takes.  The caches' lengths and demands stay.  Every layer has to run the
         production dilution operator."""
         self._need_production("tree_step")
+        parents = kernels._parents_on(tokens.device, parents)          # checked and copied once, not in every layer
         x, drafts = self.wte(tokens), []
         for block, cache in zip(self.h, caches):
             x, draft = block.tree_step(x, cache, parents)

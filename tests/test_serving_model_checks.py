@@ -7,8 +7,8 @@ import numpy as np
 import pytest
 import torch
 
-from dilution import kernels
-from dilution.lm import Eviction
+from dilution import cache, kernels
+from dilution.lm import DilutionLM, Eviction, LMConfig
 
 
 @pytest.mark.parametrize("limit,keep,first,recent", [(200, 100, 4, 48), (6, 5, 4, 1), (90, 50, 4, 23), (9, 4, 4, 0)])
@@ -58,3 +58,25 @@ def test_host_node_numbers_are_whole_and_checked():
     for good in ([], [[], []], [0, 3], np.array([1, 2])):
         with pytest.raises(RuntimeError, match="no CPU path"):
             kernels.dilution_tree_accept(q, k, v, com, 36, lse, good)
+
+
+def _model(**kw):
+    return DilutionLM(LMConfig(vocab_size=32, n_layers=3, d_model=64, n_heads=4, **kw))
+
+
+def test_a_model_step_converts_its_tree_once(monkeypatch):
+    """Every layer gets the same int32 tensor; a tree that is refused reaches none."""
+    model, seen = _model(), []
+
+    def tree_step(q, k, v, cache, parents):
+        seen.append(parents)
+        return q, {}
+
+    monkeypatch.setattr(cache, "tree_step", tree_step)
+    tokens = torch.zeros(1, 4, dtype=torch.long)
+    model.tree_step(tokens, [-1, 0, 1, -2], [{}] * 3)
+    assert len(seen) == 3 and all(p is seen[0] for p in seen)
+    assert seen[0].dtype == torch.int32 and seen[0].tolist() == [-1, 0, 1, -2]
+    with pytest.raises(ValueError, match="parent"):
+        model.tree_step(tokens, [-1, 0, 2, 1], [{}] * 3)
+    assert len(seen) == 3
