@@ -30,6 +30,8 @@ token at a time and its caches only grow.
 
 from __future__ import annotations
 
+import itertools
+
 import torch
 
 from . import kernels
@@ -54,6 +56,16 @@ def alloc_cache(k: torch.Tensor, v: torch.Tensor, capacity: int | None = None) -
     return {"k": k_buf, "v": v_buf, "len": seq, "committed": committed}
 
 
+_draft_numbers = itertools.count(1)
+"""A number for every tree step: a cache holds that of the last one on it, until it moves on."""
+
+
+def moved_on(cache: dict, length: int) -> None:
+    """Set the length after rows were written: what was drafted behind the old one is gone."""
+    cache["len"] = length
+    cache.pop("draft", None)
+
+
 def append_kv(cache: dict, k1: torch.Tensor, v1: torch.Tensor) -> int:
     """Write one new position (k1, v1: (B, H, 1, D)) and return the new
     length (model.py:86-93)."""
@@ -62,7 +74,7 @@ def append_kv(cache: dict, k1: torch.Tensor, v1: torch.Tensor) -> int:
         raise ValueError("decode step past the cache capacity (context_length)")
     cache["k"][:, :, t] = k1[:, :, 0]
     cache["v"][:, :, t] = v1[:, :, 0]
-    cache["len"] = t + 1
+    moved_on(cache, t + 1)
     return t + 1
 
 
@@ -114,24 +126,34 @@ def tree_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, pa
     below the cached context (``parents`` as in ``kernels.dilution_tree_step``).
     Writes their k and v behind the cached positions and returns (y, draft): y
     (B, H, N, D) in q.dtype, draft what ``accept_tree`` needs.  The cache's
-    length and demand stay; a later step overwrites rows that were not accepted."""
+    length and demand stay.  A later step overwrites rows that were not accepted:
+    of several tree steps the last one's draft can be, until the cache moves on."""
     t, stop = cache["len"], cache["len"] + q.shape[2]
     if stop > cache["k"].shape[2]:
         raise ValueError("drafted tokens past the cache capacity (context_length)")
+    cache["draft"] = number = next(_draft_numbers)
     cache["k"][:, :, t:stop] = k
     cache["v"][:, :, t:stop] = v
     y, aux = kernels.dilution_tree_step(q, cache["k"], cache["v"], cache["committed"], t, parents, return_aux=True)
-    return y, {"q": q, "lse": aux["lse"], "len": t}
+    return y, {"q": q, "lse": aux["lse"], "len": t, "number": number}
+
+
+def check_draft(cache: dict, draft: dict) -> None:
+    """ValueError unless ``draft`` is what the last ``tree_step`` on this cache returned, and the
+    cache is where it was."""
+    if draft["len"] != cache["len"] or "draft" not in cache or draft.get("number") != cache["draft"]:
+        raise ValueError("the cache has moved on since this tree step")
 
 
 def accept_tree(cache: dict, draft: dict, path) -> int:
     """Take a path of the tree of the last ``tree_step`` on this cache into it
     (``path`` as in ``kernels.dilution_tree_accept``); returns the new length."""
-    if draft["len"] != cache["len"]:
-        raise ValueError("the cache has moved on since this tree step")
-    cache["len"] = kernels.dilution_tree_accept(draft["q"], cache["k"], cache["v"], cache["committed"], cache["len"],
-                                                draft["lse"], path)
-    return cache["len"]
+    check_draft(cache, draft)
+    length = kernels.dilution_tree_accept(draft["q"], cache["k"], cache["v"], cache["committed"], cache["len"],
+                                          draft["lse"], path)
+    if length != cache["len"]:
+        moved_on(cache, length)
+    return length
 
 
 def evict_cache(cache: dict, keep: int, first: int = 0, recent: int = 0, capacity: int | None = None) -> dict:

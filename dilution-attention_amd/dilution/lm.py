@@ -352,7 +352,7 @@ class DilutionLM(nn.Module):
                 t = cache["len"]
                 if t >= cache["k"].shape[2]:
                     raise ValueError("decode step past the cache capacity (context_length)")
-                cache["len"] = t + 1
+                dcache.moved_on(cache, t + 1)
                 return cache["k"], cache["v"], t
 
             def attend(i, q1):
@@ -700,7 +700,7 @@ class GraphDecoder:
             self.graph.replay()
         self.len += 1
         for c in self.caches:
-            c["len"] = self.len
+            dcache.moved_on(c, self.len)
         return self.tok
 
 

@@ -80,3 +80,47 @@ def test_a_model_step_converts_its_tree_once(monkeypatch):
     with pytest.raises(ValueError, match="parent"):
         model.tree_step(tokens, [-1, 0, 2, 1], [{}] * 3)
     assert len(seen) == 3
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """The kernels' calls replaced: only what the cache dict and the model do around them runs."""
+    monkeypatch.setattr(kernels, "dilution_tree_step", lambda q, k, v, com, t, parents, return_aux: (q, {"lse": None}))
+    monkeypatch.setattr(kernels, "dilution_tree_accept", lambda q, k, v, com, t, lse, path: t + len(path))
+
+
+def _cache(length=30):
+    _, k, v, com = _state()
+    return {"k": k, "v": v, "len": length, "committed": com}
+
+
+def _draft(c, n=4, **kw):
+    q = torch.ones(2, 3, n, 64, dtype=torch.bfloat16)
+    return cache.tree_step(q, kw.get("k", q), kw.get("v", q), c, list(range(-1, n - 1)))[1]
+
+
+def test_only_the_last_draft_is_accepted(on_cpu):
+    """A second tree step has overwritten the first one's rows, at the same length."""
+    c = _cache()
+    first, second = _draft(c), _draft(c)
+    with pytest.raises(ValueError, match="moved on"):
+        cache.accept_tree(c, first, [0])
+    assert c["len"] == 30
+    with pytest.raises(ValueError, match="moved on"):      # of another cache, as long
+        cache.accept_tree(_cache(), second, [0])
+    assert cache.accept_tree(c, second, []) == 30          # nothing taken, nothing moved
+    assert cache.accept_tree(c, second, [0, 1]) == 32
+    for length in (32, 30):
+        c["len"] = length
+        with pytest.raises(ValueError, match="moved on"):
+            cache.accept_tree(c, second, [0])
+
+
+def test_a_decode_step_takes_the_draft_away(on_cpu):
+    c = _cache()
+    draft = _draft(c)
+    one = torch.zeros(2, 3, 1, 64, dtype=torch.bfloat16)
+    cache.append_kv(c, one, one)
+    c["len"] = 30                                          # as a program that takes the token back
+    with pytest.raises(ValueError, match="moved on"):
+        cache.accept_tree(c, draft, [0])
