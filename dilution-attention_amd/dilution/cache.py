@@ -128,9 +128,23 @@ def tree_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, pa
     (B, H, N, D) in q.dtype, draft what ``accept_tree`` needs.  The cache's
     length and demand stay.  A later step overwrites rows that were not accepted:
     of several tree steps the last one's draft can be, until the cache moves on."""
-    t, stop = cache["len"], cache["len"] + q.shape[2]
-    if stop > cache["k"].shape[2]:
+    # all that the kernels would refuse, before any row is written
+    if q.dim() != 4 or k.shape != q.shape or v.shape != q.shape:
+        raise ValueError(f"q, k and v must have one shape (B, H, N, D), got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    batch, heads, capacity, head_dim = cache["k"].shape
+    nodes = q.shape[2]
+    if (*q.shape[:2], q.shape[3]) != (batch, heads, head_dim):
+        raise ValueError(f"drafted rows {tuple(q.shape)} do not match the cache {tuple(cache['k'].shape)}")
+    if not 1 <= nodes <= kernels.MAX_TREE_NODES:
+        raise ValueError(f"a tree holds 1 to {kernels.MAX_TREE_NODES} drafted nodes, got {nodes}")
+    if q.dtype != cache["k"].dtype or q.device != cache["k"].device:
+        raise ValueError("q must have the caches' dtype and device")
+    t, stop = cache["len"], cache["len"] + nodes
+    if stop > capacity:
         raise ValueError("drafted tokens past the cache capacity (context_length)")
+    parents = kernels._parents_on(q.device, parents)
+    if parents.shape not in ((nodes,), (batch, nodes)):
+        raise ValueError(f"parents {tuple(parents.shape)} do not match the drafted rows {tuple(q.shape)}")
     cache["draft"] = number = next(_draft_numbers)
     cache["k"][:, :, t:stop] = k
     cache["v"][:, :, t:stop] = v

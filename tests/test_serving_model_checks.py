@@ -124,3 +124,26 @@ def test_a_decode_step_takes_the_draft_away(on_cpu):
     c["len"] = 30                                          # as a program that takes the token back
     with pytest.raises(ValueError, match="moved on"):
         cache.accept_tree(c, draft, [0])
+
+
+def test_a_refused_tree_step_leaves_the_draft_before_it(on_cpu):
+    c = _cache()
+    draft = _draft(c)
+    rows = [c[x].clone() for x in ("k", "v")]
+    q = torch.full((2, 3, 4, 64), 7.0, dtype=torch.bfloat16)
+    for args, kind in (((q, q, q, c, [-1, 0, 2, 1]), "parent"), ((q, q, q, c, [-1, 0, 1]), "parents"),
+                       ((q, q, q, c, torch.zeros(3, 4, dtype=torch.int32)), "parent"),
+                       ((q, q, q, c, torch.zeros(3, 4, dtype=torch.int32) - 1), "parents"),
+                       ((q, q[:, :, :1], q, c, [-1] * 4), "one shape"), ((q, q, q[:1], c, [-1] * 4), "one shape"),
+                       ((q[:1], q[:1], q[:1], c, [-1] * 4), "cache"), ((q[..., :32],) * 3 + (c, [-1] * 4), "cache"),
+                       ((q.float(), q, q, c, [-1] * 4), "dtype"), ((q[:, :, :0],) * 3 + (c, []), "1 to 64"),
+                       ((q.repeat(1, 1, 3, 1),) * 3 + (c, [-1] * 12), "capacity"),
+                       ((q[0], q[0], q[0], c, [-1] * 3), "B, H, N, D")):
+        with pytest.raises(ValueError, match=kind):
+            cache.tree_step(*args)
+    for x, old in zip(("k", "v"), rows):
+        assert torch.equal(c[x], old)
+    big = {"k": torch.zeros(2, 3, 99, 64, dtype=torch.bfloat16), "len": 0}
+    with pytest.raises(ValueError, match="1 to 64"):
+        cache.tree_step(*(q.repeat(1, 1, 17, 1),) * 3, big, [-1] * 68)
+    assert cache.accept_tree(c, draft, [0, 1]) == 32
