@@ -384,6 +384,10 @@ class DilutionLM(nn.Module):
     def accept_tree(self, caches, drafts, path) -> int:
         """Take a path of the last ``tree_step``'s tree into every layer's cache
         (``cache.accept_tree``); returns the new length."""
+        if len(drafts) != len(caches):
+            raise ValueError(f"{len(drafts)} drafts for {len(caches)} layers' caches")
+        for cache, draft in zip(caches, drafts):        # in every layer or in none
+            dcache.check_draft(cache, draft)
         path = kernels._path_on(caches[0]["k"].device, path, drafts[0]["q"].shape[2])       # once, not in every layer
         for cache, draft in zip(caches, drafts):
             length = dcache.accept_tree(cache, draft, path)

@@ -147,3 +147,16 @@ def test_a_refused_tree_step_leaves_the_draft_before_it(on_cpu):
     with pytest.raises(ValueError, match="1 to 64"):
         cache.tree_step(*(q.repeat(1, 1, 17, 1),) * 3, big, [-1] * 68)
     assert cache.accept_tree(c, draft, [0, 1]) == 32
+
+
+def test_a_model_accepts_in_every_layer_or_none(on_cpu):
+    model = _model()
+    caches = [_cache() for _ in range(3)]
+    drafts = [_draft(c) for c in caches]
+    with pytest.raises(ValueError, match="drafts"):
+        model.accept_tree(caches, drafts[:2], [0])
+    last = _draft(caches[2])
+    with pytest.raises(ValueError, match="moved on"):
+        model.accept_tree(caches, drafts, [0])
+    assert [c["len"] for c in caches] == [30] * 3
+    assert model.accept_tree(caches, drafts[:2] + [last], [0, 1]) == 32
