@@ -401,8 +401,13 @@ int evict(const EvictArgs& a) {
            Move{static_cast<const u32x4*>(a.k_cache), static_cast<const u32x4*>(a.v_cache), static_cast<u32x4*>(a.k_out),
                 static_cast<u32x4*>(a.v_out), a.committed_out, a.out_cap, shift, here}};
   if (one) {
-    const unsigned n = static_cast<unsigned>(a.n);
-    auto select = [&](auto e) { DIL_TIMED("evict_select", st, (evict_select<e()><<<dim3(n), kSelThreads, 0, st>>>(S))); };
+    // batches of slices: one grid holds fewer than 2^32 threads, those of 4194304 slices
+    auto select = [&](auto e) {
+      slice_batches(a.n, [&](int64_t s0, unsigned ns) {
+        S.slice0 = s0;
+        DIL_TIMED("evict_select", st, (evict_select<e()><<<dim3(ns), kSelThreads, 0, st>>>(S)));
+      });
+    };
     if (keys <= 4 * kSelThreads || a.keep == a.first + a.recent) select(std::integral_constant<int, 4>{});
     else if (keys <= 8 * kSelThreads) select(std::integral_constant<int, 8>{});
     else if (keys <= 16 * kSelThreads) select(std::integral_constant<int, 16>{});
