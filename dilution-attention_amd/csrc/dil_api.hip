@@ -331,6 +331,7 @@ int dil_decode_step_dlen(const void* q1, const void* k_cache, const void* v_cach
 
 int64_t dil_forward_workspace_bytes(int64_t n, int64_t seq, int head_dim, int dtype,
                                     int precision, int want_pk) {
+  if (n < 1 || seq < 1) return 0;
   return dil::forward_workspace_bytes(n, seq, seq, head_dim, dtype, precision, want_pk,
                                       dil::forward_key_pass_requested());
 }
@@ -404,6 +405,7 @@ int dil_forward_key_pass(int64_t chunk, int64_t start, int head_dim, int dtype, 
 
 int64_t dil_prefill_workspace_bytes(int64_t n, int64_t chunk, int64_t start, int head_dim,
                                     int dtype, int precision) {
+  if (n < 1 || chunk < 1 || start < 0) return 0;
   return dil::forward_workspace_bytes(n, chunk, start + chunk, head_dim, dtype, precision, 0,
                                       dil::forward_key_pass_requested());
 }

@@ -41,6 +41,7 @@
  *     slice count: a smaller call may be quicker with up to 1 GiB of partials
  *     that a larger one has no use for.  A workspace sized for more slices of
  *     the same rows (up to the 24 GiB) also runs fewer, with the same results.
+ *     Without slices or rows the queries return 0, and the calls refuse the sizes.
  *   - Return value: 0 on success, a positive hipError_t from the launch, or a
  *     negative argument error (see dil_status_string).  A NULL pointer where
  *     an argument is required is an argument error (-4); only `pk` of
