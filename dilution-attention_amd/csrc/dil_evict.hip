@@ -355,7 +355,12 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move(Move m, const float* 
 
 namespace {
 
-constexpr int64_t kOneMax = 32 * kSelThreads;            // keys that one workgroup holds
+// The most keys that one workgroup selects from, as many as its registers hold.  us a call
+// (head_dim 64, half of the keys stay), one workgroup a slice -> chunks:
+//   8192 keys: 1, 16, 64, 256 slices 16 -> 31, 19 -> 36, 34 -> 51, 120 -> 139
+//   16384 21 -> 36, 31 -> 45, 66 -> 81, 237 -> 253;  24576 35 -> 37, 47 -> 51, 113 -> 118, 352 -> 379
+//   32768 36.2 -> 37.5, 56.2 -> 55.7, 142 -> 143, 462 -> 488
+constexpr int64_t kOneMax = 32 * kSelThreads;
 constexpr int64_t kMaxChunks = 64;
 
 // The chunked form's chunks: of 16384 keys, longer ones where that makes more than 64.

@@ -966,7 +966,10 @@ __global__ __launch_bounds__(kTreeThreads) void tree_demand(Tree A) {
 
 // The workgroups of a slice over its cached keys: those of all slices (one more each,
 // for the drafted keys) fill whole rounds of the `slots` that the GPU holds at once,
-// as few rounds as fill 15/16 of their places (of 4 rounds the best).  At least
+// as few rounds as fill 15/16 of their places (of 4 rounds the best).  The drafted keys'
+// workgroup counts as much as the others though it ends sooner: where few workgroups a
+// slice fill a round, its place is idle most of the time (384 slices of 768 places: one
+// workgroup over the cached keys each, 16384 keys 499 us where 320 slices take 343).  At least
 // `least` keys each: 256 (16 slices of 1000 keys, 128, 256, 512, 1024 of them: shares
 // 7.2, 7.4, 10.2, 18.3 us; 15 of 5003 at head_dim 128 16, 15, 18, 27), of fp32 caches
 // 128, whose tiles take four times the matrix cycles (16 of 4096 keys 16, 19, 24, 41).
@@ -1015,8 +1018,8 @@ struct TreePlan {
     // multiple: several short rounds hide one another's start and end.  us with 3, 4, 6,
     // 8, 12, 16 places a CU, 128 slices of 65536 keys and 64 nodes (3 at once):
     // statistics 201, 245, 185, 198, 188, 205; 128 of 16384, 32 nodes (6 at once): 55, 57,
-    // 53, 59, 51, 56.  Shares of the first with 2, 3, 4, 8 places (2 at once): 464, 462,
-    // 426, 439.
+    // 53, 59, 51, 56.  Shares of the first with 2, 3, 4, 8 places (2 at once): 524, 486,
+    // 472, 463; of the second with 2, 3, 4, 8 (3 at once): 89, 92, 102, 97.
     nstat = tree_split(n, length, kCUs * (nodes > kTileNodes ? 6 : 12), least_keys(dtype));
     nchunk = tree_split(n, length, kCUs * (nodes > kTileNodes && apply_waves == 2 ? 4 : apply_waves), least_keys(dtype));
     const size_t rows = static_cast<size_t>(n * (nchunk + 1) * nodes);
@@ -1032,18 +1035,24 @@ struct TreePlan {
 // Whether a slice's whole step runs in one workgroup (one node tile): little work, where
 // two launches less count, or slices that fill the places on the GPU by themselves.
 // us a call, three launches -> one, 8 nodes, bf16 64 where nothing else stands:
-//   16 slices of 32, 128, 256, 512 keys 13.3 -> 11.2, 13.3 -> 11.6, 13.4 -> 13.5, 13.6 -> 17.1 (1 node
-//   12.9 -> 8.5, 13.6 -> 8.9, 13.8 -> 10.5, 13.6 -> 13.6); head_dim 16, 512 and 768 keys 13.2 -> 12.6,
-//   13.3 -> 14.5; head_dim 128, 32 keys 13.1 -> 13.3; fp32, 32 keys 14.2 -> 14.5
-//   256 keys: 128, 192, 256, 384, 512, 768, 900 slices 13.2 -> 13.9, 15.5 -> 14.3, 16.0 -> 14.4,
-//   19.3 -> 18.4, 26.5 -> 19.8, 33.1 -> 23.8, 40.2 -> 37.9
-//   1024 keys: 256, 384, 512, 768, 900 slices 27.8 -> 31.3, 42.2 -> 38.4, 47.6 -> 41.9, 74.3 -> 55.3,
-//   81.4 -> 88.5 (fp32 54 -> 55, 109 -> 77, 104 -> 83, 193 -> 128, 202 -> 172)
-//   16384 keys: 384, 512, 640, 768, 900, 1100, 1300 slices 494 -> 509, 577 -> 562, 681 -> 722,
-//   992 -> 786, 980 -> 1135, 1422 -> 1260, 1376 -> 1435 (head_dim 128, 4096 keys: 271 -> 253, 325 -> 276,
-//   405 -> 360, 542 -> 398, 571 -> 592, 775 -> 682, 800 -> 715)
-//   head_dim 256 (256 places), 1024 keys: 256, 320, 512, 768, 900 slices 102 -> 80, 111 -> 159,
-//   201 -> 179, 320 -> 263, 310 -> 335
+//   16 slices of 32, 128, 256, 512 keys 13.8 -> 11.3, 13.7 -> 11.6, 13.9 -> 13.5, 13.9 -> 16.8 (1 node
+//   13.8 -> 8.5, 13.8 -> 9.0, 13.8 -> 10.7, 13.7 -> 13.9; 32 nodes, 32, 128, 256 keys 20.0 -> 19.2,
+//   20.0 -> 19.6, 19.7 -> 21.3); 1, 4 and 64 slices differ by less than 0.6; head_dim 16, 512 and 768
+//   keys 13.7 -> 12.6, 13.8 -> 14.5; head_dim 128, 32 and 128 keys 14.4 -> 13.2, 14.4 -> 14.4; fp32,
+//   32 and 64 keys 15.2 -> 14.7, 16.1 -> 15.0
+//   256 keys: 128, 192, 256, 384, 512, 768, 900 slices 14.6 -> 13.7, 16.0 -> 13.9, 16.2 -> 13.9,
+//   20.2 -> 16.7, 26.4 -> 17.0, 33.5 -> 22.0, 40.1 -> 37.4
+//   1024 keys: 256, 384, 512, 768, 900 slices 27.2 -> 30.8, 42.2 -> 38.8, 47.5 -> 41.3, 74.4 -> 54.7,
+//   80.6 -> 86.1 (fp32 53 -> 54, 110 -> 77, 102 -> 80, 187 -> 110, 195 -> 153)
+//   16384 keys: 384, 512, 640, 768, 900, 1100, 1300 slices 499 -> 503, 576 -> 557, 684 -> 699,
+//   999 -> 766, 981 -> 1105, 1435 -> 1248, 1385 -> 1402 (fp32, 384 slices 1320 -> 1159; head_dim 128,
+//   4096 keys: 270 -> 257, 314 -> 281, 381 -> 361, 552 -> 393, 550 -> 587, 792 -> 666, 766 -> 715)
+//   head_dim 256 (256 places), 1024 keys: 256, 320, 512, 768, 900 slices 114 -> 79, 112 -> 143,
+//   222 -> 159, 358 -> 269, 330 -> 347
+// One threshold for all of them is off at its edges.  It takes the slower form for 900
+// slices of 1024 keys and 640 and 1300 of 16384 (1 to 7%), and misses the quicker one for one
+// node at 256 keys (22%), 384 and 512 slices at head_dim 128 (5 and 11%), 512 of 16384 keys
+// (3%) and fp32 384 of them (12%).
 template <int D, int DT>
 bool tree_in_one(int64_t n, int64_t length, int64_t places) {
   constexpr int64_t kRow = Shape<D, DT>::kRow;

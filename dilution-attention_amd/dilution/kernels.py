@@ -493,7 +493,8 @@ def dilution_tree_step(
     nodes that it does not see.  Nothing in the cache changes:
     ``dilution_tree_accept`` takes a path of the tree into it.  The same call gives
     the same bits; a slice's bits may differ in calls of another B * H, length or N,
-    which pick the order of its sums.
+    which pick the order of its sums.  The outputs are rounded to q's dtype once, at
+    the end.  A HIP graph of the call serves one ``length``, a host number.
 
     With return_aux also returns dict(lse): the (B, H, N) fp32 row statistics,
     p_ij = 2^(log2(e) q_i.k_j / sqrt(D) - lse_i), +inf for absent nodes.

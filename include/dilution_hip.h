@@ -36,7 +36,7 @@
  *     the call: the size of a call picks the order of some sums (the forward's
  *     for rows of at most 2048 keys, and at any length for operands other than
  *     bf16 at head_dim 64 and for prefill chunks that start off the multiples of
- *     512; dk's up to head_dim 128; the decode step's).
+ *     512; dk's up to head_dim 128; the decode step's; the tree step's).
  *   - The forward's and the prefill's workspace queries are not monotone in the
  *     slice count: a smaller call may be quicker with up to 1 GiB of partials
  *     that a larger one has no use for.  A workspace sized for more slices of
@@ -382,7 +382,7 @@ int dil_rows_argmax(const void* logits, int64_t rows, int64_t row_stride, int64_
  * (n, nodes) float32.  An absent node's out is 0 and its lse +inf; its K, V and q
  * rows are read but count for nothing, whatever they hold.  A node's results do not
  * depend on nodes that it does not see.  Nothing in the caches changes.  The caches
- * are 16-byte aligned.
+ * are 16-byte aligned.  length is a host value: a captured call serves it alone.
  */
 int64_t dil_tree_workspace_bytes(int64_t n, int64_t length, int64_t nodes, int head_dim, int dtype);
 int dil_tree_step(const dil_rows* q, const void* k_cache, const void* v_cache, const float* committed,
