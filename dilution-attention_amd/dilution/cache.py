@@ -25,7 +25,8 @@ variant decode step (model.py:198-241 with ``_bid_kw``).
 ``tree_step`` and ``accept_tree`` decode several drafted tokens at once (a tree
 of them, of which one path is taken), and ``evict_cache`` shrinks a cache to the
 keys that carry the demand.  The reference has no counterpart: it decodes one
-token at a time and its caches only grow.
+token at a time and its caches only grow.  Between a tree step and the next
+change of the length the dict also holds ``draft``, the number of that step.
 """
 
 from __future__ import annotations

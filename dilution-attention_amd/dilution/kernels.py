@@ -427,8 +427,8 @@ def _node_numbers(x, name: str) -> torch.Tensor:
     """Node numbers as a tensor of whole numbers, (N,) or (B, N), wherever they are."""
     if not torch.is_tensor(x):
         x = torch.as_tensor(x)
-        # an empty sequence has no type of its own; numpy's narrow whole numbers hold the same values
-        if x.numel() == 0 or x.dtype in (torch.int8, torch.uint8, torch.int16):
+        # an empty sequence has no type of its own; numpy has whole numbers of other widths
+        if x.numel() == 0 or not (x.is_floating_point() or x.is_complex() or x.dtype == torch.bool):
             x = x.to(torch.int64)
     if x.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be int32 or int64, got {x.dtype}")

@@ -55,7 +55,7 @@ def test_host_node_numbers_are_whole_and_checked():
                  torch.tensor([[-1, 0, 1, 2]] * 2)):
         with pytest.raises(RuntimeError, match="no CPU path"):
             kernels.dilution_tree_step(q, k, v, com, 36, good)
-    for good in ([], [[], []], [0, 3], np.array([1, 2])):
+    for good in ([], [[], []], [0, 3], np.array([1, 2]), np.array([0, 3], dtype=np.uint32), np.array([2], dtype=np.uint8)):
         with pytest.raises(RuntimeError, match="no CPU path"):
             kernels.dilution_tree_accept(q, k, v, com, 36, lse, good)
 
