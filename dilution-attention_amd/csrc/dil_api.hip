@@ -57,6 +57,16 @@ dil::RowsView view_of(const dil_rows* r, int64_t batch, int64_t heads, int64_t r
   const uint32_t magic = static_cast<uint32_t>(((uint64_t{1} << 32) + h - 1) / h);
   return dil::RowsView{h, magic, r->batch_stride, r->head_stride, row_stride};
 }
+// codes are read in 16-byte pieces, a row's scales (1 to 8 bytes) in one
+bool valid_fp4(const dil_fp4_cache* c) {
+  return c != nullptr && all_set(static_cast<const void*>(c->codes), static_cast<const void*>(c->scales)) &&
+         aligned16(c->codes) && reinterpret_cast<uintptr_t>(c->scales) % 8 == 0;
+}
+dil::Fp4Cache fp4_of(const dil_fp4_cache* c) { return dil::Fp4Cache{c->codes, c->scales}; }
+// rows of one call: at least one, and no more than a grid's 2^32 threads take
+bool valid_fp4_range(int64_t rows, int64_t capacity, int head_dim) {
+  return rows >= 1 && capacity < (int64_t{1} << 31) && rows <= capacity && rows * head_dim < (int64_t{1} << 36);
+}
 // slices are counted in 32 bits by the views, and their batch found by one
 // multiplication (RowsView)
 bool valid_slices(int64_t batch, int64_t heads) {
@@ -590,6 +600,56 @@ int dil_evict(const void* k_cache, const void* v_cache, const float* committed, 
   return dil::evict(dil::EvictArgs{k_cache, v_cache, committed, capacity, n, length, keep, first, recent, out_capacity,
                                    head_dim, dtype, k_out, v_out, committed_out, index, workspace, workspace_bytes,
                                    stream});
+}
+
+// ---------------------------------------------------------------------------
+// caches in 4 bits
+
+int dil_fp4_write(const dil_rows* k, const dil_rows* v, int64_t batch, int64_t heads, int64_t rows, int64_t start,
+                  const int64_t* start_dev, int64_t capacity, int head_dim, int dtype, const dil_fp4_cache* k_cache,
+                  const dil_fp4_cache* v_cache, void* stream) {
+  if (!valid_head_dim(head_dim)) return dil::kErrHeadDim;
+  if (!valid_dtype(dtype)) return dil::kErrDtype;
+  if (!valid_slices(batch, heads) || !valid_fp4_range(rows, capacity, head_dim) ||
+      (start_dev == nullptr && (start < 0 || start > capacity - rows)))
+    return dil::kErrShape;
+  if (!valid_rows(k, batch, heads, head_dim, dtype) || !valid_rows(v, batch, heads, head_dim, dtype) ||
+      !valid_fp4(k_cache) || !valid_fp4(v_cache))
+    return dil::kErrShape;
+  return dil::fp4_write(dil::Fp4WriteArgs{k->data, view_of(k, batch, heads, rows, head_dim), v->data,
+                                          view_of(v, batch, heads, rows, head_dim), fp4_of(k_cache), fp4_of(v_cache),
+                                          batch * heads, rows, capacity, start, start_dev, head_dim, dtype, stream});
+}
+
+int dil_fp4_read(const dil_fp4_cache* k_cache, const dil_fp4_cache* v_cache, int64_t n, int64_t capacity, int64_t start,
+                 int64_t rows, int head_dim, int dtype, void* k, void* v, void* stream) {
+  if (!valid_head_dim(head_dim)) return dil::kErrHeadDim;
+  if (!valid_dtype(dtype)) return dil::kErrDtype;
+  if (n < 1 || n >= (int64_t{1} << 31) || !valid_fp4_range(rows, capacity, head_dim) || start < 0 || start > capacity - rows)
+    return dil::kErrShape;
+  if (!valid_fp4(k_cache) || !valid_fp4(v_cache) || !all_set(k, v) || !aligned16(k, v)) return dil::kErrShape;
+  return dil::fp4_read(dil::Fp4ReadArgs{fp4_of(k_cache), fp4_of(v_cache), n, rows, capacity, start, k, v, head_dim, dtype,
+                                        stream});
+}
+
+int64_t dil_decode_fp4_workspace_bytes(int64_t n, int64_t length, int head_dim) {
+  return dil::decode_fp4_workspace_bytes(n, length, head_dim);
+}
+
+int dil_decode_step_fp4(const void* q1, const void* k1, const void* v1, const dil_fp4_cache* k_cache,
+                        const dil_fp4_cache* v_cache, float* committed, void* out, int64_t n, int64_t capacity,
+                        int64_t length, const int64_t* length_dev, int head_dim, int q_dtype, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  if (!valid_head_dim(head_dim)) return dil::kErrHeadDim;
+  if (!valid_dtype(q_dtype)) return dil::kErrDtype;
+  if (n < 1 || n >= (int64_t{1} << 31) || length < 1 || length > capacity || capacity >= (int64_t{1} << 31))
+    return dil::kErrShape;
+  if (!all_set(q1, static_cast<const void*>(committed), static_cast<const void*>(out), static_cast<const void*>(workspace)) ||
+      (k1 == nullptr) != (v1 == nullptr) || !aligned16(q1, k1, v1) || !valid_fp4(k_cache) || !valid_fp4(v_cache))
+    return dil::kErrShape;
+  if (workspace_bytes < dil::decode_fp4_workspace_bytes(n, length, head_dim)) return dil::kErrWorkspace;
+  return dil::decode_fp4(dil::Fp4DecodeArgs{q1, k1, v1, fp4_of(k_cache), fp4_of(v_cache), committed, out, n, capacity, length,
+                                            length_dev, head_dim, q_dtype, workspace, workspace_bytes, stream});
 }
 
 }  // extern "C"

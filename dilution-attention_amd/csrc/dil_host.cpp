@@ -49,6 +49,10 @@ struct Api {
   decltype(&dil_tree_accept) tree_accept = nullptr;
   decltype(&dil_evict_workspace_bytes) evict_workspace_bytes = nullptr;
   decltype(&dil_evict) evict = nullptr;
+  decltype(&dil_fp4_write) fp4_write = nullptr;
+  decltype(&dil_fp4_read) fp4_read = nullptr;
+  decltype(&dil_decode_fp4_workspace_bytes) decode_fp4_workspace_bytes = nullptr;
+  decltype(&dil_decode_step_fp4) decode_step_fp4 = nullptr;
 };
 Api api;
 bool bound = false;
@@ -77,6 +81,10 @@ void bind(const py::dict& a) {
   take(api.tree_accept, a, "dil_tree_accept");
   take(api.evict_workspace_bytes, a, "dil_evict_workspace_bytes");
   take(api.evict, a, "dil_evict");
+  take(api.fp4_write, a, "dil_fp4_write");
+  take(api.fp4_read, a, "dil_fp4_read");
+  take(api.decode_fp4_workspace_bytes, a, "dil_decode_fp4_workspace_bytes");
+  take(api.decode_step_fp4, a, "dil_decode_step_fp4");
   bound = true;
 }
 
@@ -526,6 +534,151 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> evict(const at::Tenso
 }
 
 // ---------------------------------------------------------------------------
+// caches in 4 bits
+
+// A cache's two tensors; returns (B, H, capacity, D) as the codes' shape says.
+struct Fp4Shape {
+  int64_t batch, heads, capacity, head_dim;
+};
+Fp4Shape check_fp4(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc, const at::Tensor& vs) {
+  if (kc.dim() != 4 || !kc.sizes().equals(vc.sizes()))
+    throw py::value_error("k_cache and v_cache must both hold (B, H, capacity, D / 2) codes, got " + dims(kc) + " and " + dims(vc));
+  const Fp4Shape s{kc.size(0), kc.size(1), kc.size(2), 2 * kc.size(3)};
+  check_head_dim(s.head_dim, nullptr);
+  for (const at::Tensor* x : {&ks, &vs})
+    if (x->dim() != 4 || x->size(0) != s.batch || x->size(1) != s.heads || x->size(2) != s.capacity ||
+        x->size(3) != (s.head_dim < 32 ? 1 : s.head_dim / 32))
+      throw py::value_error("the scales of " + dims(kc) + " codes must be (B, H, capacity, D / min(32, D)), got " + dims(*x));
+  for (const at::Tensor* x : {&kc, &ks, &vc, &vs})
+    if (x->scalar_type() != at::kByte || !x->is_contiguous())
+      throw py::value_error("codes and scales must be contiguous uint8 tensors");
+  for (const at::Tensor* x : {&kc, &vc})
+    if (reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 != 0) throw py::value_error("codes must be 16-byte aligned");
+  for (const at::Tensor* x : {&ks, &vs})
+    if (reinterpret_cast<uintptr_t>(x->data_ptr()) % 8 != 0) throw py::value_error("scales must be 8-byte aligned");
+  return s;
+}
+dil_fp4_cache fp4_ref(const at::Tensor& codes, const at::Tensor& scales) { return {codes.data_ptr(), scales.data_ptr()}; }
+const int64_t* device_number(const Maybe& x, const at::Tensor& like, const char* name) {
+  if (!x) return nullptr;
+  if (x->scalar_type() != at::kLong || x->numel() != 1 || x->device() != like.device())
+    throw py::value_error(std::string(name) + " must be a Python int or one int64 element on the caches' device");
+  return static_cast<const int64_t*>(x->data_ptr());
+}
+
+void fp4_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc,
+               const at::Tensor& vs, const Maybe& start_dev, int64_t start, uintptr_t stream) {
+  const Fp4Shape s = check_fp4(kc, ks, vc, vs);
+  if (k.dim() != 4 || !k.sizes().equals(v.sizes()) || k.size(0) != s.batch || k.size(1) != s.heads || k.size(3) != s.head_dim)
+    throw py::value_error("rows " + dims(k) + " and " + dims(v) + " do not match the cache's (" + std::to_string(s.batch) + ", " +
+                          std::to_string(s.heads) + ", ., " + std::to_string(s.head_dim) + ")");
+  const int64_t rows = k.size(2);
+  if (!k.is_floating_point() || !v.is_floating_point()) throw py::value_error("k and v must be float tensors");
+  if (rows > s.capacity || (!start_dev && (start < 0 || start > s.capacity - rows)))
+    throw py::value_error("rows [" + std::to_string(start) + ", " + std::to_string(start) + " + " + std::to_string(rows) +
+                          ") outside cache capacity " + std::to_string(s.capacity));
+  check_device({&kc, &ks, &vc, &vs, &k, &v});
+  const int64_t* at = device_number(start_dev, kc, "start");
+  need_library();
+  if (k.numel() == 0) return;
+  c10::DeviceGuard guard(k.device());
+  const at::ScalarType type = supported(at::promote_types(k.scalar_type(), v.scalar_type()));
+  const auto sd = slice_dims(s.batch, s.heads);
+  const at::Tensor kr = sliced(operand(k, type, false), sd), vr = sliced(operand(v, type, false), sd);
+  launch("dil_fp4_write", [&]() -> int {
+    const dil_rows rk = row_ref(kr), rv = row_ref(vr);
+    const dil_fp4_cache ck = fp4_ref(kc, ks), cv = fp4_ref(vc, vs);
+    return api.fp4_write(&rk, &rv, sd.first, sd.second, rows, start, at, s.capacity, static_cast<int>(s.head_dim),
+                         type_code(type), &ck, &cv, reinterpret_cast<void*>(stream));
+  });
+}
+
+std::tuple<at::Tensor, at::Tensor> fp4_read(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc,
+                                            const at::Tensor& vs, int64_t start, int64_t rows, int type, uintptr_t stream) {
+  const Fp4Shape s = check_fp4(kc, ks, vc, vs);
+  if (start < 0 || rows < 0 || rows > s.capacity || start > s.capacity - rows)
+    throw py::value_error("rows [" + std::to_string(start) + ", " + std::to_string(start) + " + " + std::to_string(rows) +
+                          ") outside cache capacity " + std::to_string(s.capacity));
+  check_device({&kc, &ks, &vc, &vs});
+  need_library();
+  c10::DeviceGuard guard(kc.device());
+  const auto o = kc.options().dtype(type == 0 ? at::kFloat : type == 1 ? at::kBFloat16 : at::kHalf);
+  at::Tensor k = at::empty({s.batch, s.heads, rows, s.head_dim}, o), v = at::empty_like(k);
+  if (k.numel() == 0) return {k, v};
+  launch("dil_fp4_read", [&]() -> int {
+    const dil_fp4_cache ck = fp4_ref(kc, ks), cv = fp4_ref(vc, vs);
+    return api.fp4_read(&ck, &cv, s.batch * s.heads, s.capacity, start, rows, static_cast<int>(s.head_dim), type, k.data_ptr(),
+                        v.data_ptr(), reinterpret_cast<void*>(stream));
+  });
+  return {k, v};
+}
+
+at::Tensor decode_step_fp4(const at::Tensor& q1, const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc,
+                           const at::Tensor& vs, const at::Tensor& committed, const Maybe& length_dev, int64_t length,
+                           const Maybe& k1, const Maybe& v1, const Maybe& into, const Maybe& scratch, uintptr_t stream) {
+  const Fp4Shape s = check_fp4(kc, ks, vc, vs);
+  const int64_t n = s.batch * s.heads, d = s.head_dim;
+  auto row_each = [&](const at::Tensor& x, const char* name) {
+    if (x.dim() != 4 || x.size(0) != s.batch || x.size(1) != s.heads || x.size(2) != 1 || x.size(3) != d)
+      throw py::value_error(std::string(name) + " must hold one row of every slice, (" + std::to_string(s.batch) + ", " +
+                            std::to_string(s.heads) + ", 1, " + std::to_string(d) + "), got " + dims(x));
+    if (!x.is_floating_point()) throw py::value_error(std::string(name) + " must be a float tensor");
+  };
+  row_each(q1, "q1");
+  if (k1.has_value() != v1.has_value()) throw py::value_error("k1 and v1 go together");
+  if (k1) {
+    row_each(*k1, "k1");
+    row_each(*v1, "v1");
+    if (k1->scalar_type() != q1.scalar_type() || v1->scalar_type() != q1.scalar_type())
+      throw py::value_error("k1 and v1 must have q1's dtype");
+  }
+  if (committed.dim() != 3 || committed.size(0) != s.batch || committed.size(1) != s.heads || committed.size(2) != s.capacity)
+    throw py::value_error("committed must be (B, H, capacity) = (" + std::to_string(s.batch) + ", " + std::to_string(s.heads) +
+                          ", " + std::to_string(s.capacity) + "), got " + dims(committed));
+  if (committed.scalar_type() != at::kFloat || !committed.is_contiguous())
+    throw py::value_error("committed must be a contiguous float32 tensor");
+  if (length < 1 || length > s.capacity)
+    throw py::value_error("length " + std::to_string(length) + " outside cache capacity " + std::to_string(s.capacity));
+  check_device({&kc, &ks, &vc, &vs, &q1, &committed});
+  if (k1) check_device({&kc, &*k1, &*v1});
+  const int64_t* live = device_number(length_dev, kc, "length");
+  need_library();
+  c10::DeviceGuard guard(kc.device());
+  // q1 keeps its own dtype, which is the output's; the new rows come in it too
+  const at::ScalarType qt = supported(q1.scalar_type());
+  auto flat = [&](const at::Tensor& x) {
+    const at::Tensor y = (x.scalar_type() == qt ? x : x.to(qt)).contiguous();
+    return reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0 ? y : y.clone();
+  };
+  const at::Tensor qf = flat(q1);
+  const Maybe kf = k1 ? Maybe(flat(*k1)) : Maybe(), vf = v1 ? Maybe(flat(*v1)) : Maybe();
+  at::Tensor out;
+  if (into) {
+    out = *into;
+    if (out.scalar_type() != qt || out.numel() != n * d || !out.is_contiguous() || out.device() != kc.device())
+      throw py::value_error("out must be a contiguous (B, H, D) tensor in q1's dtype on the caches' device");
+  } else {
+    out = at::empty({s.batch, s.heads, 1, d}, qf.options());
+  }
+  const int64_t need = api.decode_fp4_workspace_bytes(n, length, static_cast<int>(d));
+  if (scratch && (scratch->scalar_type() != at::kByte || !scratch->is_contiguous() || scratch->numel() < need ||
+                  scratch->device() != kc.device()))
+    throw py::value_error("workspace must be a contiguous uint8 tensor of at least " + std::to_string(need) +
+                          " bytes on the caches' device");
+  if (n > 0) {
+    const at::Tensor ws = scratch ? *scratch : workspace(need, kc);
+    launch("dil_decode_step_fp4", [&]() -> int {
+      const dil_fp4_cache ck = fp4_ref(kc, ks), cv = fp4_ref(vc, vs);
+      return api.decode_step_fp4(qf.data_ptr(), kf ? kf->data_ptr() : nullptr, vf ? vf->data_ptr() : nullptr, &ck, &cv,
+                                 f32(committed), out.data_ptr(), n, s.capacity, length, live, static_cast<int>(d),
+                                 type_code(qt), ws.data_ptr(), ws.numel(), reinterpret_cast<void*>(stream));
+    });
+  }
+  const at::Tensor y = out.view({s.batch, s.heads, 1, d});
+  return q1.scalar_type() == qt ? y : y.to(q1.scalar_type());
+}
+
+// ---------------------------------------------------------------------------
 // the decode step's few-row projections
 
 enum { kPlain = 0, kResid = 1, kNorm = 2, kSwiglu = 3 };
@@ -622,6 +775,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("tree_step", &tree_step);
   m.def("tree_accept", &tree_accept);
   m.def("evict", &evict);
+  m.def("fp4_write", &fp4_write);
+  m.def("fp4_read", &fp4_read);
+  m.def("decode_step_fp4", &decode_step_fp4);
   m.def("rows_linear", &rows_linear);
   m.def("rows_linear_qkv", &rows_linear_qkv);
 }

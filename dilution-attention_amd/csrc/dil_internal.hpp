@@ -262,4 +262,51 @@ struct EvictArgs {
 int64_t evict_workspace_bytes(int64_t n, int64_t length, int64_t keep);
 int evict(const EvictArgs& a);
 
+// Caches in 4 bits (dil_fp4.hpp): rows written and read back (dil_fp4.hip), the decode step
+// over them (dil_decode_fp4.hip).
+struct Fp4Cache {
+  void* codes;               // (n, cap, D / 2) bytes
+  void* scales;              // (n, cap, D / min(32, D)) bytes
+};
+
+struct Fp4WriteArgs {
+  const void* k;             // `rows` rows per slice, in dtype
+  RowsView kv;
+  const void* v;
+  RowsView vv;
+  Fp4Cache k_cache, v_cache;
+  int64_t n, rows, capacity, start;
+  const int64_t* start_dev;  // null, or the position of the first row in device memory
+  int head_dim, dtype;
+  void* stream;
+};
+int fp4_write(const Fp4WriteArgs& a);
+
+struct Fp4ReadArgs {
+  Fp4Cache k_cache, v_cache;
+  int64_t n, rows, capacity, start;
+  void* k;                   // (n, rows, D) in dtype
+  void* v;
+  int head_dim, dtype;
+  void* stream;
+};
+int fp4_read(const Fp4ReadArgs& a);
+
+struct Fp4DecodeArgs {
+  const void* q1;            // (n, D) in q_dtype
+  const void* k1;            // the new token's rows (n, D) in q_dtype, or null: they are in the caches
+  const void* v1;
+  Fp4Cache k_cache, v_cache;
+  float* committed;          // (n, cap) fp32
+  void* out;                 // (n, D) in q_dtype
+  int64_t n, capacity, length;
+  const int64_t* dlen;       // as in DecodeArgs
+  int head_dim, q_dtype;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* stream;
+};
+int64_t decode_fp4_workspace_bytes(int64_t n, int64_t length, int head_dim);
+int decode_fp4(const Fp4DecodeArgs& a);
+
 }  // namespace dil

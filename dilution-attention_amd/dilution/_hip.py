@@ -29,6 +29,15 @@ class Rows(ctypes.Structure):
 
 _rows_p = ctypes.POINTER(Rows)
 
+
+class Fp4Cache(ctypes.Structure):
+    """``dil_fp4_cache``: the codes and scales of a cache in 4 bits."""
+
+    _fields_ = [("codes", _vp), ("scales", _vp)]
+
+
+_fp4_p = ctypes.POINTER(Fp4Cache)
+
 # name -> (restype, argtypes); must match include/dilution_hip.h
 SIGNATURES = {
     "dil_abi_version": (_c_int, []),
@@ -87,6 +96,12 @@ SIGNATURES = {
     "dil_evict_workspace_bytes": (_c_int64, [_c_int64, _c_int64, _c_int64]),
     "dil_evict": (_c_int, [_vp, _vp, _vp, _c_int64, _c_int64, _c_int64, _c_int64, _c_int64, _c_int64, _c_int64, _c_int,
                            _c_int, _vp, _vp, _vp, _vp, _vp, _c_int64, _vp]),
+    "dil_fp4_write": (_c_int, [_rows_p, _rows_p, _c_int64, _c_int64, _c_int64, _c_int64, _vp, _c_int64, _c_int, _c_int,
+                               _fp4_p, _fp4_p, _vp]),
+    "dil_fp4_read": (_c_int, [_fp4_p, _fp4_p, _c_int64, _c_int64, _c_int64, _c_int64, _c_int, _c_int, _vp, _vp, _vp]),
+    "dil_decode_fp4_workspace_bytes": (_c_int64, [_c_int64, _c_int64, _c_int]),
+    "dil_decode_step_fp4": (_c_int, [_vp, _vp, _vp, _fp4_p, _fp4_p, _vp, _vp, _c_int64, _c_int64, _c_int64, _vp, _c_int,
+                                     _c_int, _vp, _c_int64, _vp]),
     "dil_timing_enable": (_c_int, [_c_int]),
     "dil_timing_reset": (_c_int, []),
     "dil_timing_count": (_c_int, []),

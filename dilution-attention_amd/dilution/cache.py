@@ -27,6 +27,11 @@ of them, of which one path is taken), and ``evict_cache`` shrinks a cache to the
 keys that carry the demand.  The reference has no counterpart: it decodes one
 token at a time and its caches only grow.  Between a tree step and the next
 change of the length the dict also holds ``draft``, the number of that step.
+
+A cache may hold its rows in 4 bits: ``k`` and ``v`` are then ``kernels.Fp4Rows``
+(``begin_cache(..., bits=4)`` or ``pack_cache``; ``unpack_cache`` is the way back).
+``append_kv`` and ``step_cache`` take both kinds; a tree step and an eviction need
+ordinary rows.
 """
 
 from __future__ import annotations
@@ -67,27 +72,82 @@ def moved_on(cache: dict, length: int) -> None:
     cache.pop("draft", None)
 
 
+def is_packed(cache: dict) -> bool:
+    """Whether the cache holds its rows in 4 bits."""
+    return isinstance(cache["k"], kernels.Fp4Rows)
+
+
+def _need_rows(cache: dict, what: str) -> None:
+    if is_packed(cache):
+        raise ValueError(f"{what} needs a cache of ordinary rows: unpack_cache() makes one of a 4-bit cache")
+
+
+def pack_cache(cache: dict, capacity: int | None = None) -> dict:
+    """A cache in 4 bits of ``max(capacity, length)`` positions (``capacity`` defaults to the
+    given one's) with the rows of a cache of ordinary ones, quantised, and its demand.  The
+    cache given is not changed."""
+    _need_rows(cache, "pack_cache")
+    k, v, length = cache["k"], cache["v"], cache["len"]
+    batch, heads, old, head_dim = k.shape
+    capacity = max(old if capacity is None else capacity, length)
+    rows = [kernels.alloc_fp4_rows(batch, heads, capacity, head_dim, k.device) for _ in range(2)]
+    kernels.dilution_fp4_write(k[:, :, :length], v[:, :, :length], *rows, 0)
+    return {"k": rows[0], "v": rows[1], "len": length, "committed": _demand_in(cache, capacity)}
+
+
+def unpack_cache(cache: dict, capacity: int | None = None, dtype: torch.dtype = torch.bfloat16) -> dict:
+    """A cache of ordinary rows in ``dtype``, with ``max(capacity, length)`` positions, holding what
+    a cache in 4 bits stands for, and its demand.  The cache given is not changed."""
+    if not is_packed(cache):
+        raise ValueError("unpack_cache needs a cache in 4 bits")
+    capacity = cache["k"].shape[2] if capacity is None else capacity
+    k, v = kernels.dilution_fp4_read(cache["k"], cache["v"], 0, cache["len"], dtype)
+    new = alloc_cache(k, v, capacity)
+    new["committed"] = _demand_in(cache, new["k"].shape[2])
+    return new
+
+
+def _demand_in(cache: dict, capacity: int) -> torch.Tensor:
+    """The demand of the cached positions in a new buffer of `capacity`, zero behind them."""
+    new = cache["committed"].new_zeros(*cache["committed"].shape[:2], capacity)
+    new[:, :, : cache["len"]] = cache["committed"][:, :, : cache["len"]]
+    return new
+
+
 def append_kv(cache: dict, k1: torch.Tensor, v1: torch.Tensor) -> int:
     """Write one new position (k1, v1: (B, H, 1, D)) and return the new
     length (model.py:86-93)."""
     t = cache["len"]
     if t >= cache["k"].shape[2]:
         raise ValueError("decode step past the cache capacity (context_length)")
-    cache["k"][:, :, t] = k1[:, :, 0]
-    cache["v"][:, :, t] = v1[:, :, 0]
+    if is_packed(cache):
+        kernels.dilution_fp4_write(k1, v1, cache["k"], cache["v"], t)
+    else:
+        cache["k"][:, :, t] = k1[:, :, 0]
+        cache["v"][:, :, t] = v1[:, :, 0]
     moved_on(cache, t + 1)
     return t + 1
 
 
 def begin_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, capacity: int | None = None,
-                chunk: int | None = None, dot_precision: str | None = None, **bid_kw):
+                chunk: int | None = None, dot_precision: str | None = None, bits: int | None = None, **bid_kw):
     """Prefill a prompt: returns (y, cache) with y (B, H, T, D) in q.dtype.
 
     chunk=None runs the one-call forward and copies ``committed_total`` into
     the cache (model.py:202-228); chunk=C prefills C rows at a time with the
     demand carried in the cache's buffer.  ``bid_kw`` (bid, share_cumsum,
-    shift) selects an ablation variant, always prefilled in one call.
+    shift) selects an ablation variant, always prefilled in one call.  bits=4
+    gives a cache in 4 bits (``pack_cache``): the prompt's own rows are computed from
+    its unrounded keys and values, the steps behind it from the quantised ones; production
+    operator only.
     """
+    if bits is not None:
+        if bits != 4:
+            raise ValueError(f"bits must be None or 4, got {bits}")
+        if bid_kw:
+            raise ValueError("a cache in 4 bits needs the production operator")
+        y, cache = begin_cache(q, k, v, chunk=chunk, dot_precision=dot_precision)
+        return y, pack_cache(cache, capacity)
     prec = dot_precision or _precision(q.dtype)
     seq = q.shape[2]
     cache = alloc_cache(k, v, capacity)
@@ -116,6 +176,15 @@ def step_cache(q1: torch.Tensor, k1: torch.Tensor, v1: torch.Tensor, cache: dict
     """One decode token: append (k1, v1) and return the new row's output
     (B, H, 1, D) in q1.dtype, advancing the cache's demand in place
     (model.py:231-241); ``bid_kw`` as in ``begin_cache``."""
+    if is_packed(cache):
+        if bid_kw:
+            raise ValueError("a cache in 4 bits needs the production operator")
+        t = cache["len"]
+        if t >= cache["k"].shape[2]:
+            raise ValueError("decode step past the cache capacity (context_length)")
+        y = kernels.dilution_decode_step_fp4(q1, cache["k"], cache["v"], cache["committed"], t + 1, k1, v1)
+        moved_on(cache, t + 1)
+        return y
     t = append_kv(cache, k1, v1)
     if bid_kw:
         return kernels_bid.dilution_decode_step(q1, cache["k"], cache["v"], cache["committed"], t, **bid_kw)
@@ -130,6 +199,7 @@ def tree_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: dict, pa
     length and demand stay.  A later step overwrites rows that were not accepted:
     of several tree steps the last one's draft can be, until the cache moves on."""
     # all that the kernels would refuse, before any row is written
+    _need_rows(cache, "a tree step")
     if q.dim() != 4 or k.shape != q.shape or v.shape != q.shape:
         raise ValueError(f"q, k and v must have one shape (B, H, N, D), got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     batch, heads, capacity, head_dim = cache["k"].shape
@@ -177,6 +247,7 @@ def evict_cache(cache: dict, keep: int, first: int = 0, recent: int = 0, capacit
     have had the fewest rows to gather demand from), in new buffers of
     ``max(capacity, keep)`` positions.  The keys hold no position, so decoding
     goes on over the kept ones.  A cache of at most ``keep`` positions is returned as it is."""
+    _need_rows(cache, "an eviction")
     if cache["len"] <= keep:
         return cache
     k, v, committed, _ = kernels.dilution_evict(cache["k"], cache["v"], cache["committed"], cache["len"], keep,

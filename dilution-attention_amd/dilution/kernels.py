@@ -25,6 +25,7 @@ and ignored: tiles are fixed for gfx950.
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -559,3 +560,99 @@ def dilution_evict(
     """
     capacity = max(keep if capacity is None else capacity, keep)
     return _native().evict(k_cache, v_cache, committed, length, keep, first, recent, capacity, _raw_stream(k_cache))
+
+
+# ---------------------------------------------------------------------------
+# caches in 4 bits (no reference counterpart; the reference's caches hold the
+# activations' type)
+
+
+class Fp4Rows(NamedTuple):
+    """The rows of a K or V cache in 4 bits: codes (B, H, capacity, D / 2) and scales
+    (B, H, capacity, D / min(32, D)), both contiguous uint8.
+
+    An element is 4 bits (the even one of a pair in the low half of its byte): a sign
+    over one of 0, 0.5, 1, 1.5, 2, 3, 4, 6, times the power of two 2^(s - 127) of its block
+    of min(32, D) elements.  The power is the smallest at which no element of the block
+    rounds beyond 6, within 2^-125 and 2^125 (past which elements count as 6): an element is off by at most half a
+    step, 1/6 of the block's largest.  s = 255: the block held a NaN or an infinity
+    and is NaN throughout; s = 0: rows that were never written, all 0."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self) -> torch.Size:
+        """(B, H, capacity, D) of the rows that the codes stand for."""
+        return torch.Size((*self.codes.shape[:3], 2 * self.codes.shape[3]))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+
+def alloc_fp4_rows(batch: int, heads: int, capacity: int, head_dim: int, device="cuda") -> Fp4Rows:
+    """Cleared ``Fp4Rows`` of (B, H, capacity, D): every row reads as zeros."""
+    _check_head_dim(head_dim)
+    return Fp4Rows(torch.zeros(batch, heads, capacity, head_dim // 2, dtype=torch.uint8, device=device),
+                   torch.zeros(batch, heads, capacity, head_dim // min(32, head_dim), dtype=torch.uint8, device=device))
+
+
+def _host_or_device(x) -> tuple:
+    """(None, x) for a host number, (x, 0) for a device tensor."""
+    return (x, 0) if torch.is_tensor(x) and x.is_cuda else (None, int(x))
+
+
+def dilution_fp4_write(k: torch.Tensor, v: torch.Tensor, k_cache: Fp4Rows, v_cache: Fp4Rows, start) -> None:
+    """Quantise the rows k and v (B, H, T, D) (any float type; views of a fused
+    projection need no copy) into positions [start, start + T) of the caches, in
+    place.  ``start`` is a host number, or one int64 element on the caches' device,
+    read when the kernel runs (as in a graph replay): rows that it would put outside
+    the cache are dropped.  Other positions stay as they are."""
+    dev, host = _host_or_device(start)
+    _native().fp4_write(k, v, *k_cache, *v_cache, dev, host, _raw_stream(k_cache.codes))
+
+
+def dilution_fp4_read(k_cache: Fp4Rows, v_cache: Fp4Rows, start: int, count: int,
+                      dtype: torch.dtype = torch.bfloat16) -> tuple:
+    """What positions [start, start + count) of the caches stand for: new (B, H, count, D)
+    tensors (k, v) in ``dtype`` (float32, bfloat16 or float16; exact, but for
+    values past float16's range, which round as any conversion does)."""
+    if dtype not in _DTYPES:
+        raise ValueError("dtype must be float32, bfloat16 or float16")
+    return _native().fp4_read(*k_cache, *v_cache, start, count, _DTYPES[dtype], _raw_stream(k_cache.codes))
+
+
+def dilution_decode_step_fp4(q1: torch.Tensor, k_cache: Fp4Rows, v_cache: Fp4Rows, committed: torch.Tensor,
+                             length: int, k1: torch.Tensor | None = None, v1: torch.Tensor | None = None) -> torch.Tensor:
+    """``dilution_decode_step`` over caches in 4 bits: the step on the values that they
+    stand for, in fp32; returns the new row's output (B, H, 1, D) in q1.dtype, rounded once.
+
+    q1: (B, H, 1, D).  committed: contiguous (B, H, capacity) fp32, zero at
+    position length - 1; advanced in place over [0, length).  k1, v1 ((B, H, 1, D) in
+    q1.dtype): the new token's rows, which the call quantises into position
+    length - 1 first, as ``dilution_fp4_write`` would; without them that position is
+    written already.  A slice's bits may differ in calls of another B * H or length."""
+    return _native().decode_step_fp4(q1, *k_cache, *v_cache, committed, None, int(length), k1, v1, None, None,
+                                     _raw_stream(k_cache.codes))
+
+
+def decode_step_fp4_device_length(q1: torch.Tensor, k_cache: Fp4Rows, v_cache: Fp4Rows, committed: torch.Tensor,
+                                  length: torch.Tensor, max_length: int, k1: torch.Tensor | None = None,
+                                  v1: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                                  workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """``dilution_decode_step_fp4`` with the length in device memory, as
+    ``decode_step_device_length``: one int64 element on the caches' device, read when the
+    kernels run and clamped to [0, max_length], so that one captured HIP graph serves
+    every decode step.  ``out`` ((B, H, D) in q1's dtype) and ``workspace``
+    (``decode_fp4_workspace(...)``) may be given so that the call allocates nothing.
+    Results equal ``dilution_decode_step_fp4`` at the live length, bitwise."""
+    if not torch.is_tensor(length):
+        raise ValueError("length must be one int64 element on the caches' device")
+    return _native().decode_step_fp4(q1, *k_cache, *v_cache, committed, length, int(max_length), k1, v1, out, workspace,
+                                     _raw_stream(k_cache.codes))
+
+
+def decode_fp4_workspace(batch: int, heads: int, max_length: int, head_dim: int, device) -> torch.Tensor:
+    """A workspace for ``decode_step_fp4_device_length`` up to ``max_length``."""
+    return _workspace(_hip.lib().dil_decode_fp4_workspace_bytes(batch * heads, max_length, head_dim), device)

@@ -194,7 +194,9 @@ class SoftmaxAttention(_AttentionBase):
         q, k, v = self._split_heads(x)
         return self._merge_heads(_sdpa(q, k, v, True), batch, seq)
 
-    def begin_cache(self, x: torch.Tensor, capacity: int | None = None):
+    def begin_cache(self, x: torch.Tensor, capacity: int | None = None, bits: int | None = None):
+        if bits is not None:
+            raise ValueError("a cache in 4 bits needs the production dilution operator")
         batch, seq, _ = x.shape
         q, k, v = self._split_heads(x)
         y = self._merge_heads(_sdpa(q, k, v, True), batch, seq)
@@ -230,11 +232,11 @@ class DilutionAttention(_AttentionBase):
             y = ops.dilution_attention_forward(q, k, v, dot_precision=prec, **self.bid_kw)
         return self._merge_heads(y.to(x.dtype), batch, seq)
 
-    def begin_cache(self, x: torch.Tensor, capacity: int | None = None):
+    def begin_cache(self, x: torch.Tensor, capacity: int | None = None, bits: int | None = None):
         batch, seq, _ = x.shape
         q, k, v = self._split_heads(x)
         y, cache = dcache.begin_cache(q, k.contiguous(), v.contiguous(), capacity=capacity,
-                                      chunk=self.prefill_chunk, **self.bid_kw)
+                                      chunk=self.prefill_chunk, bits=bits, **self.bid_kw)
         return self._merge_heads(y.to(x.dtype), batch, seq), cache
 
     def step_cache(self, x1: torch.Tensor, cache: dict) -> torch.Tensor:
@@ -277,8 +279,8 @@ class Block(nn.Module):
         x = x + self.attn(self.ln_1(x))
         return x + self.mlp(self.ln_2(x))
 
-    def begin_cache(self, x: torch.Tensor, capacity: int | None = None):
-        y, cache = self.attn.begin_cache(self.ln_1(x), capacity)
+    def begin_cache(self, x: torch.Tensor, capacity: int | None = None, bits: int | None = None):
+        y, cache = self.attn.begin_cache(self.ln_1(x), capacity, bits)
         x = x + y
         return x + self.mlp(self.ln_2(x)), cache
 
@@ -332,11 +334,14 @@ class DilutionLM(nn.Module):
         return logits, loss
 
     @torch.no_grad()
-    def prefill(self, idx: torch.Tensor, capacity: int | None = None):
+    def prefill(self, idx: torch.Tensor, capacity: int | None = None, cache_bits: int | None = None):
+        """Logits (B, 1, vocab) behind a prompt and the layers' caches; ``cache_bits=4``
+        holds them in 4 bits (``cache.begin_cache``), each layer's ordinary rows released before
+        the next layer's are made."""
         x = self.wte(idx)
         caches = []
         for block in self.h:
-            x, cache = block.begin_cache(x, capacity)
+            x, cache = block.begin_cache(x, capacity, cache_bits)
             caches.append(cache)
         return self.lm_head(self.ln_f(x[:, [-1], :])), caches
 
@@ -347,16 +352,20 @@ class DilutionLM(nn.Module):
         torch's modules, the same computation up to accumulation order)."""
         batch = token.shape[0]
         if fused and self.fused_decode_eligible(batch):
+            new = self._new_row_buffers(caches)
+
             def slot(i):
                 cache = caches[i]
                 t = cache["len"]
                 if t >= cache["k"].shape[2]:
                     raise ValueError("decode step past the cache capacity (context_length)")
                 dcache.moved_on(cache, t + 1)
-                return cache["k"], cache["v"], t
+                return self._new_rows(cache, new, t)
 
             def attend(i, q1):
                 c = caches[i]
+                if dcache.is_packed(c):
+                    return kernels.dilution_decode_step_fp4(q1, c["k"], c["v"], c["committed"], c["len"], *new)
                 return kernels.dilution_decode_step(q1, c["k"], c["v"], c["committed"], c["len"])
 
             x2 = self._fused_layers(self.wte(token).view(batch, -1), slot, attend)
@@ -430,6 +439,21 @@ class DilutionLM(nn.Module):
                 and cfg.d_model % 256 == 0 and cfg.d_model <= _LIN_MAX_K
                 and hidden % 256 == 0 and hidden <= _LIN_MAX_K and 1 <= batch <= _LIN_MAX_ROWS)
 
+    def _new_row_buffers(self, caches) -> list | None:
+        """Where a fused step leaves the new token's k and v for caches in 4 bits, whose decode
+        step quantises them: (B, H, 1, D) buffers for all layers in turn (None without such caches)."""
+        packed = [c["k"] for c in caches if dcache.is_packed(c)]
+        if not packed:
+            return None
+        batch, heads, _, head_dim = packed[0].shape
+        return [torch.empty(batch, heads, 1, head_dim, device=packed[0].device, dtype=self.lm_head.weight.dtype)
+                for _ in range(2)]
+
+    @staticmethod
+    def _new_rows(cache: dict, new: list | None, pos):
+        """The buffers and position that ``rows_linear_qkv`` writes a layer's new k and v to."""
+        return (*new, 0) if dcache.is_packed(cache) else (cache["k"], cache["v"], pos)
+
     @staticmethod
     def _norm_eps(norm: nn.Module) -> float:
         return norm.eps if norm.eps is not None else torch.finfo(torch.bfloat16).eps
@@ -463,7 +487,7 @@ class DilutionLM(nn.Module):
     def generate(self, idx: torch.Tensor, max_new_tokens: int, temperature: float = 0.0,
                  top_k: int | None = None, top_p: float | None = None,
                  generator: torch.Generator | None = None, vocab_limit: int | None = None,
-                 graph: bool = False, eviction: "Eviction | None" = None) -> torch.Tensor:
+                 graph: bool = False, eviction: "Eviction | None" = None, cache_bits: int | None = None) -> torch.Tensor:
         """Cached generation with caches sized prompt + max_new_tokens
         (model.py:473-509): temperature 0 is greedy, otherwise a sample of
         softmax(logits / temperature) after top-k / nucleus truncation;
@@ -473,16 +497,23 @@ class DilutionLM(nn.Module):
         tokens, one HIP graph replay per step).  ``eviction`` bounds the caches:
         when they hold ``eviction.limit`` positions they shrink to its ``keep``, in
         buffers of at most ``limit`` positions, whatever the prompt's length (not
-        with ``graph``, whose captured step holds the caches' addresses)."""
+        with ``graph``, whose captured step holds the caches' addresses).
+        ``cache_bits=4`` holds the caches in 4 bits (``kernels.Fp4Rows``), a quarter
+        of the memory and of the decode step's traffic at the cost of their rounding
+        (not with ``eviction``, which moves ordinary rows)."""
         if vocab_limit is not None and not 0 < vocab_limit <= self.cfg.vocab_size:
             raise ValueError(f"vocab_limit must be in (0, {self.cfg.vocab_size}]")
+        if cache_bits is not None:
+            if eviction is not None:
+                raise ValueError("an eviction moves ordinary rows: it needs cache_bits=None")
+            self._need_production("cache_bits")
         capacity = idx.shape[1] + max_new_tokens
         if eviction is not None:
             if graph:
                 raise ValueError("a graph-replayed generation keeps its caches: eviction needs graph=False")
             self._need_production("eviction")
             capacity = min(capacity, max(idx.shape[1], eviction.limit))
-        logits, caches = self.prefill(idx, capacity=capacity)
+        logits, caches = self.prefill(idx, capacity=capacity, cache_bits=cache_bits)
         tokens = idx
         if graph and max_new_tokens > 0 and not (temperature and temperature > 0.0) and self.graph_decode_eligible():
             last = logits[:, -1, :].float()
@@ -635,7 +666,12 @@ class GraphDecoder:
         qdt = model.lm_head.weight.dtype
         self.outs = [torch.empty(self.batch, self.heads, self.head_dim, device=dev, dtype=qdt)
                      for _ in caches]
-        self.ws = kernels.decode_workspace(self.batch, self.heads, self.capacity, self.head_dim, dev)
+        if len({dcache.is_packed(c) for c in caches}) != 1:
+            raise ValueError("the layers' caches must all hold ordinary rows, or all 4-bit ones")
+        self.packed = dcache.is_packed(caches[0])
+        make = kernels.decode_fp4_workspace if self.packed else kernels.decode_workspace
+        self.ws = make(self.batch, self.heads, self.capacity, self.head_dim, dev)
+        self.new = model._new_row_buffers(caches)
         self.logits = torch.empty(self.batch, 1, model.cfg.vocab_size, device=dev, dtype=qdt)
         self.mask = None
         self.limit = model.cfg.vocab_size if vocab_limit is None else int(vocab_limit)
@@ -649,17 +685,25 @@ class GraphDecoder:
         """Layer i's cache append at the device-resident position and its
         decode step at the device-resident length."""
         cache = self.caches[i]
+        if self.packed:
+            return self._attend_packed(i, q1, k1, v1)
         cache["k"].index_copy_(2, self.pos, k1)
         cache["v"].index_copy_(2, self.pos, v1)
         return kernels.decode_step_device_length(q1, cache["k"], cache["v"], cache["committed"], self.live,
                                                  self.capacity, out=self.outs[i], workspace=self.ws)
 
-    def _slot(self, i: int):
+    def _attend_packed(self, i: int, q1, k1, v1) -> torch.Tensor:
         cache = self.caches[i]
-        return cache["k"], cache["v"], self.pos
+        return kernels.decode_step_fp4_device_length(q1, cache["k"], cache["v"], cache["committed"], self.live,
+                                                     self.capacity, k1, v1, out=self.outs[i], workspace=self.ws)
+
+    def _slot(self, i: int):
+        return self.model._new_rows(self.caches[i], self.new, self.pos)
 
     def _attend_q(self, i: int, q1) -> torch.Tensor:
         cache = self.caches[i]
+        if self.packed:
+            return self._attend_packed(i, q1, *self.new)
         return kernels.decode_step_device_length(q1, cache["k"], cache["v"], cache["committed"], self.live,
                                                  self.capacity, out=self.outs[i], workspace=self.ws)
 

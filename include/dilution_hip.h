@@ -36,7 +36,7 @@
  *     the call: the size of a call picks the order of some sums (the forward's
  *     for rows of at most 2048 keys, and at any length for operands other than
  *     bf16 at head_dim 64 and for prefill chunks that start off the multiples of
- *     512; dk's up to head_dim 128; the decode step's; the tree step's).
+ *     512; dk's up to head_dim 128; the decode steps'; the tree step's).
  *   - The forward's and the prefill's workspace queries are not monotone in the
  *     slice count: a smaller call may be quicker with up to 1 GiB of partials
  *     that a larger one has no use for.  A workspace sized for more slices of
@@ -425,6 +425,52 @@ int dil_evict(const void* k_cache, const void* v_cache, const float* committed, 
               int64_t length, int64_t keep, int64_t first, int64_t recent, int64_t out_capacity, int head_dim,
               int dtype, void* k_out, void* v_out, float* committed_out, int32_t* index, void* workspace,
               int64_t workspace_bytes, void* stream);
+
+/*
+ * Decode caches in 4 bits.  No counterpart in the reference, whose caches hold the
+ * activations' type (src/dilution/model.py:76-93).
+ *
+ * A cache of K (or V) rows is `codes`, (n, capacity, head_dim / 2) bytes, and `scales`,
+ * (n, capacity, head_dim / block) bytes with block = min(32, head_dim).  An element is 4
+ * bits, the even one of a pair in the low half: a sign over one of 0, 0.5, 1, 1.5, 2, 3, 4,
+ * 6 (in this order), times its block's 2^(s - 127), s the scale byte.  With 1.m 2^E the
+ * block's largest magnitude, s - 127 = E - 2, or E - 1 where 1.m >= 1.75, within [-125, 125];
+ * an element takes the nearest code, at most 6, and the one of even mantissa of two as near.
+ * s = 255: the block held a NaN or an infinity and stands for NaN throughout (its codes are
+ * 0); s = 0: a row of a cleared cache, all 0.  codes are 16-byte, scales 8-byte aligned.
+ *
+ * dil_fp4_write quantises `rows` rows per slice of k and v (dil_rows of `dtype`) into the
+ * positions from `start` on, or from the int64_t that start_dev points to on the device; rows
+ * that this would put outside [0, capacity) are dropped.  Nothing else in the caches changes.
+ * dil_fp4_read gives the values of positions [start, start + rows) as (n, rows, head_dim) of
+ * `dtype` (exact but for values past the type's range; a 16-byte aligned destination).
+ */
+typedef struct dil_fp4_cache {
+  void* codes;
+  void* scales;
+} dil_fp4_cache;
+
+int dil_fp4_write(const dil_rows* k, const dil_rows* v, int64_t batch, int64_t heads, int64_t rows, int64_t start,
+                  const int64_t* start_dev, int64_t capacity, int head_dim, int dtype, const dil_fp4_cache* k_cache,
+                  const dil_fp4_cache* v_cache, void* stream);
+int dil_fp4_read(const dil_fp4_cache* k_cache, const dil_fp4_cache* v_cache, int64_t n, int64_t capacity, int64_t start,
+                 int64_t rows, int head_dim, int dtype, void* k, void* v, void* stream);
+
+/*
+ * dil_decode_step over caches in 4 bits: the same step on the values that they stand for.
+ * q1, out: (n, head_dim) in q_dtype; committed (n, capacity) float32, advanced in place.
+ * k1, v1: the new token's rows (n, head_dim) in q_dtype, which the call quantises into
+ * position length - 1 first, or both NULL when they are there.  length_dev not NULL: the
+ * length is read from device memory when the kernels run (clamped to [0, length]; with 0
+ * nothing is read or written but out, which becomes 0), and `length` sizes grid and workspace.
+ * q1, k1 and v1 are 16-byte aligned.  The workspace query serves both forms and, without
+ * slices or keys, returns 0.
+ */
+int64_t dil_decode_fp4_workspace_bytes(int64_t n, int64_t length, int head_dim);
+int dil_decode_step_fp4(const void* q1, const void* k1, const void* v1, const dil_fp4_cache* k_cache,
+                        const dil_fp4_cache* v_cache, float* committed, void* out, int64_t n, int64_t capacity,
+                        int64_t length, const int64_t* length_dev, int head_dim, int q_dtype, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 /*
  * Kernel timing for measurement harnesses.  No reference counterpart (the
