@@ -9,12 +9,14 @@
 // and fp4_finish.
 //
 // A key costs D + 2 D / 32 bytes of codes and scales, 8 of demand and 8 of affinities (84 at
-// D = 64, where 16-bit caches take 272).  A lane reads 16 bytes of codes, one block of 32
-// elements, so the scales stay out of the walks: a K walk leaves each block's sum of q times
-// codes in LDS, where one thread a key applies the scales and adds the blocks; the shares go
-// into LDS once for each block, times the V scale.  bf16 queries multiply on v_dot2_f32_bf16
-// (codes are exact in bf16), others in fp32.
+// D = 64, where 16-bit caches take 272), so both walks have to be short of instructions.  The
+// scores come from the matrix unit, which takes codes and scales as they lie: 16 bytes of codes a
+// lane go from memory into its operand.  V rows need one conversion for two elements and one fma
+// each (fp32 sums); their scales stay out of the walk, since the shares go into LDS once for each
+// block, times its V scale.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "dil_decode_impl.hpp"
 #include "dil_fp4.hpp"
@@ -22,17 +24,56 @@
 namespace dil {
 namespace {
 
-constexpr int kQThreads = 1024;
+// One workgroup per slice takes 1024 threads; the chunked step workgroups of 256 over chunks of
+// at most 1024 keys, eight to a CU, so that some load while others reduce, and a rule as the
+// decode step's (decode_chunk): as many chunks as fill whole rounds of what the GPU holds at
+// once.  us per step (bf16, head_dim 64: 128 slices of 16384 keys; 16 and 256 of 131072), each with
+// its best unroll: 1024 threads and 2048 keys 45, 45, 531; 512 and 2048 40, 41, 489; 256 and 1024
+// 40, 42, 491; 128 and 512 41, 46, 512; 256 and 512 43, 50, 540.  256 x 1024 leads in the other widths.
+constexpr int kOneThreads = 1024;
+constexpr int kOneWaves = kOneThreads / 64;
+constexpr int kQThreads = 256;
 constexpr int kQWaves = kQThreads / 64;
+constexpr int64_t kQResident = 2048;
+constexpr int64_t kQMaxChunk = 1024;
+constexpr int64_t kQMinChunk = 256;
 
-// E elements a lane, so that D / E neighbouring lanes hold a row
-template <int D, int E> struct QLayout {
+__host__ __device__ inline int64_t fp4_target_chunks(int64_t n, int64_t length) {
+  const int64_t base = (length + kQMaxChunk - 1) / kQMaxChunk;
+  const int64_t rounds = (n * base + kQResident - 1) / kQResident;
+  const int64_t target = rounds * kQResident / n;
+  return target < base ? base : target;
+}
+__host__ __device__ inline int64_t fp4_chunk(int64_t n, int64_t length) {
+  if (length < 1 || n < 1) return kQMinChunk;
+  const int64_t target = fp4_target_chunks(n, length);
+  const int64_t chunk = (length + target - 1) / target;
+  return chunk < kQMinChunk ? kQMinChunk : chunk;
+}
+// Chunks per slice in the grid and the scratch (as decode_chunks: device_length for every live
+// length up to `length`).
+inline int64_t fp4_chunks(int64_t n, int64_t length, bool device_length) {
+  if (length < 1) return 1;
+  if (!device_length) {
+    const int64_t chunk = fp4_chunk(n, length);
+    return (length + chunk - 1) / chunk;
+  }
+  const int64_t per_min = (length + kQMinChunk - 1) / kQMinChunk;
+  const int64_t target = fp4_target_chunks(n < 1 ? 1 : n, length);
+  return per_min < target ? per_min : target;
+}
+
+// E elements a lane, so that D / E neighbouring lanes hold a row; W waves
+template <int D, int E, int W> struct QLayout {
   static constexpr int kLanesPerRow = D / E;
   static constexpr int kRowsPerWave = 64 / kLanesPerRow;
-  static constexpr int kRowsPerBlock = kRowsPerWave * kQWaves;
+  static constexpr int kRowsPerBlock = kRowsPerWave * W;
   static constexpr int kWords = E / 8;
 };
-template <int D> constexpr int kQElems = D < 32 ? D : 32;
+// K: a block of elements a lane.  V: half of one, which leaves the registers (one sum an
+// element) for eight workgroups of a CU; at head_dim 256 the LDS admits four, and whole blocks
+// are quicker (64 slices of 32768 keys 131 -> 119 us; at 64 the other way, 496 -> 490).
+template <int D> constexpr int kVElems = D == 256 ? 32 : 16;
 
 template <int W> struct CodeWords {
   uint32_t w[W];
@@ -52,92 +93,224 @@ __device__ __forceinline__ CodeWords<W> load_codes(const uint8_t* p) {
   return r;
 }
 
-// The workgroup's walk over `count` rows of codes from `base` on (this lane's part of row 0),
-// U rows a lane in flight; rows past the end are read as the last one.
-template <int D, int E>
+// The workgroup's walk over `count` rows of codes from `base` on, U rows a lane in flight; rows
+// past the end are read as the last one.  A walk of three and more such blocks keeps the next one
+// in flight behind the one at hand (one workgroup a slice, 8000 keys: 24 -> 21 us; below, the
+// copies cost 0.3 us).
+template <int D, int E, int W>
 struct CodeStream {
-  using L = QLayout<D, E>;
-  static constexpr int U = 4, kRows = L::kRowsPerBlock;
-  const uint8_t* src;
+  using L = QLayout<D, E, W>;
+  static constexpr int U = 4, kRows = L::kRowsPerBlock, kStep = U * kRows;
+  const uint8_t* base;
   int first, count;
+  uint32_t part;                                          // this lane's bytes of a row
   CodeWords<L::kWords> r[U];
-  __device__ __forceinline__ CodeStream(const uint8_t* base, int wave, int lane, int n)
-      : src(base), first(wave * L::kRowsPerWave + lane / L::kLanesPerRow), count(n) {}
+  __device__ __forceinline__ CodeStream(const uint8_t* b, int wave, int lane, int n)
+      : base(b), first(wave * L::kRowsPerWave + lane / L::kLanesPerRow), count(n), part(lane % L::kLanesPerRow * (E / 2)) {}
   __device__ __forceinline__ void at(int jb) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) r[u] = load_codes<L::kWords>(src + static_cast<int64_t>(min(jb + u * kRows, count - 1)) * (D / 2));
+    for (int u = 0; u < U; ++u)
+      r[u] = load_codes<L::kWords>(base + (static_cast<uint32_t>(min(jb + u * kRows, count - 1)) * (D / 2) + part));
   }
   __device__ __forceinline__ void load() {
     if (count > 0) at(first);
   }
   template <typename F>
-  __device__ __forceinline__ void walk(F&& f) {
-    for (int jb = first; jb < count; jb += U * kRows) {
-      if (jb != first) at(jb);
+  __device__ __forceinline__ void each(int jb, const CodeWords<L::kWords> (&c)[U], F&& f) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = jb + u * kRows;
-        if (j < count) f(j, r[u]);
+    for (int u = 0; u < U; ++u) {
+      const int j = jb + u * kRows;
+      if (j < count) f(j, c[u]);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void walk(F&& f) {
+    if (count <= 2 * kStep) {
+      for (int jb = first; jb < count; jb += kStep) {
+        if (jb != first) at(jb);
+        each(jb, r, f);
+      }
+      return;
+    }
+    for (int jb = first; jb < count; jb += kStep) {
+      CodeWords<L::kWords> c[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) c[u] = r[u];
+      if (jb + kStep < count) at(jb + kStep);
+      each(jb, c, f);
+    }
+  }
+};
+
+// The scores of 64 keys by one wave, on v_mfma_scale_f32_16x16x128_f8f6f4: B holds 16 keys a
+// column each (codes and scales as they lie in the cache), A the query.
+//
+// A query element is a sum of digits: part i is the nearest whole multiple, -16 to 16, of
+// 2^(E - 3 - 5 i) to what the parts before leave, E the exponent of the largest of its 32 elements.
+// fp8 (e4m3) holds these numbers, the powers are A's scales.  Within a block the unit adds
+// products only down to 2^-13 of the largest one (measured; whole blocks and C in fp32), which
+// whole numbers up to 16 times codes never reach: a block's sum is exact.  8 parts leave less than
+// 2^-39 of the largest element, of bf16 elements next to it nothing after 4 (which would take half
+// of the products: 1% less time at 128 slices of 16384 keys, and errors of 2^-19 of the largest
+// element in the small ones).  The 16 rows of A hold parts 0 to 3 four times over; the second
+// four parts are a product of their own into the same sums.
+//
+// A lane's 16 bytes of codes are one block of one key; the 4 blocks of K = 128 (lane group
+// kb = lane / 16 holds block kb of B and both operands' scales of it) are rows of 4, 2 or 1 keys.
+// fp8 operands lie otherwise: lane group g holds elements 16 (g % 2) to 16 (g % 2) + 15 of blocks
+// g / 2 and 2 + g / 2.  For D <= 64 the rows of A are 0 in the blocks of keys that are not theirs, so
+// that lane group g of the result (rows 4 g to 4 g + 3) gets the keys of its own set.  For
+// D >= 128 each 16 keys have sums of their own and the lane group picks its.  So lane l ends with
+// the score of key l.
+typedef int intx8 __attribute__((ext_vector_type(8)));
+
+template <int D> struct KeyTiles {
+  static constexpr int kBlocks = Fp4Row<D>::kBlocks;
+  static constexpr int kMma = kBlocks;                    // instructions for 64 keys
+  static constexpr int kSets = kBlocks >= 4 ? 1 : 4 / kBlocks;        // of 16 keys in one instruction
+  static constexpr int kHalves = kBlocks >= 4 ? kBlocks / 4 : 1;      // instructions of a row
+  static constexpr int kWords = D < 32 ? 2 : 4;
+  // block kb of K = 128 of instruction m: a key of the 64 (for column c), and a block of its row
+  __device__ static __forceinline__ int key(int m, int kb, int c) {
+    if constexpr (kSets == 1) return 16 * (m / kHalves) + c;
+    else return 16 * (kSets * m + kb * kSets / 4) + c;
+  }
+  __device__ static __forceinline__ int block(int m, int kb) {
+    if constexpr (kSets == 1) return 4 * (m % kHalves) + kb;
+    else return kb % kBlocks;
+  }
+};
+
+constexpr int kParts = 8;
+template <int D> struct QueryShared {
+  uint8_t part[kParts][D];
+  int exponent[Fp4Row<D>::kBlocks];
+};
+
+__device__ __forceinline__ int part_exponent(int e, int i) { return e - 3 - 5 * i; }
+
+// Element t of the query (0 past the row): loaded ahead of the keys, so that its parts do not
+// wait for them (loads complete in issue order).
+template <int D>
+__device__ __forceinline__ float query_element(const void* q1, int64_t idx, int qdt, int t) {
+  if (t >= D) return 0.f;
+  if (qdt == DT_F32) return static_cast<const float*>(q1)[idx + t];
+  const uint16_t x = static_cast<const uint16_t*>(q1)[idx + t];
+  return qdt == DT_BF16 ? bf16_bits_to_f32(x) : f16_bits_to_f32(x);
+}
+
+// The query's parts into LDS, one element a thread (the first D threads); a barrier follows.
+template <int D>
+__device__ __forceinline__ void split_query(float x, QueryShared<D>& sh) {
+  const int t = threadIdx.x;
+  if (t >= D) return;
+  uint32_t top = __float_as_uint(x) & 0x7fffffffu;
+#pragma unroll
+  for (int o = 1; o < Fp4Row<D>::kBlock; o <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
+  // within what fp32 scales by exactly; a query with a NaN or an infinity becomes NaN
+  const int e = min(max(static_cast<int>(top >> 23) - 127, -80), 127);
+  if (t % Fp4Row<D>::kBlock == 0) sh.exponent[t / Fp4Row<D>::kBlock] = e;
+  const bool bad = top >= 0x7f800000u;
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) {
+    const int unit = part_exponent(e, i);
+    const float digit = rintf(x * __uint_as_float(static_cast<uint32_t>(127 - unit) << 23));
+    x = fmaf(-digit, __uint_as_float(static_cast<uint32_t>(127 + unit) << 23), x);
+    sh.part[i][t] = bad ? 0x7f : static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(digit, 0.f, 0, false));
+  }
+}
+
+// A wave's A operands: in registers, but for head_dim 256, whose 32 registers would halve the
+// waves of a CU: there read from LDS at each use.
+template <int D> struct QueryTiles {
+  using T = KeyTiles<D>;
+  static constexpr bool kHeld = T::kHalves == 1;
+  const QueryShared<D>& sh;
+  int lane;
+  intx8 a[kHeld ? kParts / 4 : 1];
+  int scale[kParts / 4][T::kHalves];
+  __device__ __forceinline__ QueryTiles(const QueryShared<D>& s, int l) : sh(s), lane(l) {
+#pragma unroll
+    for (int p = 0; p < kParts / 4; ++p) {
+#pragma unroll
+      for (int h = 0; h < T::kHalves; ++h) scale[p][h] = 127 + part_exponent(sh.exponent[T::block(h, lane >> 4)], (lane & 3) + 4 * p);
+      if constexpr (kHeld) a[p] = read(p, 0);
+    }
+  }
+  __device__ __forceinline__ intx8 read(int p, int h) const {
+    const int set = (lane & 15) >> 2, g = lane >> 4;
+    intx8 x;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const int kb = g / 2 + 2 * (w / 4), at = 16 * (g % 2) + 4 * (w % 4);
+      const bool mine = (T::kSets == 1 || kb * T::kSets / 4 == set % T::kSets) && at < Fp4Row<D>::kBlock;
+      const int y = *reinterpret_cast<const int*>(&sh.part[(lane & 3) + 4 * p][T::block(h, kb) * Fp4Row<D>::kBlock + (mine ? at : 0)]);
+      x[w] = mine ? y : 0;
+    }
+    return x;
+  }
+  __device__ __forceinline__ intx8 operand(int p, int h) const {
+    if constexpr (kHeld) return a[p];
+    else return read(p, h);
+  }
+  // The score of key `lane` of the 64 whose codes and scales these are
+  __device__ __forceinline__ float score(const CodeWords<T::kWords> (&c)[T::kMma], const uint32_t (&s)[T::kMma]) const {
+    constexpr int kOuts = 4 / T::kSets;                   // 16-key groups with sums of their own
+    float out = 0.f;
+#pragma unroll
+    for (int g = 0; g < kOuts; ++g) {
+      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < T::kHalves; ++h) {
+        const int m = g * T::kHalves + h;
+        intx8 b = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < T::kWords; ++w) b[w] = static_cast<int>(c[m].w[w]);
+#pragma unroll
+        for (int p = 0; p < kParts / 4; ++p)
+          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(p, h), b, acc, 0, 4, 0, scale[p][h], 0,
+                                                                 static_cast<int>(s[m]));
+      }
+      const float x = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+      out = g == 0 || (lane >> 4) * kOuts / 4 == g ? x : out;
+    }
+    // every lane's operands count: the products must not move into a branch that some lanes leave
+    asm volatile("" : "+v"(out));
+    return out;
+  }
+};
+
+// A wave's groups of 64 keys: `group`, group + step, ... (keys past the end are read as the last one);
+// f(key, score) once a lane and group.
+template <int D> struct KeyGroups {
+  using T = KeyTiles<D>;
+  // groups in flight: 4 loads of codes a lane.  8 are no quicker, and their registers leave one
+  // workgroup of 1024 threads a CU instead of two (600 slices of 4000 keys 47 us, 40 with 4).
+  static constexpr int U = T::kMma >= 4 ? 1 : 4 / T::kMma;
+  CodeWords<T::kWords> c[U][T::kMma];
+  uint32_t s[U][T::kMma];
+  __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales, int count, int group, int step, int lane) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int m = 0; m < T::kMma; ++m) {
+        const uint32_t j = static_cast<uint32_t>(min(64 * (group + u * step) + T::key(m, lane >> 4, lane & 15), count - 1));
+        const uint32_t b = static_cast<uint32_t>(T::block(m, lane >> 4));
+        c[u][m] = load_codes<T::kWords>(codes + (j * (D / 2) + b * (Fp4Row<D>::kBlock / 2)));
+        s[u][m] = scales[j * T::kBlocks + b];
       }
     }
   }
-};
-
-// A lane's part of the query, and its products with codes
-template <int E, int QT> struct QueryPart {
-  float q[E];
-  __device__ __forceinline__ QueryPart(const void* q1, int64_t idx, int qdt) {
+  template <typename F>
+  __device__ __forceinline__ void each(const QueryTiles<D>& q, int count, int group, int step, int lane, F&& f) {
 #pragma unroll
-    for (int e = 0; e < E; e += 8) {
-      float x[8];
-      load8_f32(q1, idx + e, qdt, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[e + i] = x[i];
+    for (int u = 0; u < U; ++u) {
+      const int j = 64 * (group + u * step);
+      if (j < count) f(j + lane, q.score(c[u], s[u]));
     }
-  }
-  __device__ __forceinline__ float dot(const CodeWords<E / 8>& c) const {
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < E / 8; ++w) {
-      float v[8];
-      fp4_values8(c.w[w], v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s = fmaf(q[8 * w + i], v[i], s);
-    }
-    return s;
-  }
-};
-template <int E> struct QueryPart<E, DT_BF16> {
-  bf16x2 q[E / 2];
-  __device__ __forceinline__ QueryPart(const void* q1, int64_t idx, int) {
-#pragma unroll
-    for (int e = 0; e < E / 8; ++e) {
-      const bf16x8 x = *reinterpret_cast<const bf16x8*>(static_cast<const __bf16*>(q1) + idx + 8 * e);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) q[4 * e + i] = bf16x2{x[2 * i], x[2 * i + 1]};
-    }
-  }
-  __device__ __forceinline__ float dot(const CodeWords<E / 8>& c) const {
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < E / 8; ++w) {
-      s = __builtin_amdgcn_fdot2_f32_bf16(q[4 * w], __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.w[w], 1.f, 0), s, false);
-      s = __builtin_amdgcn_fdot2_f32_bf16(q[4 * w + 1], __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.w[w], 1.f, 1), s, false);
-      s = __builtin_amdgcn_fdot2_f32_bf16(q[4 * w + 2], __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.w[w], 1.f, 2), s, false);
-      s = __builtin_amdgcn_fdot2_f32_bf16(q[4 * w + 3], __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.w[w], 1.f, 3), s, false);
-    }
-    return s;
   }
 };
 
-// A key's block sums under its scales, in block order
-template <int N>
-__device__ __forceinline__ float scaled_sum(const float* part, typename ScaleWord<N>::type s) {
-  float a = 0.f;
-#pragma unroll
-  for (int b = 0; b < N; ++b) a = fmaf(part[b], fp4_factor(static_cast<uint32_t>(s >> (8 * b)) & 255u), a);
-  return a;
-}
 // A key's share for each block of its V row
 template <int N>
 __device__ __forceinline__ void scaled_shares(float* dst, float share, typename ScaleWord<N>::type s) {
@@ -193,11 +366,11 @@ constexpr int scattered(int n, int o) {
 // The workgroup's sums of share v, one row of D for each wave
 template <int D, int E>
 __device__ __forceinline__ void wave_sums(float (&acc)[E], int lane, float* row) {
-  using L = QLayout<D, E>;
-  int at = (lane % L::kLanesPerRow) * E;
-  scatter_sums<E, L::kLanesPerRow>(acc, lane, at);
+  constexpr int kLanesPerRow = D / E;
+  int at = lane % kLanesPerRow * E;
+  scatter_sums<E, kLanesPerRow>(acc, lane, at);
 #pragma unroll
-  for (int i = 0; i < scattered(E, L::kLanesPerRow); ++i) row[at + i] = acc[i];   // lanes with the same `at` hold the same sums
+  for (int i = 0; i < scattered(E, kLanesPerRow); ++i) row[at + i] = acc[i];   // lanes with the same `at` hold the same sums
 }
 
 // The new token's rows into position `pos`: 32 lanes of the first wave each for K and V
@@ -229,73 +402,96 @@ __device__ __forceinline__ const typename ScaleWord<Fp4Row<D>::kBlocks>::type* s
 }
 
 // A slice's whole step in one workgroup; s: floats of LDS, one for each key and block.
-template <int D, int QT>
+template <int D>
 __device__ __forceinline__ void fp4_one_slice(const Fp4DecodeArgs& A, int64_t slice, int live, float qscale, float* s) {
-  constexpr int E = kQElems<D>, N = Fp4Row<D>::kBlocks;
-  using L = QLayout<D, E>;
-  __shared__ float sm[kQWaves], ss[kQWaves];
-  __shared__ float red[kQWaves][D + 1];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, sub = lane % L::kLanesPerRow;
+  constexpr int EV = 16, N = Fp4Row<D>::kBlocks;
+  __shared__ QueryShared<D> qs;
+  __shared__ float sm[kOneWaves], ss[kOneWaves];
+  __shared__ float red[kOneWaves][D + 1];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int64_t row0 = slice * A.capacity;
   float* crow = A.committed + row0;
   if (A.k1 != nullptr && live > 0) {
     append_rows<D>(A, slice, live - 1);
     __syncthreads();
   }
-  const QueryPart<E, QT> q(A.q1, slice * D + sub * E, A.q_dtype);
-  {
-    CodeStream<D, E> k(code_rows<D>(A.k_cache, row0) + sub * (E / 2), wave, lane, live);
-    k.load();
-    k.walk([&](int j, const CodeWords<E / 8>& c) { s[j * N + sub] = q.dot(c); });
-  }
-  CodeStream<D, E> v(code_rows<D>(A.v_cache, row0) + sub * (E / 2), wave, lane, live);
-  v.load();                                             // in flight over the reductions
-  const auto* ks = scale_rows<D>(A.k_cache, row0);
+  // group i of a wave is keys t, t + 1024, ... of its threads: what a thread leaves in s it reads back
+  const uint8_t* kc = code_rows<D>(A.k_cache, row0);
+  const uint8_t* ks = static_cast<const uint8_t*>(A.k_cache.scales) + row0 * N;
+  const float qx = query_element<D>(A.q1, slice * D, A.q_dtype, t);
+  KeyGroups<D> keys;
   const auto* vs = scale_rows<D>(A.v_cache, row0);
+  // the demand and the V scales of this thread's first keys, in flight over the scores
+  constexpr int kAhead = 2;
+  float c0[kAhead] = {};
+  typename ScaleWord<N>::type v0[kAhead] = {};
+  if (live > 0) {
+    keys.load(kc, ks, live, wave, kOneWaves, lane);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int j = min(t + u * kOneThreads, live - 1);
+      c0[u] = __builtin_nontemporal_load(crow + j);
+      v0[u] = vs[j];
+    }
+  }
+  split_query<D>(qx, qs);
   __syncthreads();
   float m = -INFINITY;
-  for (int j = t; j < live; j += kQThreads) {
-    const float a = qscale * scaled_sum<N>(s + j * N, ks[j]);
-    s[j * N] = a;
-    m = fmaxf(m, a);
+  {
+    const QueryTiles<D> q(qs, lane);
+    for (int g = wave; 64 * g < live; g += KeyGroups<D>::U * kOneWaves) {
+      if (g != wave) keys.load(kc, ks, live, g, kOneWaves, lane);
+      keys.each(q, live, g, kOneWaves, lane, [&](int j, float x) {
+        if (j >= live) return;
+        const float a = qscale * x;
+        s[j * N] = a;
+        m = fmaxf(m, a);
+      });
+    }
   }
+  CodeStream<D, EV, kOneWaves> v(code_rows<D>(A.v_cache, row0), wave, lane, live);
+  v.load();                                             // in flight over the reductions
   const float wm = wave_max(m);
   if (lane == 0) sm[wave] = wm;
   __syncthreads();
   float M = sm[0];
 #pragma unroll
-  for (int w = 1; w < kQWaves; ++w) M = fmaxf(M, sm[w]);
+  for (int w = 1; w < kOneWaves; ++w) M = fmaxf(M, sm[w]);
   float l = 0.f;
-  for (int j = t; j < live; j += kQThreads) l += fast_exp2(s[j * N] - M);
+  for (int j = t; j < live; j += kOneThreads) l += fast_exp2(s[j * N] - M);
   l = wave_sum(l);
   if (lane == 0) ss[wave] = l;
   __syncthreads();
   float tot = 0.f;
 #pragma unroll
-  for (int w = 0; w < kQWaves; ++w) tot += ss[w];
+  for (int w = 0; w < kOneWaves; ++w) tot += ss[w];
   const float lse = M + __log2f(tot);
   float ssum = 0.f;
-  for (int j = t; j < live; j += kQThreads) {
+  auto take = [&](int j, float cm, typename ScaleWord<N>::type scale) {
     const float p = fast_exp2(s[j * N] - lse);
-    const float cm = crow[j];
     const float sh = p * fast_rcp(cm + p + kEps);
-    crow[j] = cm + p;
-    scaled_shares<N>(s + j * N, sh, vs[j]);
+    __builtin_nontemporal_store(cm + p, crow + j);
+    scaled_shares<N>(s + j * N, sh, scale);
     ssum += sh;
-  }
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u)
+    if (t + u * kOneThreads < live) take(t + u * kOneThreads, c0[u], v0[u]);
+  for (int j = t + kAhead * kOneThreads; j < live; j += kOneThreads) take(j, __builtin_nontemporal_load(crow + j), vs[j]);
   ssum = wave_sum(ssum);
   if (lane == 0) red[wave][D] = ssum;
   __syncthreads();
-  float acc[E];
+  const int vb = lane % (D / EV) * EV / Fp4Row<D>::kBlock;
+  float acc[EV];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  v.walk([&](int j, const CodeWords<E / 8>& c) { add_codes<E>(acc, s[j * N + sub], c); });
-  wave_sums<D, E>(acc, lane, red[wave]);
+  for (int e = 0; e < EV; ++e) acc[e] = 0.f;
+  v.walk([&](int j, const CodeWords<EV / 8>& c) { add_codes<EV>(acc, s[j * N + vb], c); });
+  wave_sums<D, EV>(acc, lane, red[wave]);
   __syncthreads();
   if (t < D) {
     float x = 0.f, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kQWaves; ++w) {
+    for (int w = 0; w < kOneWaves; ++w) {
       x += red[w][t];
       sum += red[w][D];
     }
@@ -303,33 +499,23 @@ __device__ __forceinline__ void fp4_one_slice(const Fp4DecodeArgs& A, int64_t sl
   }
 }
 
-template <int D, int QT>
-__global__ __launch_bounds__(kQThreads) void fp4_one(Fp4DecodeArgs A, float qscale, int64_t slice0) {
+template <int D>
+__global__ __launch_bounds__(kOneThreads, D <= 128 ? 8 : 4) void fp4_one(Fp4DecodeArgs A, float qscale, int64_t slice0) {
   extern __shared__ float one_s[];
-  fp4_one_slice<D, QT>(A, slice0 + blockIdx.x, static_cast<int>(live_length(A.dlen, A.length)), qscale, one_s);
+  fp4_one_slice<D>(A, slice0 + blockIdx.x, static_cast<int>(live_length(A.dlen, A.length)), qscale, one_s);
 }
 
-// ONE: a device-resident length that may be short: one workgroup a slice then does the whole
-// step, as in dec_stats.
-template <int D, int QT, bool ONE>
+template <int D>
 __global__ __launch_bounds__(kQThreads) void fp4_stats(Fp4DecodeArgs A, float* __restrict__ aff, float2* __restrict__ part,
                                                        int64_t chunk, int nchunk, float qscale, int64_t slice0,
                                                        int64_t one_max) {
-  constexpr int E = kQElems<D>, N = Fp4Row<D>::kBlocks;
-  using L = QLayout<D, E>;
+  constexpr int N = Fp4Row<D>::kBlocks;
   const int64_t live = live_length(A.dlen, A.length);
-  if constexpr (ONE) {
-    extern __shared__ float one_s[];
-    if (live <= one_max) {
-      const unsigned block = blockIdx.y * gridDim.x + blockIdx.x;
-      if (block < gridDim.y) fp4_one_slice<D, QT>(A, slice0 + block, static_cast<int>(live), qscale, one_s);
-      return;
-    }
-  }
+  if (live <= one_max) return;                            // fp4_finish does the whole step
   const int64_t slice = slice0 + blockIdx.y;
   const int c = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % L::kLanesPerRow;
-  if (A.dlen != nullptr) chunk = decode_chunk(A.n, live);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (A.dlen != nullptr) chunk = fp4_chunk(A.n, live);
   const int nlive = live_chunks(live, chunk);
   if (c >= nlive) return;
   const int64_t j0 = c * chunk, row0 = slice * A.capacity + j0;
@@ -338,25 +524,31 @@ __global__ __launch_bounds__(kQThreads) void fp4_stats(Fp4DecodeArgs A, float* _
     append_rows<D>(A, slice, live - 1);
     __syncthreads();
   }
-  CodeStream<D, E> k(code_rows<D>(A.k_cache, row0) + sub * (E / 2), wave, lane, count);
-  k.load();
-  const QueryPart<E, QT> q(A.q1, slice * D + sub * E, A.q_dtype);
-  __shared__ float s[kDecMaxChunk * N];
-  k.walk([&](int j, const CodeWords<E / 8>& w) { s[j * N + sub] = q.dot(w); });
-  const auto* ks = scale_rows<D>(A.k_cache, row0);
+  const uint8_t* kc = code_rows<D>(A.k_cache, row0);
+  const uint8_t* ks = static_cast<const uint8_t*>(A.k_cache.scales) + row0 * N;
+  const float qx = query_element<D>(A.q1, slice * D, A.q_dtype, threadIdx.x);
+  KeyGroups<D> keys;
+  keys.load(kc, ks, count, wave, kQWaves, lane);
+  __shared__ QueryShared<D> qs;
+  split_query<D>(qx, qs);
   __syncthreads();
+  const QueryTiles<D> q(qs, lane);
   float* arow = aff + slice * A.length + j0;
   float m = -INFINITY, l = 0.f;
   bool bad = false;
-  for (int j = threadIdx.x; j < count; j += kQThreads) {
-    const float a = qscale * scaled_sum<N>(s + j * N, ks[j]);
-    arow[j] = a;
-    bad |= a != a;
-    const float mn = fmaxf(m, a);
-    if (mn > -INFINITY) {
-      l = l * fast_exp2(m - mn) + fast_exp2(a - mn);
-      m = mn;
-    }
+  for (int g = wave; 64 * g < count; g += KeyGroups<D>::U * kQWaves) {
+    if (g != wave) keys.load(kc, ks, count, g, kQWaves, lane);
+    keys.each(q, count, g, kQWaves, lane, [&](int j, float x) {
+      if (j >= count) return;
+      const float a = qscale * x;
+      arow[j] = a;
+      bad |= a != a;
+      const float mn = fmaxf(m, a);
+      if (mn > -INFINITY) {
+        l = l * fast_exp2(m - mn) + fast_exp2(a - mn);
+        m = mn;
+      }
+    });
   }
   const float wm = wave_max(m);
   float ws = wave_sum(bad ? NAN : m == -INFINITY ? 0.f : l * fast_exp2(m - wm));
@@ -376,14 +568,13 @@ template <int D>
 __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const float* __restrict__ aff,
                                                        const float2* __restrict__ part, float* __restrict__ part_out,
                                                        int64_t chunk, int nchunk, int64_t slice0, int64_t one_max) {
-  constexpr int E = kQElems<D>, N = Fp4Row<D>::kBlocks;
-  using L = QLayout<D, E>;
+  constexpr int E = kVElems<D>, N = Fp4Row<D>::kBlocks;
   const int64_t live = live_length(A.dlen, A.length);
-  if (live <= one_max) return;                            // fp4_stats did the whole step
+  if (live <= one_max) return;                            // fp4_finish does the whole step
   const int64_t slice = slice0 + blockIdx.y;
   const int c = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % L::kLanesPerRow;
-  if (A.dlen != nullptr) chunk = decode_chunk(A.n, live);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (A.dlen != nullptr) chunk = fp4_chunk(A.n, live);
   const int nlive = live_chunks(live, chunk);
   if (c >= nlive) return;
   const int64_t j0 = c * chunk, row0 = slice * A.capacity + j0;
@@ -391,23 +582,27 @@ __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const fl
   const float* arow = aff + slice * A.length + j0;
   float* crow = A.committed + row0;
   const auto* vs = scale_rows<D>(A.v_cache, row0);
-  CodeStream<D, E> v(code_rows<D>(A.v_cache, row0) + sub * (E / 2), wave, lane, count);
-  v.load();
-  // this thread's keys, which do not wait for the statistics
-  constexpr int kOwn = static_cast<int>(kDecMaxChunk / kQThreads);
+  // what comes first is loaded first (loads complete in issue order): the chunks' statistics, then
+  // this thread's keys, then V rows.  The demand goes past the caches,
+  // both ways, and leaves them to the affinities: 256 slices of 131072 keys 487 -> 445 us.
+  const float2* prow = part + slice * nchunk;
+  const float2 first = prow[min(lane, nlive - 1)];
+  constexpr int kOwn = static_cast<int>(kQMaxChunk / kQThreads);
   float av[kOwn], cv[kOwn];
   typename ScaleWord<N>::type sv[kOwn];
 #pragma unroll
   for (int u = 0; u < kOwn; ++u) {
     const int j = min(static_cast<int>(threadIdx.x) + u * kQThreads, count - 1);
     av[u] = arow[j];
-    cv[u] = crow[j];
+    cv[u] = __builtin_nontemporal_load(crow + j);
     sv[u] = vs[j];
   }
+  CodeStream<D, E, kQWaves> v(code_rows<D>(A.v_cache, row0), wave, lane, count);
+  v.load();
   // the slice's statistics from its chunks' (every wave by itself)
   float m = -INFINITY, l = 0.f;
   for (int i = lane; i < nlive; i += 64) {
-    const float2 ps = part[slice * nchunk + i];
+    const float2 ps = i == lane ? first : prow[i];
     const float mn = fmaxf(m, ps.x);
     l = (m > -INFINITY ? l * fast_exp2(m - mn) : l) + (ps.x > -INFINITY ? ps.y * fast_exp2(ps.x - mn) : ps.y);
     m = mn;
@@ -416,7 +611,7 @@ __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const fl
   const float gs = wave_sum(m > -INFINITY ? l * fast_exp2(m - gm) : l);
   const float lse = gm + __log2f(gs);
 
-  __shared__ float s[kDecMaxChunk * N];
+  __shared__ float s[kQMaxChunk * N];
   __shared__ float red[kQWaves][D + 1];
   float ssum = 0.f;
 #pragma unroll
@@ -425,17 +620,18 @@ __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const fl
     if (j >= count) break;
     const float p = fast_exp2(av[u] - lse);
     const float sh = p * fast_rcp(cv[u] + p + kEps);
-    crow[j] = cv[u] + p;
+    __builtin_nontemporal_store(cv[u] + p, crow + j);
     scaled_shares<N>(s + j * N, sh, sv[u]);
     ssum += sh;
   }
   ssum = wave_sum(ssum);
   if (lane == 0) red[wave][D] = ssum;
   __syncthreads();
+  const int vb = lane % (D / E) * E / Fp4Row<D>::kBlock;
   float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  v.walk([&](int j, const CodeWords<E / 8>& w) { add_codes<E>(acc, s[j * N + sub], w); });
+  v.walk([&](int j, const CodeWords<E / 8>& w) { add_codes<E>(acc, s[j * N + vb], w); });
   wave_sums<D, E>(acc, lane, red[wave]);
   __syncthreads();
   for (int i = threadIdx.x; i <= D; i += kQThreads) {
@@ -445,13 +641,81 @@ __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const fl
   }
 }
 
-// The most keys of a slice that one workgroup takes whole: an LDS float for each key and block.
+// One workgroup per slice: the chunks' columns (D of share v, one of the shares) summed by kGroups
+// threads each, every kGroups-th chunk a thread and four in flight, then over the groups; always in the
+// same order.  ONE: a device-resident length that may be short: then the whole step is done here,
+// and the launches before had nothing to do.
+template <int D, bool ONE>
+__global__ __launch_bounds__(ONE ? kOneThreads : 512, ONE && D <= 128 ? 8 : 4) void fp4_finish(Fp4DecodeArgs A, const float* __restrict__ part_out,
+                                                                      int64_t chunk, int nchunk, float qscale,
+                                                                      int64_t slice0, int64_t one_max) {
+  constexpr int kThreads = ONE ? kOneThreads : 512;
+  constexpr int kCols = D + 1, kGroups = 512 / kCols < 16 ? 512 / kCols : 16;
+  const int64_t slice = slice0 + blockIdx.x, live = live_length(A.dlen, A.length);
+  if constexpr (ONE) {
+    extern __shared__ float one_s[];
+    if (live <= one_max) {
+      fp4_one_slice<D>(A, slice, static_cast<int>(live), qscale, one_s);
+      return;
+    }
+  }
+  __shared__ float sum[kGroups][kCols];
+  if (A.dlen != nullptr) chunk = fp4_chunk(A.n, live);
+  const int nlive = live_chunks(live, chunk);
+  for (int e = threadIdx.x; e < kGroups * kCols; e += kThreads) {
+    const int g = e / kCols;
+    const float* p = part_out + slice * nchunk * kCols + e % kCols;
+    float x = 0.f;
+    int i = g;
+    for (; i + 3 * kGroups < nlive; i += 4 * kGroups) {
+      float y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y[u] = p[static_cast<int64_t>(i + u * kGroups) * kCols];
+      x += (y[0] + y[1]) + (y[2] + y[3]);
+    }
+    for (; i < nlive; i += kGroups) x += p[static_cast<int64_t>(i) * kCols];
+    sum[g][e % kCols] = x;
+  }
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float x = 0.f, shares = 0.f;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      x += sum[g][threadIdx.x];
+      shares += sum[g][D];
+    }
+    store_as(A.out, slice * D + threadIdx.x, A.q_dtype, x / (shares + kEps));
+  }
+}
+
+// The most keys of a slice that one workgroup takes whole; above, the chunked step, whose three
+// launches take 10 us at least and whose many workgroups catch up where few slices leave CUs idle.
+// us per step, one workgroup -> chunked (bf16 queries):
+//   64:  1 slice 2000 keys 8.5 -> 10.3, 4000 12.6 -> 10.9; 16 slices 2000 9.4 -> 11.3, 4000 13.3 -> 11.6;
+//        64 slices 4000 13.7 -> 15.7, 8000 22.9 -> 19.8; 128 slices 8100 24.6 -> 26.9, 12000 33 -> 32;
+//        160 slices 8100 26 -> 29, 16000 44 -> 46; 256 slices 2000 12 -> 20, 16000 58 -> 69;
+//        264 slices 8100 42.8 -> 42.7, 10000 60 -> 48; 300 slices 8100 43 -> 45; 400 slices 8100 48 -> 57,
+//        12000 74 -> 75; 600 slices 8100 71 -> 78, 12000 110 -> 104; 1024 slices 16000 207 -> 234
+//   128: 16 slices 1000 9.0 -> 12.3, 2000 12.3 -> 12.6; 64 slices 2000 12.7 -> 14.7, 4000 21 -> 18;
+//        128 slices 4000 22 -> 24, 6000 30 -> 31; 256 slices 8000 52 -> 62; 264 slices 4000 39 -> 39,
+//        6000 64 -> 52; 400 slices 4000 46 -> 50
+//   256: 16 slices 500 11 -> 14, 1000 17 -> 14; 128 slices 1000 18 -> 19, 2000 30 -> 25; 256 slices 4000
+//        56 -> 66; 264 slices 2000 52 -> 43; 400 slices 500 23 -> 24; 512 slices 2000 60 -> 66
+//   16:  16 slices 4000 8.3 -> 10.9, 8000 12.4 -> 12.2; 128 slices 16000 23.5 -> 23, 32000 41 -> 35
 template <int D>
 int64_t fp4_one_max(int64_t n) {
-  constexpr int64_t kKeyBytes = D + 2 * Fp4Row<D>::kBlocks + 8, kMost = 16384 / Fp4Row<D>::kBlocks;
-  if (n >= 160) return kMost;
-  const int64_t keys = ((272 + 3 * n) << 10) / kKeyBytes;
-  return keys < 4096 ? (keys < kMost ? keys : kMost) : (4096 < kMost ? 4096 : kMost);
+  constexpr int64_t kKeyBytes = D + 2 * Fp4Row<D>::kBlocks + 8;
+  constexpr int64_t kMost = 32768 / Fp4Row<D>::kBlocks;               // 128 KB of LDS: one float a key and block
+  if (n < 144) {
+    const int64_t keys = (D == 256 ? (420 + n) << 9 : (210 + 4 * n) << 10) / kKeyBytes;
+    return std::min({keys, kMost, int64_t{16384}});
+  }
+  if (n <= 256) return kMost;
+  // more slices than CUs: up to 64 KB (and but for head_dim 256, by its registers) two of them share a
+  // CU; else rounds of 256, worth it where the last one is filled
+  const int64_t places = (n + 255) / 256 * 256;
+  if (16 * n >= 13 * places) return kMost;
+  return D == 256 ? 512 : kMost / 2;
 }
 
 struct Fp4Scratch {
@@ -463,49 +727,44 @@ struct Fp4Scratch {
   }
 };
 
-template <int D, int QT>
+template <int D>
 int launch_fp4(const Fp4DecodeArgs& a) {
-  const int64_t chunk = decode_chunk(a.n, a.length);
-  const int nchunk = static_cast<int>(decode_chunks(a.n, a.length, a.dlen != nullptr));
+  const int64_t chunk = fp4_chunk(a.n, a.length);
+  const int nchunk = static_cast<int>(fp4_chunks(a.n, a.length, a.dlen != nullptr));
   const float qscale = kLog2e / sqrtf(static_cast<float>(D));
-  constexpr int N = Fp4Row<D>::kBlocks;
   hipStream_t st = static_cast<hipStream_t>(a.stream);
   const int64_t keys = fp4_one_max<D>(a.n);
-  const auto lds_of = [](int64_t k) { return sizeof(float) * static_cast<size_t>((k + 63) / 64 * 64 * N); };
+  const auto lds_of = [](int64_t k) { return sizeof(float) * static_cast<size_t>((k + 63) / 64 * 64 * Fp4Row<D>::kBlocks); };
   if (a.length <= keys) {
     slice_batches(a.n, [&](int64_t s0, unsigned ns) {
-      DIL_TIMED("fp4_one", st, (fp4_one<D, QT><<<dim3(ns), kQThreads, lds_of(a.length), st>>>(a, qscale, s0)));
+      DIL_TIMED("fp4_one", st, (fp4_one<D><<<dim3(ns), kOneThreads, lds_of(a.length), st>>>(a, qscale, s0)));
     });
     return static_cast<int>(hipGetLastError());
   }
-  const int64_t one_max = a.dlen != nullptr ? keys : -1;
+  const int64_t one_max = a.dlen != nullptr ? keys : -1;  // a device-resident length may be short
   const Fp4Scratch w(a.n, a.length, D, nchunk);
   char* ws = static_cast<char*>(a.workspace);
   float* aff = reinterpret_cast<float*>(ws);
   float2* part = reinterpret_cast<float2*>(ws + w.part);
   float* part_out = reinterpret_cast<float*>(ws + w.part_out);
   slice_batches(a.n, [&](int64_t s0, unsigned ns) {
-    const dim3 grid(nchunk, ns);
-    if (one_max >= 0)
-      DIL_TIMED("fp4_stats", st,
-                (fp4_stats<D, QT, true><<<grid, kQThreads, lds_of(one_max), st>>>(a, aff, part, chunk, nchunk, qscale, s0, one_max)));
-    else
-      DIL_TIMED("fp4_stats", st,
-                (fp4_stats<D, QT, false><<<grid, kQThreads, 0, st>>>(a, aff, part, chunk, nchunk, qscale, s0, one_max)));
+    DIL_TIMED("fp4_stats", st,
+              (fp4_stats<D><<<dim3(nchunk, ns), kQThreads, 0, st>>>(a, aff, part, chunk, nchunk, qscale, s0, one_max)));
   });
   slice_batches(a.n, [&](int64_t s0, unsigned ns) {
     DIL_TIMED("fp4_apply", st,
               (fp4_apply<D><<<dim3(nchunk, ns), kQThreads, 0, st>>>(a, aff, part, part_out, chunk, nchunk, s0, one_max)));
   });
-  DIL_TIMED("fp4_finish", st,
-            (dec_finish<D><<<dim3(static_cast<unsigned>(a.n)), kFinishThreads, 0, st>>>(part_out, nchunk, a.out, D, a.q_dtype,
-                                                                                      a.length, chunk, a.dlen, one_max)));
+  slice_batches(a.n, [&](int64_t s0, unsigned ns) {
+    if (one_max >= 0)
+      DIL_TIMED("fp4_finish", st,
+                (fp4_finish<D, true><<<dim3(ns), kOneThreads, lds_of(one_max), st>>>(a, part_out, chunk, nchunk, qscale, s0,
+                                                                                        one_max)));
+    else
+      DIL_TIMED("fp4_finish", st,
+                (fp4_finish<D, false><<<dim3(ns), 512, 0, st>>>(a, part_out, chunk, nchunk, qscale, s0, one_max)));
+  });
   return static_cast<int>(hipGetLastError());
-}
-
-template <int D>
-int decode_fp4_type(const Fp4DecodeArgs& a) {
-  return a.q_dtype == DT_BF16 ? launch_fp4<D, DT_BF16>(a) : launch_fp4<D, DT_F32>(a);
 }
 
 }  // namespace
@@ -513,16 +772,16 @@ int decode_fp4_type(const Fp4DecodeArgs& a) {
 // Sized for a device-resident length up to `length`, as the decode step's.
 int64_t decode_fp4_workspace_bytes(int64_t n, int64_t length, int head_dim) {
   if (n < 1 || length < 1) return 0;
-  return static_cast<int64_t>(Fp4Scratch(n, length, head_dim, decode_chunks(n, length, true)).total);
+  return static_cast<int64_t>(Fp4Scratch(n, length, head_dim, fp4_chunks(n, length, true)).total);
 }
 
 int decode_fp4(const Fp4DecodeArgs& a) {
   switch (a.head_dim) {
-    case 16: return decode_fp4_type<16>(a);
-    case 32: return decode_fp4_type<32>(a);
-    case 64: return decode_fp4_type<64>(a);
-    case 128: return decode_fp4_type<128>(a);
-    case 256: return decode_fp4_type<256>(a);
+    case 16: return launch_fp4<16>(a);
+    case 32: return launch_fp4<32>(a);
+    case 64: return launch_fp4<64>(a);
+    case 128: return launch_fp4<128>(a);
+    case 256: return launch_fp4<256>(a);
     default: return kErrHeadDim;
   }
 }
