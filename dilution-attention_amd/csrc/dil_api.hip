@@ -65,7 +65,7 @@ bool valid_fp4(const dil_fp4_cache* c) {
 dil::Fp4Cache fp4_of(const dil_fp4_cache* c) { return dil::Fp4Cache{c->codes, c->scales}; }
 // rows of one call: at least one, and no more than a grid's 2^32 threads take
 bool valid_fp4_range(int64_t rows, int64_t capacity, int head_dim) {
-  return rows >= 1 && capacity < (int64_t{1} << 31) && rows <= capacity && rows * head_dim < (int64_t{1} << 36);
+  return rows >= 1 && capacity < (int64_t{1} << 31) && rows <= capacity && rows * head_dim < (int64_t{1} << 34);
 }
 // slices are counted in 32 bits by the views, and their batch found by one
 // multiplication (RowsView)
@@ -644,10 +644,11 @@ int dil_decode_step_fp4(const void* q1, const void* k1, const void* v1, const di
   if (!valid_dtype(q_dtype)) return dil::kErrDtype;
   if (n < 1 || n >= (int64_t{1} << 31) || length < 1 || length > capacity || capacity >= (int64_t{1} << 31))
     return dil::kErrShape;
-  if (!all_set(q1, static_cast<const void*>(committed), static_cast<const void*>(out), static_cast<const void*>(workspace)) ||
+  const int64_t need = dil::decode_fp4_workspace_bytes(n, length, head_dim);
+  if (!all_set(q1, static_cast<const void*>(committed), static_cast<const void*>(out)) || (need > 0 && workspace == nullptr) ||
       (k1 == nullptr) != (v1 == nullptr) || !aligned16(q1, k1, v1) || !valid_fp4(k_cache) || !valid_fp4(v_cache))
     return dil::kErrShape;
-  if (workspace_bytes < dil::decode_fp4_workspace_bytes(n, length, head_dim)) return dil::kErrWorkspace;
+  if (workspace_bytes < need) return dil::kErrWorkspace;
   return dil::decode_fp4(dil::Fp4DecodeArgs{q1, k1, v1, fp4_of(k_cache), fp4_of(v_cache), committed, out, n, capacity, length,
                                             length_dev, head_dim, q_dtype, workspace, workspace_bytes, stream});
 }

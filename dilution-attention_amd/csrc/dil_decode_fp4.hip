@@ -769,9 +769,16 @@ int launch_fp4(const Fp4DecodeArgs& a) {
 
 }  // namespace
 
-// Sized for a device-resident length up to `length`, as the decode step's.
+// Sized for a device-resident length up to `length`, as the decode step's; nothing where every
+// length up to it takes one workgroup a slice.
 int64_t decode_fp4_workspace_bytes(int64_t n, int64_t length, int head_dim) {
   if (n < 1 || length < 1) return 0;
+  const int64_t one = head_dim == 16    ? fp4_one_max<16>(n)
+                      : head_dim == 32  ? fp4_one_max<32>(n)
+                      : head_dim == 64  ? fp4_one_max<64>(n)
+                      : head_dim == 128 ? fp4_one_max<128>(n)
+                                        : fp4_one_max<256>(n);
+  if (length <= one) return 0;
   return static_cast<int64_t>(Fp4Scratch(n, length, head_dim, fp4_chunks(n, length, true)).total);
 }
 

@@ -666,12 +666,13 @@ at::Tensor decode_step_fp4(const at::Tensor& q1, const at::Tensor& kc, const at:
     throw py::value_error("workspace must be a contiguous uint8 tensor of at least " + std::to_string(need) +
                           " bytes on the caches' device");
   if (n > 0) {
-    const at::Tensor ws = scratch ? *scratch : workspace(need, kc);
+    const Maybe ws = scratch ? scratch : need > 0 ? Maybe(workspace(need, kc)) : Maybe();
     launch("dil_decode_step_fp4", [&]() -> int {
       const dil_fp4_cache ck = fp4_ref(kc, ks), cv = fp4_ref(vc, vs);
       return api.decode_step_fp4(qf.data_ptr(), kf ? kf->data_ptr() : nullptr, vf ? vf->data_ptr() : nullptr, &ck, &cv,
                                  f32(committed), out.data_ptr(), n, s.capacity, length, live, static_cast<int>(d),
-                                 type_code(qt), ws.data_ptr(), ws.numel(), reinterpret_cast<void*>(stream));
+                                 type_code(qt), ws ? ws->data_ptr() : nullptr, ws ? ws->numel() : 0,
+                                 reinterpret_cast<void*>(stream));
     });
   }
   const at::Tensor y = out.view({s.batch, s.heads, 1, d});

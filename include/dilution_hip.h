@@ -44,9 +44,10 @@
  *     Without slices or rows the queries return 0, and the calls refuse the sizes.
  *   - Return value: 0 on success, a positive hipError_t from the launch, or a
  *     negative argument error (see dil_status_string).  A NULL pointer where
- *     an argument is required is an argument error (-4); only `pk` of
- *     dil_forward may be NULL, and `carry` of dil_forward and
- *     dil_prefill_chunk on calls that take the key pass.  Argument errors are
+ *     an argument is required is an argument error (-4); `pk` of
+ *     dil_forward may be NULL, `carry` of dil_forward and
+ *     dil_prefill_chunk on calls that take the key pass, and what an entry point
+ *     says may be.  Argument errors are
  *     returned before any launch.
  */
 #ifndef DILUTION_HIP_H
@@ -463,8 +464,8 @@ int dil_fp4_read(const dil_fp4_cache* k_cache, const dil_fp4_cache* v_cache, int
  * position length - 1 first, or both NULL when they are there.  length_dev not NULL: the
  * length is read from device memory when the kernels run (clamped to [0, length]; with 0
  * nothing is read or written but out, which becomes 0), and `length` sizes grid and workspace.
- * q1, k1 and v1 are 16-byte aligned.  The workspace query serves both forms and, without
- * slices or keys, returns 0.
+ * q1, k1 and v1 are 16-byte aligned.  The workspace query serves both forms; where it returns 0
+ * (short contexts, which one launch does; no slices or keys) workspace may be NULL.
  */
 int64_t dil_decode_fp4_workspace_bytes(int64_t n, int64_t length, int head_dim);
 int dil_decode_step_fp4(const void* q1, const void* k1, const void* v1, const dil_fp4_cache* k_cache,

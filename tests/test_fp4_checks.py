@@ -151,16 +151,17 @@ def test_c_entry_argument_errors():
                 dict(kc=off), dict(kc=none)):
         assert read(**bad) == -4, bad
 
-    need = lib.dil_decode_fp4_workspace_bytes(6, 40, 64)
+    need = lib.dil_decode_fp4_workspace_bytes(6, 40000, 64)
+    assert need > 0 and lib.dil_decode_fp4_workspace_bytes(6, 40, 64) == 0
 
-    def step(q=at[0], k1=None, v1=None, kc=c, vc=c, com=at[1], out=at[2], n=6, cap=40, length=40, d=64, dt=1, ws=at[3],
-             size=need):
+    def step(q=at[0], k1=None, v1=None, kc=c, vc=c, com=at[1], out=at[2], n=6, cap=40000, length=40000, d=64, dt=1,
+             ws=at[3], size=need):
         return lib.dil_decode_step_fp4(q, k1, v1, ctypes.byref(kc), ctypes.byref(vc), com, out, n, cap, length, None, d, dt, ws,
                                        size, None)
 
     assert step(d=20) == -1 and step(dt=7) == -2 and step(size=need - 1) == -3
     for bad in (dict(q=None), dict(k1=at[4]), dict(v1=at[4]), dict(k1=ctypes.c_void_p(4104), v1=at[4]), dict(kc=off), dict(vc=odd),
-                dict(com=None), dict(out=None), dict(n=0), dict(length=0), dict(length=41), dict(cap=1 << 31, length=4),
+                dict(com=None), dict(out=None), dict(n=0), dict(length=0), dict(length=40001), dict(cap=1 << 31, length=4),
                 dict(ws=None), dict(q=ctypes.c_void_p(4098))):
         assert step(**bad) == -4, bad
     for n, length in ((0, 5), (-1, 5), (3, 0), (3, -2)):

@@ -335,9 +335,11 @@ def test_device_length_refusals():
     for out in (torch.empty(1, 2, 64, device="cuda"), torch.empty(1, 2, 32, device="cuda", dtype=q.dtype), torch.empty(1, 2, 64, dtype=q.dtype)):
         with pytest.raises(ValueError, match="out"):
             step(q, kc, vc, com, n, 300, out=out)
-    for ws in (torch.empty(16, dtype=torch.uint8, device="cuda"), kernels.decode_fp4_workspace(1, 2, 300, 64, "cpu")):
+    long = _state(1, 2, 9000, 0, 64, torch.bfloat16, seed=15)        # a length that needs a workspace
+    good = kernels.decode_fp4_workspace(1, 2, 9000, 64, "cuda")
+    for ws in (good[:-1], good.cpu(), good.float(), good.repeat(2)[::2]):
         with pytest.raises(ValueError, match="workspace"):
-            step(q, kc, vc, com, n, 300, workspace=ws)
+            step(*long, n, 9000, workspace=ws)
     with pytest.raises(ValueError, match="start"):
         kernels.dilution_fp4_write(q, q, kc, vc, torch.tensor([5], device="cuda", dtype=torch.int32))
 
