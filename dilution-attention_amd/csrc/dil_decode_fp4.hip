@@ -205,8 +205,12 @@ __device__ __forceinline__ void split_query(float x, QueryShared<D>& sh) {
   const int t = threadIdx.x;
   if (t >= D) return;
   uint32_t top = __float_as_uint(x) & 0x7fffffffu;
-#pragma unroll
-  for (int o = 1; o < Fp4Row<D>::kBlock; o <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o, 64)));
+  auto with = [&](int other) { top = max(top, static_cast<uint32_t>(other)); };
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0xB1, 0xF, 0xF, true));      // quad_perm [1, 0, 3, 2]
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0x4E, 0xF, 0xF, true));      // quad_perm [2, 3, 0, 1]
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0x141, 0xF, 0xF, true));     // row_half_mirror
+  with(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0x140, 0xF, 0xF, true));     // row_mirror
+  if constexpr (Fp4Row<D>::kBlock == 32) with(__shfl_xor(static_cast<int>(top), 16, 64));
   // within what fp32 scales by exactly; a query with a NaN or an infinity becomes NaN
   const int e = min(max(static_cast<int>(top >> 23) - 127, -80), 127);
   if (t % Fp4Row<D>::kBlock == 0) sh.exponent[t / Fp4Row<D>::kBlock] = e;
@@ -330,37 +334,83 @@ __device__ __forceinline__ void add_codes(float (&acc)[E], float w, const CodeWo
   }
 }
 
-// The sums of v over the lanes that differ in the bits O and above: each step halves what a
-// lane holds, so that lane l ends with the sums of its element `at` alone (N - 1 moves and the
-// rest of the 6 - log2 O steps one each, where a sum element by element takes N moves a step).
-template <int N, int O>
+// Lane moves on the vector unit: a wave's reduction by LDS shuffles is six round trips of ~100
+// cycles, and the step has eight of them in a row.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ float dpp(float old, float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(x), CTRL, ROWS, 0xF, false));
+}
+constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143;
+__device__ __forceinline__ float last_lane(float x) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+__device__ __forceinline__ float wave_sum_dpp(float x) {
+  x += dpp<kShr1>(0.f, x);
+  x += dpp<kShr2>(0.f, x);
+  x += dpp<kShr4>(0.f, x);
+  x += dpp<kShr8>(0.f, x);
+  x += dpp<kBcast15, 0xA>(0.f, x);
+  x += dpp<kBcast31, 0xC>(0.f, x);
+  return last_lane(x);
+}
+__device__ __forceinline__ float wave_max_dpp(float x) {
+  constexpr float kNone = -INFINITY;
+  x = fmaxf(x, dpp<kShr1>(kNone, x));
+  x = fmaxf(x, dpp<kShr2>(kNone, x));
+  x = fmaxf(x, dpp<kShr4>(kNone, x));
+  x = fmaxf(x, dpp<kShr8>(kNone, x));
+  x = fmaxf(x, dpp<kBcast15, 0xA>(kNone, x));
+  x = fmaxf(x, dpp<kBcast31, 0xC>(kNone, x));
+  return last_lane(x);
+}
+template <int O> __device__ __forceinline__ float from_xor(float x) {
+  if constexpr (O == 1) return dpp<0xB1>(0.f, x);         // quad_perm [1, 0, 3, 2]
+  else if constexpr (O == 2) return dpp<0x4E>(0.f, x);    // quad_perm [2, 3, 0, 1]
+  else if constexpr (O == 8) return dpp<0x128>(0.f, x);   // row_ror:8
+  else return __shfl_xor(x, O, 64);
+}
+
+// The sums of v over the lanes that differ in the bits O, O / 2, ..., LEAST: each step halves what
+// a lane holds, so that it ends with the sums of its elements from `at` on alone (N - 1 moves
+// and one for each step that is left then, where a sum element by element takes N moves a step).
+template <int N, int O, int LEAST>
 __device__ __forceinline__ void scatter_sums(float (&v)[N], int lane, int& at) {
-  if constexpr (O < 64) {
+  if constexpr (O >= LEAST) {
     if constexpr (N > 1) {
       constexpr int H = N / 2;
       const bool up = lane & O;
       float h[H];
 #pragma unroll
       for (int i = 0; i < H; ++i) {
-        const float keep = up ? v[i + H] : v[i], send = up ? v[i] : v[i + H];
-        h[i] = keep + __shfl_xor(send, O, 64);
+        if constexpr (O >= 16) {
+          // swaps the half (row) of the one with the other half (row) of the other
+          u32x2 r;
+          if constexpr (O == 32) {
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + H]), false, false);
+            r = u32x2{x[0], x[1]};
+          } else {
+            const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + H]), false, false);
+            r = u32x2{x[0], x[1]};
+          }
+          h[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        } else {
+          const float keep = up ? v[i + H] : v[i], send = up ? v[i] : v[i + H];
+          h[i] = keep + from_xor<O>(send);
+        }
       }
       at += up ? H : 0;
-      scatter_sums<H, 2 * O>(h, lane, at);
+      scatter_sums<H, O / 2, LEAST>(h, lane, at);
 #pragma unroll
       for (int i = 0; i < H; ++i) v[i] = h[i];
     } else {
-      v[0] += __shfl_xor(v[0], O, 64);
-      scatter_sums<1, 2 * O>(v, lane, at);
+      v[0] += from_xor<O>(v[0]);
+      scatter_sums<1, O / 2, LEAST>(v, lane, at);
     }
   }
 }
 // How many elements a lane ends with
-constexpr int scattered(int n, int o) {
-  while (o < 64 && n > 1) {
-    n /= 2;
-    o *= 2;
-  }
+constexpr int scattered(int n, int least) {
+  for (int o = 32; o >= least && n > 1; o /= 2) n /= 2;
   return n;
 }
 // The workgroup's sums of share v, one row of D for each wave
@@ -368,9 +418,34 @@ template <int D, int E>
 __device__ __forceinline__ void wave_sums(float (&acc)[E], int lane, float* row) {
   constexpr int kLanesPerRow = D / E;
   int at = lane % kLanesPerRow * E;
-  scatter_sums<E, kLanesPerRow>(acc, lane, at);
+  scatter_sums<E, 32, kLanesPerRow>(acc, lane, at);
 #pragma unroll
   for (int i = 0; i < scattered(E, kLanesPerRow); ++i) row[at + i] = acc[i];   // lanes with the same `at` hold the same sums
+}
+
+// Maximum and sum of 2^(a - maximum) of affinities, joined in any order of parts.  A NaN among
+// them, which no maximum shows, makes the sum NaN.
+struct RowStats {
+  float m = -INFINITY, l = 0.f;
+  bool bad = false;
+  __device__ __forceinline__ void add(float a) {
+    bad |= a != a;
+    const float mn = fmaxf(m, a);
+    if (mn > -INFINITY) {
+      l = l * fast_exp2(m - mn) + fast_exp2(a - mn);
+      m = mn;
+    }
+  }
+  __device__ __forceinline__ float2 of_lane() const { return make_float2(m, bad ? NAN : l); }
+};
+// The same from a part a lane, in every lane (a part without a maximum, of no affinities or of NaN
+// alone, adds its sum as it is)
+__device__ __forceinline__ float2 join_stats(float2 p) {
+  const float m = wave_max_dpp(p.x);
+  return make_float2(m, wave_sum_dpp(p.x > -INFINITY ? p.y * fast_exp2(p.x - m) : p.y));
+}
+__device__ __forceinline__ float2 part_of_lane(const float2* p, int n, int lane) {
+  return lane < n ? p[lane] : make_float2(-INFINITY, 0.f);
 }
 
 // The new token's rows into position `pos`: 32 lanes of the first wave each for K and V
@@ -406,7 +481,7 @@ template <int D>
 __device__ __forceinline__ void fp4_one_slice(const Fp4DecodeArgs& A, int64_t slice, int live, float qscale, float* s) {
   constexpr int EV = 16, N = Fp4Row<D>::kBlocks;
   __shared__ QueryShared<D> qs;
-  __shared__ float sm[kOneWaves], ss[kOneWaves];
+  __shared__ float2 part[kOneWaves];
   __shared__ float red[kOneWaves][D + 1];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int64_t row0 = slice * A.capacity;
@@ -436,7 +511,7 @@ __device__ __forceinline__ void fp4_one_slice(const Fp4DecodeArgs& A, int64_t sl
   }
   split_query<D>(qx, qs);
   __syncthreads();
-  float m = -INFINITY;
+  RowStats stats;
   {
     const QueryTiles<D> q(qs, lane);
     for (int g = wave; 64 * g < live; g += KeyGroups<D>::U * kOneWaves) {
@@ -445,27 +520,17 @@ __device__ __forceinline__ void fp4_one_slice(const Fp4DecodeArgs& A, int64_t sl
         if (j >= live) return;
         const float a = qscale * x;
         s[j * N] = a;
-        m = fmaxf(m, a);
+        stats.add(a);
       });
     }
   }
   CodeStream<D, EV, kOneWaves> v(code_rows<D>(A.v_cache, row0), wave, lane, live);
   v.load();                                             // in flight over the reductions
-  const float wm = wave_max(m);
-  if (lane == 0) sm[wave] = wm;
+  const float2 ws = join_stats(stats.of_lane());
+  if (lane == 0) part[wave] = ws;
   __syncthreads();
-  float M = sm[0];
-#pragma unroll
-  for (int w = 1; w < kOneWaves; ++w) M = fmaxf(M, sm[w]);
-  float l = 0.f;
-  for (int j = t; j < live; j += kOneThreads) l += fast_exp2(s[j * N] - M);
-  l = wave_sum(l);
-  if (lane == 0) ss[wave] = l;
-  __syncthreads();
-  float tot = 0.f;
-#pragma unroll
-  for (int w = 0; w < kOneWaves; ++w) tot += ss[w];
-  const float lse = M + __log2f(tot);
+  const float2 all = join_stats(part_of_lane(part, kOneWaves, lane));
+  const float lse = all.x + __log2f(all.y);
   float ssum = 0.f;
   auto take = [&](int j, float cm, typename ScaleWord<N>::type scale) {
     const float p = fast_exp2(s[j * N] - lse);
@@ -478,7 +543,7 @@ __device__ __forceinline__ void fp4_one_slice(const Fp4DecodeArgs& A, int64_t sl
   for (int u = 0; u < kAhead; ++u)
     if (t + u * kOneThreads < live) take(t + u * kOneThreads, c0[u], v0[u]);
   for (int j = t + kAhead * kOneThreads; j < live; j += kOneThreads) take(j, __builtin_nontemporal_load(crow + j), vs[j]);
-  ssum = wave_sum(ssum);
+  ssum = wave_sum_dpp(ssum);
   if (lane == 0) red[wave][D] = ssum;
   __syncthreads();
   const int vb = lane % (D / EV) * EV / Fp4Row<D>::kBlock;
@@ -534,34 +599,23 @@ __global__ __launch_bounds__(kQThreads) void fp4_stats(Fp4DecodeArgs A, float* _
   __syncthreads();
   const QueryTiles<D> q(qs, lane);
   float* arow = aff + slice * A.length + j0;
-  float m = -INFINITY, l = 0.f;
-  bool bad = false;
+  RowStats stats;
   for (int g = wave; 64 * g < count; g += KeyGroups<D>::U * kQWaves) {
     if (g != wave) keys.load(kc, ks, count, g, kQWaves, lane);
     keys.each(q, count, g, kQWaves, lane, [&](int j, float x) {
       if (j >= count) return;
       const float a = qscale * x;
       arow[j] = a;
-      bad |= a != a;
-      const float mn = fmaxf(m, a);
-      if (mn > -INFINITY) {
-        l = l * fast_exp2(m - mn) + fast_exp2(a - mn);
-        m = mn;
-      }
+      stats.add(a);
     });
   }
-  const float wm = wave_max(m);
-  float ws = wave_sum(bad ? NAN : m == -INFINITY ? 0.f : l * fast_exp2(m - wm));
-  __shared__ float sm[kQWaves], ss[kQWaves];
-  if (lane == 0) { sm[wave] = wm; ss[wave] = ws; }
+  __shared__ float2 waves[kQWaves];
+  const float2 ws = join_stats(stats.of_lane());
+  if (lane == 0) waves[wave] = ws;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    float bm = -INFINITY, bs = 0.f;
-    for (int w = 0; w < kQWaves; ++w) bm = fmaxf(bm, sm[w]);
-    // a wave of NaN alone has no maximum, and its sum makes the slice's NaN
-    for (int w = 0; w < kQWaves; ++w) bs += sm[w] > -INFINITY ? ss[w] * fast_exp2(sm[w] - bm) : ss[w];
-    part[slice * nchunk + c] = make_float2(bm, bs);
-  }
+  if (wave != 0) return;
+  const float2 all = join_stats(part_of_lane(waves, kQWaves, lane));
+  if (lane == 0) part[slice * nchunk + c] = all;
 }
 
 template <int D>
@@ -607,9 +661,8 @@ __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const fl
     l = (m > -INFINITY ? l * fast_exp2(m - mn) : l) + (ps.x > -INFINITY ? ps.y * fast_exp2(ps.x - mn) : ps.y);
     m = mn;
   }
-  const float gm = wave_max(m);
-  const float gs = wave_sum(m > -INFINITY ? l * fast_exp2(m - gm) : l);
-  const float lse = gm + __log2f(gs);
+  const float2 all = join_stats(make_float2(m, l));
+  const float lse = all.x + __log2f(all.y);
 
   __shared__ float s[kQMaxChunk * N];
   __shared__ float red[kQWaves][D + 1];
@@ -624,7 +677,7 @@ __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const fl
     scaled_shares<N>(s + j * N, sh, sv[u]);
     ssum += sh;
   }
-  ssum = wave_sum(ssum);
+  ssum = wave_sum_dpp(ssum);
   if (lane == 0) red[wave][D] = ssum;
   __syncthreads();
   const int vb = lane % (D / E) * E / Fp4Row<D>::kBlock;
