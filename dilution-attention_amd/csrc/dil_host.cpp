@@ -558,6 +558,11 @@ Fp4Shape check_fp4(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor&
     if (reinterpret_cast<uintptr_t>(x->data_ptr()) % 8 != 0) throw py::value_error("scales must be 8-byte aligned");
   return s;
 }
+// What writes both caches needs two of them
+void check_apart(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc, const at::Tensor& vs) {
+  if (kc.numel() > 0 && (kc.data_ptr() == vc.data_ptr() || ks.data_ptr() == vs.data_ptr()))
+    throw py::value_error("k_cache and v_cache must be two caches: rows are written to both");
+}
 dil_fp4_cache fp4_ref(const at::Tensor& codes, const at::Tensor& scales) { return {codes.data_ptr(), scales.data_ptr()}; }
 const int64_t* device_number(const Maybe& x, const at::Tensor& like, const char* name) {
   if (!x) return nullptr;
@@ -579,6 +584,7 @@ void fp4_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc, c
                           ") outside cache capacity " + std::to_string(s.capacity));
   check_device({&kc, &ks, &vc, &vs, &k, &v});
   const int64_t* at = device_number(start_dev, kc, "start");
+  check_apart(kc, ks, vc, vs);
   need_library();
   if (k.numel() == 0) return;
   c10::DeviceGuard guard(k.device());
@@ -640,7 +646,10 @@ at::Tensor decode_step_fp4(const at::Tensor& q1, const at::Tensor& kc, const at:
   if (length < 1 || length > s.capacity)
     throw py::value_error("length " + std::to_string(length) + " outside cache capacity " + std::to_string(s.capacity));
   check_device({&kc, &ks, &vc, &vs, &q1, &committed});
-  if (k1) check_device({&kc, &*k1, &*v1});
+  if (k1) {
+    check_device({&kc, &*k1, &*v1});
+    check_apart(kc, ks, vc, vs);
+  }
   const int64_t* live = device_number(length_dev, kc, "length");
   need_library();
   c10::DeviceGuard guard(kc.device());

@@ -25,6 +25,7 @@ and ignored: tiles are fixed for gfx950.
 from __future__ import annotations
 
 import math
+import operator
 from typing import NamedTuple
 
 import torch
@@ -574,9 +575,10 @@ class Fp4Rows(NamedTuple):
     An element is 4 bits (the even one of a pair in the low half of its byte): a sign
     over one of 0, 0.5, 1, 1.5, 2, 3, 4, 6, times the power of two 2^(s - 127) of its block
     of min(32, D) elements.  The power is the smallest at which no element of the block
-    rounds beyond 6, within 2^-125 and 2^125 (past which elements count as 6): an element is off by at most half a
-    step, 1/6 of the block's largest.  s = 255: the block held a NaN or an infinity
-    and is NaN throughout; s = 0: rows that were never written, all 0."""
+    rounds beyond 6, within 2^-125 and 2^125 (past which elements count as 6): an element
+    is off by at most half a step, and half a step is at most 1/5 of the block's largest
+    element.  s = 255: the block held a NaN or an infinity and is NaN throughout; s = 0:
+    rows that were never written, all 0."""
 
     codes: torch.Tensor
     scales: torch.Tensor
@@ -599,8 +601,8 @@ def alloc_fp4_rows(batch: int, heads: int, capacity: int, head_dim: int, device=
 
 
 def _host_or_device(x) -> tuple:
-    """(None, x) for a host number, (x, 0) for a device tensor."""
-    return (x, 0) if torch.is_tensor(x) and x.is_cuda else (None, int(x))
+    """(None, x) for a host number (a whole one), (x, 0) for a device tensor."""
+    return (x, 0) if torch.is_tensor(x) and x.is_cuda else (None, operator.index(x))
 
 
 def dilution_fp4_write(k: torch.Tensor, v: torch.Tensor, k_cache: Fp4Rows, v_cache: Fp4Rows, start) -> None:
@@ -633,7 +635,7 @@ def dilution_decode_step_fp4(q1: torch.Tensor, k_cache: Fp4Rows, v_cache: Fp4Row
     q1.dtype): the new token's rows, which the call quantises into position
     length - 1 first, as ``dilution_fp4_write`` would; without them that position is
     written already.  A slice's bits may differ in calls of another B * H or length."""
-    return _native().decode_step_fp4(q1, *k_cache, *v_cache, committed, None, int(length), k1, v1, None, None,
+    return _native().decode_step_fp4(q1, *k_cache, *v_cache, committed, None, operator.index(length), k1, v1, None, None,
                                      _raw_stream(k_cache.codes))
 
 
@@ -649,7 +651,8 @@ def decode_step_fp4_device_length(q1: torch.Tensor, k_cache: Fp4Rows, v_cache: F
     Results equal ``dilution_decode_step_fp4`` at the live length, bitwise."""
     if not torch.is_tensor(length):
         raise ValueError("length must be one int64 element on the caches' device")
-    return _native().decode_step_fp4(q1, *k_cache, *v_cache, committed, length, int(max_length), k1, v1, out, workspace,
+    return _native().decode_step_fp4(q1, *k_cache, *v_cache, committed, length, operator.index(max_length), k1, v1, out,
+                                     workspace,
                                      _raw_stream(k_cache.codes))
 
 

@@ -44,8 +44,13 @@ def test_write_refusals():
         write(k, k[:, :, :3], kc, vc, 0)
     with pytest.raises(ValueError, match="float"):
         write(k.int(), k.int(), kc, vc, 0)
+    for start in (1.0, 2.5, "3", None, [4]):
+        with pytest.raises(TypeError):
+            write(k, k, kc, vc, start)
     with pytest.raises(RuntimeError, match="no CPU path"):
         write(k, k, kc, vc, 0)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        write(k, k, kc, vc, torch.tensor(3))
 
 
 def _bad_caches():
@@ -117,6 +122,9 @@ def test_step_refusals():
         step(q, kc, vc, com, 5, q, q[..., :32])
     with pytest.raises(ValueError, match="dtype"):
         step(q, kc, vc, com, 5, q, q.float())
+    for length in (5.0, "5", None):
+        with pytest.raises(TypeError):
+            step(q, kc, vc, com, length)
     with pytest.raises(RuntimeError, match="no CPU path"):
         step(q, kc, vc, com, 5, q, q)
     with pytest.raises(ValueError, match="length"):

@@ -294,6 +294,72 @@ def test_what_is_no_number(length):
     assert kernels.dilution_decode_step_fp4(q, kc, vc, before.clone(), length)[0, 0].isnan().all()
 
 
+@pytest.mark.parametrize("d", WIDTHS)
+@pytest.mark.parametrize("n", [1, 40, 143, 144, 256, 257, 300, 512])
+def test_both_forms_at_their_border(n, d):
+    """The longest contexts that one workgroup takes whole (no workspace), and one key more: float64, and
+    a device-resident length on either side of the border."""
+    from dilution import _hip
+
+    query = _hip.lib().dil_decode_fp4_workspace_bytes
+    short, long = 1, 40000
+    assert query(n, short, d) == 0 and query(n, long, d) > 0
+    while long - short > 1:
+        mid = (short + long) // 2
+        short, long = (mid, long) if query(n, mid, d) == 0 else (short, mid)
+    kc, vc = _caches(n, 1, long, d, seed=n)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    q = torch.randn(n, 1, 1, d, generator=g, device="cuda").bfloat16() / 2
+    com = torch.rand(n, 1, long, generator=g, device="cuda")
+    at = sorted({0, n // 2, n - 1})
+    pick = lambda c: kernels.Fp4Rows(c.codes[at], c.scales[at])                                # noqa: E731
+    for length in (short, long):
+        mine, dev = com.clone(), com.clone()
+        out = kernels.dilution_decode_step_fp4(q, kc, vc, mine, length)
+        _check(q[at], pick(kc), pick(vc), com[at], out[at], mine[at], length)
+        got = kernels.decode_step_fp4_device_length(q, kc, vc, dev, torch.tensor([length], device="cuda"), long)
+        assert torch.equal(got, out) and torch.equal(dev, mine)
+
+
+def test_queries_with_small_and_large_elements():
+    """Elements over the whole range of their type beside one another, down to subnormal ones: every
+    query element counts to fp32's precision of its block's largest."""
+    for dtype, spread in ((torch.bfloat16, 12.0), (torch.float16, 5.0), (torch.float32, 12.0)):
+        for d in WIDTHS:
+            q, kc, vc, com = _state(2, 2, 900, 0, d, torch.float32, seed=d)
+            g = torch.Generator(device="cuda").manual_seed(d + 1)
+            q = (q * torch.exp2(-spread * torch.rand(q.shape, generator=g, device="cuda") ** 0.5)).to(dtype)
+            q[0, 0, 0, 1::2] *= torch.finfo(dtype).tiny
+            q[0, 1] = 0
+            before = com.clone()
+            out = kernels.dilution_decode_step_fp4(q, kc, vc, com, 900)
+            _check(q, kc, vc, before, out, com, 900)
+
+
+def test_a_query_that_is_no_number():
+    """A NaN or an infinity in a query makes its slice's row NaN and no other's."""
+    for length in (300, 9000):
+        q, kc, vc, com = _state(2, 2, length, 0, 64, torch.bfloat16, seed=8)
+        want = kernels.dilution_decode_step_fp4(q, kc, vc, com.clone(), length)
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            x, c = q.clone(), com.clone()
+            x[0, 1, 0, 40] = bad
+            out = kernels.dilution_decode_step_fp4(x, kc, vc, c, length)
+            assert out[0, 1].isnan().all() and c[0, 1].isnan().all()
+            for i, j in ((0, 0), (1, 0), (1, 1)):
+                assert torch.equal(out[i, j], want[i, j])
+
+
+def test_one_cache_for_both_is_refused():
+    q, kc, vc, com = _state(1, 2, 30, 0, 64, torch.bfloat16, seed=2)
+    for pair in ((kc, kc), (kc, kernels.Fp4Rows(vc.codes, kc.scales)), (kernels.Fp4Rows(vc.codes, kc.scales), vc)):
+        with pytest.raises(ValueError, match="two caches"):
+            kernels.dilution_fp4_write(q, q, *pair, 3)
+        with pytest.raises(ValueError, match="two caches"):
+            kernels.dilution_decode_step_fp4(q, *pair, com, 30, q, q)
+    kernels.dilution_decode_step_fp4(q, kc, kc, com, 30)    # reading one for both writes nothing
+
+
 @pytest.mark.parametrize("b,h,top,d", [(1, 2, 300, 64), (2, 3, 9000, 64), (170, 1, 9000, 32), (1, 1, 9000, 256), (3, 1, 5000, 16)])
 @pytest.mark.parametrize("new", [False, True])
 def test_a_device_length_gives_the_same_bits(b, h, top, d, new):
