@@ -1,7 +1,8 @@
 // The decode step over caches in 4 bits (dil_decode_step_fp4; the format is in dil_fp4.hpp):
 // dil_decode_step's mathematics on the values that codes and scales stand for,
 //
-//   a_j = log2(e) q.k_j / sqrt(D),  p_j = 2^(a_j - lse),  share_j = p_j / (committed_j + p_j + eps)
+//   a_j = log2(e) q.k_j / sqrt(D),  p_j = 2^(a_j - m) / sum 2^(a - m),  m = max a
+//   share_j = p_j / (committed_j + p_j + eps)
 //   committed_j += p_j,  out = sum share_j v_j / (sum share_j + eps)
 //
 // in the same launches: fp4_one where one workgroup does a slice's whole step, else fp4_stats
@@ -530,10 +531,10 @@ __device__ __forceinline__ void fp4_one_slice(const Fp4DecodeArgs& A, int64_t sl
   if (lane == 0) part[wave] = ws;
   __syncthreads();
   const float2 all = join_stats(part_of_lane(part, kOneWaves, lane));
-  const float lse = all.x + __log2f(all.y);
+  const float inv = 1.f / all.y;
   float ssum = 0.f;
   auto take = [&](int j, float cm, typename ScaleWord<N>::type scale) {
-    const float p = fast_exp2(s[j * N] - lse);
+    const float p = fast_exp2(s[j * N] - all.x) * inv;
     const float sh = p * fast_rcp(cm + p + kEps);
     __builtin_nontemporal_store(cm + p, crow + j);
     scaled_shares<N>(s + j * N, sh, scale);
@@ -662,7 +663,7 @@ __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const fl
     m = mn;
   }
   const float2 all = join_stats(make_float2(m, l));
-  const float lse = all.x + __log2f(all.y);
+  const float inv = 1.f / all.y;
 
   __shared__ float s[kQMaxChunk * N];
   __shared__ float red[kQWaves][D + 1];
@@ -671,7 +672,7 @@ __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const fl
   for (int u = 0; u < kOwn; ++u) {
     const int j = threadIdx.x + u * kQThreads;
     if (j >= count) break;
-    const float p = fast_exp2(av[u] - lse);
+    const float p = fast_exp2(av[u] - all.x) * inv;
     const float sh = p * fast_rcp(cv[u] + p + kEps);
     __builtin_nontemporal_store(cv[u] + p, crow + j);
     scaled_shares<N>(s + j * N, sh, sv[u]);
