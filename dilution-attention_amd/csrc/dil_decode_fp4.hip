@@ -28,9 +28,9 @@ namespace {
 // One workgroup per slice takes 1024 threads; the chunked step workgroups of 256 over chunks of
 // at most 1024 keys, eight to a CU, so that some load while others reduce, and a rule as the
 // decode step's (decode_chunk): as many chunks as fill whole rounds of what the GPU holds at
-// once.  us per step (bf16, head_dim 64: 128 slices of 16384 keys; 16 and 256 of 131072), each with
-// its best unroll: 1024 threads and 2048 keys 45, 45, 531; 512 and 2048 40, 41, 489; 256 and 1024
-// 40, 42, 491; 128 and 512 41, 46, 512; 256 and 512 43, 50, 540.  256 x 1024 leads in the other widths.
+// once.  us per step (bf16, head_dim 64: 128 slices of 16384 keys; 16 and 256 of 131072): 256 threads
+// and 1024 keys 37, 38, 440; 512 and 2048 36, 37, 441 (at head_dim 32, 128 slices of 65536 keys, 77
+// against 75); 128 and 512 37, 41, 450; 256 and 512 39, 46, 493; 256 and 2048 36, 39, 454.
 constexpr int kOneThreads = 1024;
 constexpr int kOneWaves = kOneThreads / 64;
 constexpr int kQThreads = 256;
@@ -71,10 +71,9 @@ template <int D, int E, int W> struct QLayout {
   static constexpr int kRowsPerBlock = kRowsPerWave * W;
   static constexpr int kWords = E / 8;
 };
-// K: a block of elements a lane.  V: half of one, which leaves the registers (one sum an
-// element) for eight workgroups of a CU; at head_dim 256 the LDS admits four, and whole blocks
-// are quicker (64 slices of 32768 keys 131 -> 119 us; at 64 the other way, 496 -> 490).
-template <int D> constexpr int kVElems = D == 256 ? 32 : 16;
+// Elements of a V row that a lane takes: half a block, whose sums (one an element) leave the
+// registers for eight workgroups of a CU (whole blocks, in the order above: 39, 42, 478 us).
+constexpr int kVElems = 16;
 
 template <int W> struct CodeWords {
   uint32_t w[W];
@@ -85,11 +84,10 @@ __device__ __forceinline__ CodeWords<W> load_codes(const uint8_t* p) {
   if constexpr (W == 4) {
     const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
     r.w[0] = x[0]; r.w[1] = x[1]; r.w[2] = x[2]; r.w[3] = x[3];
-  } else if constexpr (W == 2) {
+  } else {
+    static_assert(W == 2, "8 or 16 bytes");
     const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
     r.w[0] = x[0]; r.w[1] = x[1];
-  } else {
-    r.w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
   }
   return r;
 }
@@ -183,7 +181,7 @@ template <int D> struct KeyTiles {
 };
 
 constexpr int kParts = 8;
-template <int D> struct QueryShared {
+template <int D> struct alignas(16) QueryShared {
   uint8_t part[kParts][D];
   int exponent[Fp4Row<D>::kBlocks];
 };
@@ -289,8 +287,8 @@ template <int D> struct QueryTiles {
 // f(key, score) once a lane and group.
 template <int D> struct KeyGroups {
   using T = KeyTiles<D>;
-  // groups in flight: 4 loads of codes a lane.  8 are no quicker, and their registers leave one
-  // workgroup of 1024 threads a CU instead of two (600 slices of 4000 keys 47 us, 40 with 4).
+  // groups in flight: 4 loads of codes a lane.  The registers of 8 would leave one workgroup of
+  // 1024 threads a CU instead of two, or spill (600 slices of 4000 keys 56 us, 40 with 4).
   static constexpr int U = T::kMma >= 4 ? 1 : 4 / T::kMma;
   CodeWords<T::kWords> c[U][T::kMma];
   uint32_t s[U][T::kMma];
@@ -480,7 +478,7 @@ __device__ __forceinline__ const typename ScaleWord<Fp4Row<D>::kBlocks>::type* s
 // A slice's whole step in one workgroup; s: floats of LDS, one for each key and block.
 template <int D>
 __device__ __forceinline__ void fp4_one_slice(const Fp4DecodeArgs& A, int64_t slice, int live, float qscale, float* s) {
-  constexpr int EV = 16, N = Fp4Row<D>::kBlocks;
+  constexpr int EV = kVElems, N = Fp4Row<D>::kBlocks;
   __shared__ QueryShared<D> qs;
   __shared__ float2 part[kOneWaves];
   __shared__ float red[kOneWaves][D + 1];
@@ -623,7 +621,7 @@ template <int D>
 __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const float* __restrict__ aff,
                                                        const float2* __restrict__ part, float* __restrict__ part_out,
                                                        int64_t chunk, int nchunk, int64_t slice0, int64_t one_max) {
-  constexpr int E = kVElems<D>, N = Fp4Row<D>::kBlocks;
+  constexpr int E = kVElems, N = Fp4Row<D>::kBlocks;
   const int64_t live = live_length(A.dlen, A.length);
   if (live <= one_max) return;                            // fp4_finish does the whole step
   const int64_t slice = slice0 + blockIdx.y;
@@ -639,7 +637,7 @@ __global__ __launch_bounds__(kQThreads) void fp4_apply(Fp4DecodeArgs A, const fl
   const auto* vs = scale_rows<D>(A.v_cache, row0);
   // what comes first is loaded first (loads complete in issue order): the chunks' statistics, then
   // this thread's keys, then V rows.  The demand goes past the caches,
-  // both ways, and leaves them to the affinities: 256 slices of 131072 keys 487 -> 445 us.
+  // both ways, and leaves them to the affinities: 256 slices of 131072 keys 489 -> 440 us.
   const float2* prow = part + slice * nchunk;
   const float2 first = prow[min(lane, nlive - 1)];
   constexpr int kOwn = static_cast<int>(kQMaxChunk / kQThreads);
@@ -743,19 +741,19 @@ __global__ __launch_bounds__(ONE ? kOneThreads : 512, ONE && D <= 128 ? 8 : 4) v
 }
 
 // The most keys of a slice that one workgroup takes whole; above, the chunked step, whose three
-// launches take 10 us at least and whose many workgroups catch up where few slices leave CUs idle.
+// launches take 9.5 us at least and whose many workgroups catch up where few slices leave CUs idle.
 // us per step, one workgroup -> chunked (bf16 queries):
-//   64:  1 slice 2000 keys 8.5 -> 10.3, 4000 12.6 -> 10.9; 16 slices 2000 9.4 -> 11.3, 4000 13.3 -> 11.6;
-//        64 slices 4000 13.7 -> 15.7, 8000 22.9 -> 19.8; 128 slices 8100 24.6 -> 26.9, 12000 33 -> 32;
-//        160 slices 8100 26 -> 29, 16000 44 -> 46; 256 slices 2000 12 -> 20, 16000 58 -> 69;
-//        264 slices 8100 42.8 -> 42.7, 10000 60 -> 48; 300 slices 8100 43 -> 45; 400 slices 8100 48 -> 57,
-//        12000 74 -> 75; 600 slices 8100 71 -> 78, 12000 110 -> 104; 1024 slices 16000 207 -> 234
-//   128: 16 slices 1000 9.0 -> 12.3, 2000 12.3 -> 12.6; 64 slices 2000 12.7 -> 14.7, 4000 21 -> 18;
-//        128 slices 4000 22 -> 24, 6000 30 -> 31; 256 slices 8000 52 -> 62; 264 slices 4000 39 -> 39,
-//        6000 64 -> 52; 400 slices 4000 46 -> 50
-//   256: 16 slices 500 11 -> 14, 1000 17 -> 14; 128 slices 1000 18 -> 19, 2000 30 -> 25; 256 slices 4000
-//        56 -> 66; 264 slices 2000 52 -> 43; 400 slices 500 23 -> 24; 512 slices 2000 60 -> 66
-//   16:  16 slices 4000 8.3 -> 10.9, 8000 12.4 -> 12.2; 128 slices 16000 23.5 -> 23, 32000 41 -> 35
+//   64:  1 slice 2000 keys 8.1 -> 9.6, 4000 12.2 -> 9.7; 16 slices 2000 9.0 -> 10.4, 4000 12.9 -> 10.8;
+//        64 slices 4000 13.4 -> 14.6, 8000 22 -> 19; 128 slices 8100 24 -> 26, 12000 33 -> 32;
+//        160 slices 8100 26 -> 29, 16000 44 -> 45; 256 slices 2000 12 -> 19, 16000 56 -> 69;
+//        264 slices 8100 44 -> 42, 10000 59 -> 47; 300 slices 8100 44 -> 44; 400 slices 8100 49 -> 57,
+//        12000 74 -> 76; 600 slices 8100 73 -> 79, 12000 108 -> 104; 1024 slices 16000 206 -> 235
+//   128: 16 slices 1000 8.3 -> 11.7, 2000 11.7 -> 12.0; 64 slices 2000 12.0 -> 13.9, 4000 20 -> 17;
+//        128 slices 4000 22 -> 24, 6000 30 -> 30; 256 slices 8000 51 -> 61; 264 slices 4000 39 -> 39,
+//        6000 63 -> 52; 400 slices 4000 43 -> 49
+//   256: 16 slices 500 10 -> 13, 1000 15 -> 13; 128 slices 1000 16 -> 17, 2000 25 -> 24; 256 slices 4000
+//        54 -> 65; 264 slices 2000 50 -> 42; 400 slices 500 21 -> 23; 512 slices 2000 57 -> 65
+//   16:  16 slices 4000 7.8 -> 9.9, 8000 11.9 -> 10.9; 128 slices 16000 22 -> 22, 32000 40 -> 34
 template <int D>
 int64_t fp4_one_max(int64_t n) {
   constexpr int64_t kKeyBytes = D + 2 * Fp4Row<D>::kBlocks + 8;

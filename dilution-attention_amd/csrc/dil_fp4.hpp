@@ -10,8 +10,8 @@
 // infinite; a block past 6 * 2^125 saturates), is 255 for a block that holds a NaN or an
 // infinity, all NaN then, and 0 in a row that was never written, all 0.
 //
-// gfx950 converts two codes an instruction, exactly (v_cvt_scalef32_pk_f32_fp4 and _bf16_fp4 to
-// and v_cvt_scalef32_pk_fp4_f32 from them, nearest, ties to even).
+// gfx950 converts two codes an instruction, exactly (v_cvt_scalef32_pk_f32_fp4, and
+// v_cvt_scalef32_pk_fp4_f32 back, nearest, ties to even).
 #pragma once
 
 #include "dil_common.hpp"

@@ -353,6 +353,7 @@ class DilutionLM(nn.Module):
         batch = token.shape[0]
         if fused and self.fused_decode_eligible(batch):
             new = self._new_row_buffers(caches)
+            packed = [new is not None and dcache.is_packed(c) for c in caches]
 
             def slot(i):
                 cache = caches[i]
@@ -360,11 +361,11 @@ class DilutionLM(nn.Module):
                 if t >= cache["k"].shape[2]:
                     raise ValueError("decode step past the cache capacity (context_length)")
                 dcache.moved_on(cache, t + 1)
-                return self._new_rows(cache, new, t)
+                return (*new, 0) if packed[i] else (cache["k"], cache["v"], t)
 
             def attend(i, q1):
                 c = caches[i]
-                if dcache.is_packed(c):
+                if packed[i]:
                     return kernels.dilution_decode_step_fp4(q1, c["k"], c["v"], c["committed"], c["len"], *new)
                 return kernels.dilution_decode_step(q1, c["k"], c["v"], c["committed"], c["len"])
 
@@ -448,11 +449,6 @@ class DilutionLM(nn.Module):
         batch, heads, _, head_dim = packed[0].shape
         return [torch.empty(batch, heads, 1, head_dim, device=packed[0].device, dtype=self.lm_head.weight.dtype)
                 for _ in range(2)]
-
-    @staticmethod
-    def _new_rows(cache: dict, new: list | None, pos):
-        """The buffers and position that ``rows_linear_qkv`` writes a layer's new k and v to."""
-        return (*new, 0) if dcache.is_packed(cache) else (cache["k"], cache["v"], pos)
 
     @staticmethod
     def _norm_eps(norm: nn.Module) -> float:
@@ -698,7 +694,8 @@ class GraphDecoder:
                                                      self.capacity, k1, v1, out=self.outs[i], workspace=self.ws)
 
     def _slot(self, i: int):
-        return self.model._new_rows(self.caches[i], self.new, self.pos)
+        cache = self.caches[i]
+        return (*self.new, 0) if self.packed else (cache["k"], cache["v"], self.pos)
 
     def _attend_q(self, i: int, q1) -> torch.Tensor:
         cache = self.caches[i]

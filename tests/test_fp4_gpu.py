@@ -336,6 +336,27 @@ def test_queries_with_small_and_large_elements():
             _check(q, kc, vc, before, out, com, 900)
 
 
+@pytest.mark.parametrize("d", WIDTHS)
+@pytest.mark.parametrize("value", [1.9375, 1.0, 1.99999988079071044921875, 0.03125 + 2.0 ** -20])
+def test_the_largest_sums_of_a_block(d, value):
+    """Every product of a block as large as can be and of one sign, but one of the smallest code: the
+    small one counts (its loss would be 500 times the bound).  Small block powers keep the bids apart."""
+    length, b, h = 300, 1, 2
+    g = torch.Generator().manual_seed(d)
+    sign = torch.randint(0, 2, (d,), generator=g)
+    q = (value * (1 - 2 * sign.float())).expand(b, h, 1, d).contiguous().cuda()
+    code = (7 + 8 * sign).expand(b, h, length, d).clone()   # 6 times the query's sign
+    at = torch.randint(0, d, (b, h, length, 1), generator=g)
+    code.scatter_(3, at, 1 + 8 * torch.randint(0, 2, at.shape, generator=g))       # 0.5, either sign
+    kc = kernels.Fp4Rows((code[..., 0::2] | (code[..., 1::2] << 4)).to(torch.uint8).cuda(),
+                         torch.full((b, h, length, d // min(32, d)), 127 - 9, dtype=torch.uint8, device="cuda"))
+    _, _, vc, com = _state(b, h, length, 0, d, torch.float32, seed=1)
+    com[:] = 0.5 / length
+    before = com.clone()
+    out = kernels.dilution_decode_step_fp4(q, kc, vc, com, length)
+    _check(q, kc, vc, before, out, com, length)
+
+
 def test_a_query_that_is_no_number():
     """A NaN or an infinity in a query makes its slice's row NaN and no other's."""
     for length in (300, 9000):
