@@ -558,9 +558,13 @@ Fp4Shape check_fp4(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor&
     if (reinterpret_cast<uintptr_t>(x->data_ptr()) % 8 != 0) throw py::value_error("scales must be 8-byte aligned");
   return s;
 }
-// What writes both caches needs two of them
+// What writes both caches needs two of them, no byte of which is another's too
 void check_apart(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc, const at::Tensor& vs) {
-  if (kc.numel() > 0 && (kc.data_ptr() == vc.data_ptr() || ks.data_ptr() == vs.data_ptr()))
+  auto overlap = [](const at::Tensor& a, const at::Tensor& b) {
+    const auto x = reinterpret_cast<uintptr_t>(a.data_ptr()), y = reinterpret_cast<uintptr_t>(b.data_ptr());
+    return x < y + b.nbytes() && y < x + a.nbytes();
+  };
+  if (overlap(kc, vc) || overlap(ks, vs) || overlap(kc, ks) || overlap(kc, vs) || overlap(vc, ks) || overlap(vc, vs))
     throw py::value_error("k_cache and v_cache must be two caches: rows are written to both");
 }
 dil_fp4_cache fp4_ref(const at::Tensor& codes, const at::Tensor& scales) { return {codes.data_ptr(), scales.data_ptr()}; }

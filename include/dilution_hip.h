@@ -439,6 +439,7 @@ int dil_evict(const void* k_cache, const void* v_cache, const float* committed, 
  * an element takes the nearest code, at most 6, and the one of even mantissa of two as near.
  * s = 255: the block held a NaN or an infinity and stands for NaN throughout (its codes are
  * 0); s = 0: a row of a cleared cache, all 0.  codes are 16-byte, scales 8-byte aligned.
+ * Where a call writes rows, the two caches' buffers do not overlap.
  *
  * dil_fp4_write quantises `rows` rows per slice of k and v (dil_rows of `dtype`) into the
  * positions from `start` on, or from the int64_t that start_dev points to on the device; rows

@@ -381,6 +381,31 @@ def test_one_cache_for_both_is_refused():
     kernels.dilution_decode_step_fp4(q, kc, kc, com, 30)    # reading one for both writes nothing
 
 
+def test_caches_that_share_bytes_are_refused():
+    b, h, cap, d = 1, 2, 32, 64
+    rows = b * h * cap
+    q = torch.randn(b, h, 1, d, device="cuda")
+    buf = torch.zeros(4 * rows * d // 2, dtype=torch.uint8, device="cuda")
+    codes = lambda at: buf[at : at + rows * d // 2].view(b, h, cap, d // 2)
+    scales = lambda at: buf[at : at + rows * d // 32].view(b, h, cap, d // 32)
+    com = torch.zeros(b, h, cap, device="cuda")
+    size, end = rows * d // 2, rows * d // 32
+    F = kernels.Fp4Rows
+    for kc, vc in ((F(codes(0), scales(2 * size)), F(codes(size - 16), scales(3 * size))),          # codes and codes
+                   (F(codes(0), scales(2 * size)), F(codes(size), scales(2 * size + end - 8))),      # scales and scales
+                   (F(codes(0), scales(size - 8)), F(codes(2 * size), scales(3 * size))),            # one cache's own two
+                   (F(codes(0), scales(3 * size - 8)), F(codes(2 * size), scales(3 * size)))):       # scales and the other's codes
+        with pytest.raises(ValueError, match="two caches"):
+            kernels.dilution_fp4_write(q, q, kc, vc, 3)
+        with pytest.raises(ValueError, match="two caches"):
+            kernels.dilution_decode_step_fp4(q, kc, vc, com, 20, q, q)
+    assert not buf.any() and not com.any()
+    # parts of one buffer that only touch are two caches
+    kc, vc = F(codes(0), scales(2 * size)), F(codes(size), scales(2 * size + end))
+    kernels.dilution_fp4_write(q, q, kc, vc, 3)
+    assert torch.equal(kc.codes, vc.codes) and torch.equal(kc.scales, vc.scales) and kc.codes.any()
+
+
 @pytest.mark.parametrize("b,h,top,d", [(1, 2, 300, 64), (2, 3, 9000, 64), (170, 1, 9000, 32), (1, 1, 9000, 256), (3, 1, 5000, 16)])
 @pytest.mark.parametrize("new", [False, True])
 def test_a_device_length_gives_the_same_bits(b, h, top, d, new):
