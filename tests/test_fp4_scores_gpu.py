@@ -1,0 +1,52 @@
+"""The 4-bit decode step's bids and outputs on the GPU against float64, within the bound of its own arithmetic
+(tests/fp4_scores.py, which test_fp4_scores.py shows to fail for planted mistakes)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import fp4_reference as ref
+import fp4_scores as fs
+from dilution import kernels
+from gpu_helpers import needs_gpu
+
+pytestmark = [pytest.mark.gpu, needs_gpu]
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+WIDTHS = [16, 32, 64, 128, 256]
+
+
+def _step(heads, dtype):
+    """One step over heads of (q, codes, scales), no demand before: bids and outputs of each."""
+    length, d = heads[0][1].shape[0], heads[0][0].shape[0]
+    n = len(heads)
+    g = torch.Generator().manual_seed(length + d)
+    kc = kernels.Fp4Rows(*(torch.stack([x[i] for x in heads])[None].cuda() for i in (1, 2)))
+    vc = kernels.Fp4Rows(*(x.cuda() for x in ref.quantise(torch.randn(1, n, length, d, generator=g))))
+    com = torch.zeros(1, n, length, device="cuda")
+    q = torch.stack([x[0] for x in heads])[None, :, None].to(dtype)
+    out = kernels.dilution_decode_step_fp4(q.cuda(), kc, vc, com, length).cpu()
+    kv, vv = ref.values(kc.codes.cpu(), kc.scales.cpu()), ref.values(vc.codes.cpu(), vc.scales.cpu())
+    for i in range(n):
+        p, rel = fs.bids(q[0, i, 0], kv[0, i])
+        assert fs.worst(com[0, i], p, rel) <= 1
+        want, _, spread, _ = ref.step_f64(q[0, i, 0], kv[0, i], vv[0, i], torch.zeros(length), length)
+        bound = ref.out_bound(want, spread, dtype, rel.max().item(), length)
+        assert ((out[0, i, 0].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("d", WIDTHS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("length", [400, 9000])
+@pytest.mark.parametrize("spread", fs.SPREADS)
+def test_every_part_of_a_query_counts(d, dtype, length, spread):
+    """Queries whose blocks hold elements 2^spread below their largest, which meets zeros only; one
+    workgroup for a slice, and chunks."""
+    _step([fs.inputs(d, length, spread, seed, dtype) for seed in (d + spread, length)], dtype)
+
+
+@pytest.mark.parametrize("d", WIDTHS)
+@pytest.mark.parametrize("value", [1.9375, 1.0, 1.99999988079071044921875, 0.03125 + 2.0 ** -20])
+def test_one_small_product_among_the_largest(d, value):
+    _step([fs.largest_sums(d, 300, value, seed) for seed in (d, d + 1)], torch.float32)
