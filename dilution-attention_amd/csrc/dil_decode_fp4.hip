@@ -154,6 +154,11 @@ struct CodeStream {
 // element in the small ones).  The 16 rows of A hold parts 0 to 3 four times over; the second
 // four parts are a product of their own into the same sums.
 //
+// The last part's unit is 2^(E - 38), and a scale is 2^-127 or more: a block below 2^-80 is taken 2^t up to
+// it, exactly, and its keys' scales t down, so that elements down to the subnormal ones count in full against
+// keys of powers up to 2^125.  A scale that would fall below 2^-127 is held there (t is 47 at most: its key
+// is below 2^-78, its products with that block below 2^-158, nothing beside a bid's rounding).
+//
 // A lane's 16 bytes of codes are one block of one key; the 4 blocks of K = 128 (lane group
 // kb = lane / 16 holds block kb of B and both operands' scales of it) are rows of 4, 2 or 1 keys.
 // fp8 operands lie otherwise: lane group g holds elements 16 (g % 2) to 16 (g % 2) + 15 of blocks
@@ -184,7 +189,9 @@ constexpr int kParts = 8;
 template <int D> struct alignas(16) QueryShared {
   uint8_t part[kParts][D];
   int exponent[Fp4Row<D>::kBlocks];
+  int up[Fp4Row<D>::kBlocks];                             // the t of a block
 };
+constexpr int kLeastExponent = -80;
 
 __device__ __forceinline__ int part_exponent(int e, int i) { return e - 3 - 5 * i; }
 
@@ -210,10 +217,16 @@ __device__ __forceinline__ void split_query(float x, QueryShared<D>& sh) {
   with(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0x141, 0xF, 0xF, true));     // row_half_mirror
   with(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0x140, 0xF, 0xF, true));     // row_mirror
   if constexpr (Fp4Row<D>::kBlock == 32) with(__shfl_xor(static_cast<int>(top), 16, 64));
-  // within what fp32 scales by exactly; a query with a NaN or an infinity becomes NaN
-  const int e = min(max(static_cast<int>(top >> 23) - 127, -80), 127);
-  if (t % Fp4Row<D>::kBlock == 0) sh.exponent[t / Fp4Row<D>::kBlock] = e;
+  // a query with a NaN or an infinity becomes NaN
   const bool bad = top >= 0x7f800000u;
+  int e = min(static_cast<int>(top >> 23) - 127, 127);
+  const int up = top != 0u ? max(kLeastExponent - e, 0) : 0;
+  e = max(e, kLeastExponent);
+  x *= __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+  if (t % Fp4Row<D>::kBlock == 0) {
+    sh.exponent[t / Fp4Row<D>::kBlock] = e;
+    sh.up[t / Fp4Row<D>::kBlock] = up;
+  }
 #pragma unroll
   for (int i = 0; i < kParts; ++i) {
     const int unit = part_exponent(e, i);
@@ -232,11 +245,16 @@ template <int D> struct QueryTiles {
   int lane;
   intx8 a[kHeld ? kParts / 4 : 1];
   int scale[kParts / 4][T::kHalves];
+  bool any_up = false;                                    // the same in all lanes
   __device__ __forceinline__ QueryTiles(const QueryShared<D>& s, int l) : sh(s), lane(l) {
 #pragma unroll
     for (int p = 0; p < kParts / 4; ++p) {
 #pragma unroll
-      for (int h = 0; h < T::kHalves; ++h) scale[p][h] = 127 + part_exponent(sh.exponent[T::block(h, lane >> 4)], (lane & 3) + 4 * p);
+      for (int h = 0; h < T::kHalves; ++h) {
+        const int b = T::block(h, lane >> 4), up = sh.up[b];
+        scale[p][h] = (127 + part_exponent(sh.exponent[b], (lane & 3) + 4 * p)) | up << 8;      // the unit takes the low byte
+        any_up |= __ballot(up != 0) != 0;
+      }
       if constexpr (kHeld) a[p] = read(p, 0);
     }
   }
@@ -255,6 +273,14 @@ template <int D> struct QueryTiles {
   __device__ __forceinline__ intx8 operand(int p, int h) const {
     if constexpr (kHeld) return a[p];
     else return read(p, h);
+  }
+  // The keys' scales on queries with blocks that were taken up (NaN blocks stay such)
+  __device__ __forceinline__ void lower(uint32_t (&s)[T::kMma]) const {
+#pragma unroll
+    for (int m = 0; m < T::kMma; ++m) {
+      const int x = static_cast<int>(s[m]) - (scale[0][m % T::kHalves] >> 8);
+      s[m] = s[m] == 255u ? 255u : static_cast<uint32_t>(max(x, 0));
+    }
   }
   // The score of key `lane` of the 64 whose codes and scales these are
   __device__ __forceinline__ float score(const CodeWords<T::kWords> (&c)[T::kMma], const uint32_t (&s)[T::kMma]) const {
@@ -309,7 +335,9 @@ template <int D> struct KeyGroups {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = 64 * (group + u * step);
-      if (j < count) f(j + lane, q.score(c[u], s[u]));
+      if (j >= count) break;
+      if (q.any_up) q.lower(s[u]);
+      f(j + lane, q.score(c[u], s[u]));
     }
   }
 };

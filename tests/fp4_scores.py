@@ -112,6 +112,22 @@ def inputs(d: int, length: int, spread: int, seed: int, dtype=torch.float32, rea
     return q, codes, scales + math.floor(math.log2(reach / total.max().item()))
 
 
+def small_query(d: int, length: int, top: int, seed: int, dtype=torch.float32, beside: bool = False, reach: float = 40.0):
+    """`inputs` with a query of elements near 2^top (top < 0) and keys of powers as large as 2^125, and one key in
+    seven of powers down to 2^-125.  beside: the row's first block is of ordinary size, on keys of ordinary size."""
+    q, codes, scales = inputs(d, length, 0, seed, reach=reach / 2)
+    n, block = blocks(d)
+    power = min(-top, 125 + 127 - int(scales.max()))
+    small = torch.ldexp(q, torch.tensor(top)).to(dtype)
+    shifted = scales + power
+    if beside:
+        small[:block] = q[:block].to(dtype)
+        shifted[:, 0] = scales[:, 0]
+    at = torch.arange(0, length, 7)
+    shifted[at] = torch.randint(2, 60, (len(at), n), generator=torch.Generator().manual_seed(seed)).to(torch.uint8)
+    return small, codes, shifted
+
+
 def largest_sums(d: int, length: int, value: float, seed: int, reach: float = 40.0):
     """Every product of a block as large as can be and of one sign, but, in two keys of three, one of the smallest
     code: a third of the keys each with none, a positive and a negative one."""

@@ -50,3 +50,30 @@ def test_every_part_of_a_query_counts(d, dtype, length, spread):
 @pytest.mark.parametrize("value", [1.9375, 1.0, 1.99999988079071044921875, 0.03125 + 2.0 ** -20])
 def test_one_small_product_among_the_largest(d, value):
     _step([fs.largest_sums(d, 300, value, seed) for seed in (d, d + 1)], torch.float32)
+
+
+@pytest.mark.parametrize("d", WIDTHS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("length", [400, 9000])
+def test_small_queries_on_large_keys(d, dtype, length):
+    """Queries down to subnormal elements, whose products with keys of powers up to 2^125 are of ordinary size."""
+    _step([fs.small_query(d, length, top, d - top, dtype) for top in (-70, -85, -100, -106, -112, -119, -126, -135)], dtype)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("length", [400, 9000])
+def test_small_blocks_beside_ordinary_ones(d, length):
+    _step([fs.small_query(d, length, top, d - top, beside=True) for top in (-85, -106, -119, -126, -135)], torch.float32)
+
+
+@pytest.mark.parametrize("d", WIDTHS)
+def test_a_block_that_is_no_number_meets_a_small_query(d):
+    for length in (400, 9000):
+        q, codes, scales = (x.cuda() for x in fs.small_query(d, length, -110, d))
+        kc = kernels.Fp4Rows(codes[None, None].repeat(1, 2, 1, 1), scales[None, None].repeat(1, 2, 1, 1))
+        kc.scales[0, 1, length // 2, -1] = 255
+        vc = kernels.Fp4Rows(kc.codes.clone(), torch.full_like(kc.scales, 127))
+        com = torch.zeros(1, 2, length, device="cuda")
+        out = kernels.dilution_decode_step_fp4(q.expand(1, 2, 1, d), kc, vc, com, length)
+        assert out[0, 0].isfinite().all() and com[0, 0].isfinite().all()
+        assert out[0, 1].isnan().all() and com[0, 1].isnan().all()
