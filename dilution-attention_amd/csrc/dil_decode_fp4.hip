@@ -157,7 +157,9 @@ struct CodeStream {
 // The last part's unit is 2^(E - 38), and a scale is 2^-127 or more: a block below 2^-80 is taken 2^t up to
 // it, exactly, and its keys' scales t down, so that elements down to the subnormal ones count in full against
 // keys of powers up to 2^125.  A scale that would fall below 2^-127 is held there (t is 47 at most: its key
-// is below 2^-78, its products with that block below 2^-158, nothing beside a bid's rounding).
+// is below 2^-78, its products with that block below 2^-158, nothing beside a bid's rounding).  A
+// first part can be 2^(E + 1), past the element itself: A's scales are half of the parts' and the factor
+// of the affinities twice itself, so that the sums of a score below 2^128 stay finite.
 //
 // A lane's 16 bytes of codes are one block of one key; the 4 blocks of K = 128 (lane group
 // kb = lane / 16 holds block kb of B and both operands' scales of it) are rows of 4, 2 or 1 keys.
@@ -252,7 +254,7 @@ template <int D> struct QueryTiles {
 #pragma unroll
       for (int h = 0; h < T::kHalves; ++h) {
         const int b = T::block(h, lane >> 4), up = sh.up[b];
-        scale[p][h] = (127 + part_exponent(sh.exponent[b], (lane & 3) + 4 * p)) | up << 8;      // the unit takes the low byte
+        scale[p][h] = (126 + part_exponent(sh.exponent[b], (lane & 3) + 4 * p)) | up << 8;      // the unit takes the low byte
         any_up |= __ballot(up != 0) != 0;
       }
       if constexpr (kHeld) a[p] = read(p, 0);
@@ -282,7 +284,7 @@ template <int D> struct QueryTiles {
       s[m] = s[m] == 255u ? 255u : static_cast<uint32_t>(max(x, 0));
     }
   }
-  // The score of key `lane` of the 64 whose codes and scales these are
+  // Half the score of key `lane` of the 64 whose codes and scales these are
   __device__ __forceinline__ float score(const CodeWords<T::kWords> (&c)[T::kMma], const uint32_t (&s)[T::kMma]) const {
     constexpr int kOuts = 4 / T::kSets;                   // 16-key groups with sums of their own
     float out = 0.f;
@@ -310,7 +312,7 @@ template <int D> struct QueryTiles {
 };
 
 // A wave's groups of 64 keys: `group`, group + step, ... (keys past the end are read as the last one);
-// f(key, score) once a lane and group.
+// f(key, half its score) once a lane and group.
 template <int D> struct KeyGroups {
   using T = KeyTiles<D>;
   // groups in flight: 4 loads of codes a lane.  The registers of 8 would leave one workgroup of
@@ -811,7 +813,7 @@ template <int D>
 int launch_fp4(const Fp4DecodeArgs& a) {
   const int64_t chunk = fp4_chunk(a.n, a.length);
   const int nchunk = static_cast<int>(fp4_chunks(a.n, a.length, a.dlen != nullptr));
-  const float qscale = kLog2e / sqrtf(static_cast<float>(D));
+  const float qscale = 2.f * kLog2e / sqrtf(static_cast<float>(D));      // of half a score
   hipStream_t st = static_cast<hipStream_t>(a.stream);
   const int64_t keys = fp4_one_max<D>(a.n);
   const auto lds_of = [](int64_t k) { return sizeof(float) * static_cast<size_t>((k + 63) / 64 * 64 * Fp4Row<D>::kBlocks); };

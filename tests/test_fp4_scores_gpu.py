@@ -77,3 +77,33 @@ def test_a_block_that_is_no_number_meets_a_small_query(d):
         out = kernels.dilution_decode_step_fp4(q.expand(1, 2, 1, d), kc, vc, com, length)
         assert out[0, 0].isfinite().all() and com[0, 0].isfinite().all()
         assert out[0, 1].isnan().all() and com[0, 1].isnan().all()
+
+
+@pytest.mark.parametrize("d", WIDTHS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("length", [400, 9000])
+def test_scores_at_the_end_of_fp32(d, dtype, length):
+    """The type's largest value against a key of 1: the score is finite, its key takes the whole bid.  A row of
+    equal scores as large divides it evenly."""
+    q = torch.zeros(1, 2, 1, d, dtype=dtype)
+    q[..., -1] = torch.finfo(dtype).max
+    codes = torch.zeros(1, 2, length, d // 2, dtype=torch.uint8)
+    codes[0, 0, :, -1] = 0x10                               # 0.5 in the last element
+    codes[0, 0, 7, -1] = 0x20                               # 1
+    codes[0, 1, :, -1] = 0x20
+    kc = kernels.Fp4Rows(codes.cuda(), torch.full((1, 2, length, fs.blocks(d)[0]), 127, dtype=torch.uint8, device="cuda"))
+    vc = kernels.Fp4Rows(*(x.cuda() for x in ref.quantise(torch.randn(1, 2, length, d, generator=torch.Generator().manual_seed(d)))))
+    com = torch.zeros(1, 2, length, device="cuda")
+    out = kernels.dilution_decode_step_fp4(q.cuda(), kc, vc, com, length).double().cpu()
+    v = ref.values(*(x.cpu() for x in vc))[0]
+    want = torch.zeros(length)
+    want[7] = 1.0
+    assert torch.equal(com[0, 0].cpu(), want)
+    # shares of p / (p + eps), and their sum plus eps
+    u = torch.finfo(dtype).eps / 2
+    assert ((out[0, 0, 0] - v[0, 7] / (1 + 2e-9)).abs() <= (u + 2.0 ** -20) * v[0, 7].abs()).all()
+    # even bids: every power is 1 and their sums are whole, so that only the division rounds (by a step at most)
+    assert (com[0, 1].double().cpu() * length - 1).abs().max() <= 2 * fs.U
+    # the mean: sums of length / 64 additions in a lane, 24 across lanes and waves
+    mean = v[1].mean(0)
+    assert ((out[0, 1, 0] - mean).abs() <= u * mean.abs() + 2.0 ** -14 * v[1].abs().mean(0)).all()
