@@ -645,7 +645,7 @@ int dil_decode_step_fp4(const void* q1, const void* k1, const void* v1, const di
   if (n < 1 || n >= (int64_t{1} << 31) || length < 1 || length > capacity || capacity >= (int64_t{1} << 31))
     return dil::kErrShape;
   const int64_t need = dil::decode_fp4_workspace_bytes(n, length, head_dim);
-  if (!all_set(q1, static_cast<const void*>(committed), static_cast<const void*>(out)) || (need > 0 && workspace == nullptr) ||
+  if (!all_set(q1, static_cast<const void*>(committed), static_cast<const void*>(out)) || (need > 0 && (workspace == nullptr || !aligned16(workspace))) ||
       (k1 == nullptr) != (v1 == nullptr) || !aligned16(q1, k1, v1) || !valid_fp4(k_cache) || !valid_fp4(v_cache))
     return dil::kErrShape;
   if (workspace_bytes < need) return dil::kErrWorkspace;

@@ -678,6 +678,8 @@ at::Tensor decode_step_fp4(const at::Tensor& q1, const at::Tensor& kc, const at:
                   scratch->device() != kc.device()))
     throw py::value_error("workspace must be a contiguous uint8 tensor of at least " + std::to_string(need) +
                           " bytes on the caches' device");
+  if (scratch && need > 0 && reinterpret_cast<uintptr_t>(scratch->data_ptr()) % 16 != 0)
+    throw py::value_error("workspace must be 16-byte aligned");
   if (n > 0) {
     const Maybe ws = scratch ? scratch : need > 0 ? Maybe(workspace(need, kc)) : Maybe();
     launch("dil_decode_step_fp4", [&]() -> int {

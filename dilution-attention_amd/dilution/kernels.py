@@ -647,8 +647,8 @@ def decode_step_fp4_device_length(q1: torch.Tensor, k_cache: Fp4Rows, v_cache: F
     ``decode_step_device_length``: one int64 element on the caches' device, read when the
     kernels run and clamped to [0, max_length], so that one captured HIP graph serves
     every decode step.  ``out`` ((B, H, D) in q1's dtype) and ``workspace``
-    (``decode_fp4_workspace(...)``) may be given so that the call allocates nothing.
-    Results equal ``dilution_decode_step_fp4`` at the live length, bitwise."""
+    (``decode_fp4_workspace(...)``; a buffer of the caller's own must be 16-byte aligned) may be given
+    so that the call allocates nothing.  Results equal ``dilution_decode_step_fp4`` at the live length, bitwise."""
     if not torch.is_tensor(length):
         raise ValueError("length must be one int64 element on the caches' device")
     return _native().decode_step_fp4(q1, *k_cache, *v_cache, committed, length, operator.index(max_length), k1, v1, out,

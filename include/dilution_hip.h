@@ -466,7 +466,8 @@ int dil_fp4_read(const dil_fp4_cache* k_cache, const dil_fp4_cache* v_cache, int
  * length is read from device memory when the kernels run (clamped to [0, length]; with 0
  * nothing is read or written but out, which becomes 0), and `length` sizes grid and workspace.
  * q1, k1 and v1 are 16-byte aligned.  The workspace query serves both forms; where it returns 0
- * (short contexts, which one launch does; no slices or keys) workspace may be NULL.
+ * (short contexts, which one launch does; no slices or keys) workspace may be NULL, elsewhere one that is
+ * not 16-byte aligned is refused.
  */
 int64_t dil_decode_fp4_workspace_bytes(int64_t n, int64_t length, int head_dim);
 int dil_decode_step_fp4(const void* q1, const void* k1, const void* v1, const dil_fp4_cache* k_cache,

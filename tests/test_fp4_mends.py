@@ -1,0 +1,21 @@
+"""Calls on 4-bit caches that are refused before they write, and calls beside them that are taken, on the CPU."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from dilution import _hip
+
+
+@pytest.mark.parametrize("off", [1, 2, 4, 8, 12])
+def test_a_workspace_off_its_alignment_is_refused(off):
+    lib = _hip.lib()
+    c = _hip.Fp4Cache(4096, 8192)
+    need = lib.dil_decode_fp4_workspace_bytes(6, 40000, 64)
+    assert need > 0
+    at = ctypes.c_void_p
+    # refused before any launch: the addresses are never used
+    assert lib.dil_decode_step_fp4(at(4096), None, None, ctypes.byref(c), ctypes.byref(c), at(8192), at(12288), 6, 40000, 40000,
+                                   None, 64, 1, at(16384 + off), need, None) == -4
