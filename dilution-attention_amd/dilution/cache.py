@@ -121,6 +121,8 @@ def append_kv(cache: dict, k1: torch.Tensor, v1: torch.Tensor) -> int:
     if t >= cache["k"].shape[2]:
         raise ValueError("decode step past the cache capacity (context_length)")
     if is_packed(cache):
+        if k1.dim() != 4 or k1.shape[2] != 1:
+            raise ValueError(f"one new position is appended, k1 and v1 of (B, H, 1, D), got {tuple(k1.shape)}")
         kernels.dilution_fp4_write(k1, v1, cache["k"], cache["v"], t)
     else:
         cache["k"][:, :, t] = k1[:, :, 0]

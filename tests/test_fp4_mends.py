@@ -5,8 +5,9 @@ from __future__ import annotations
 import ctypes
 
 import pytest
+import torch
 
-from dilution import _hip
+from dilution import _hip, cache, kernels
 
 
 @pytest.mark.parametrize("off", [1, 2, 4, 8, 12])
@@ -19,3 +20,14 @@ def test_a_workspace_off_its_alignment_is_refused(off):
     # refused before any launch: the addresses are never used
     assert lib.dil_decode_step_fp4(at(4096), None, None, ctypes.byref(c), ctypes.byref(c), at(8192), at(12288), 6, 40000, 40000,
                                    None, 64, 1, at(16384 + off), need, None) == -4
+
+
+@pytest.mark.parametrize("rows", [0, 2, 3])
+def test_one_position_is_appended(rows):
+    """Not two, of which the second would lie behind the new length, and not none."""
+    k, v = (kernels.alloc_fp4_rows(1, 2, 8, 64, device="cpu") for _ in range(2))
+    c = {"k": k, "v": v, "len": 5, "committed": torch.zeros(1, 2, 8)}
+    x = torch.ones(1, 2, rows, 64)
+    with pytest.raises(ValueError, match="one new position"):
+        cache.append_kv(c, x, x)
+    assert c["len"] == 5 and not k.codes.any()

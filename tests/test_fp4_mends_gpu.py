@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import fp4_reference as ref
-from dilution import kernels
+from dilution import cache, kernels
 from gpu_helpers import needs_gpu
 
 pytestmark = [pytest.mark.gpu, needs_gpu]
@@ -35,3 +35,18 @@ def test_a_workspace_off_its_alignment_is_refused():
     # where one launch does the step no workspace is used
     short = torch.tensor([300], device="cuda")
     kernels.decode_step_fp4_device_length(q, kc, vc, com, short, 300, workspace=buf[1:])
+
+
+def test_one_position_is_appended():
+    q, kc, vc, com = _state(1, 2, 8, 64, 2)
+    c = {"k": kc, "v": vc, "len": 5, "committed": com}
+    before = [x.clone() for x in (*kc, *vc)]
+    for rows in (0, 2, 3):
+        x = torch.ones(1, 2, rows, 64, device="cuda")
+        with pytest.raises(ValueError, match="one new position"):
+            cache.append_kv(c, x, x)
+    assert c["len"] == 5 and all(torch.equal(x, y) for x, y in zip((*kc, *vc), before))
+    assert cache.append_kv(c, q, -q) == 6 == c["len"]
+    k, v = kernels.dilution_fp4_read(kc, vc, 5, 1, torch.float32)
+    want = ref.values(*ref.quantise(q)).float()
+    assert torch.equal(k.cpu(), want) and torch.equal(v.cpu(), -want)
