@@ -264,6 +264,11 @@ class SwiGLUMLP(nn.Module):
         return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
 
 
+def _given(**kw) -> dict:
+    """The arguments that are not None: modules of a caller's own need not know the others."""
+    return {name: x for name, x in kw.items() if x is not None}
+
+
 _ATTENTION_CLASSES = {"dilution": DilutionAttention, "softmax": SoftmaxAttention}
 
 
@@ -280,7 +285,7 @@ class Block(nn.Module):
         return x + self.mlp(self.ln_2(x))
 
     def begin_cache(self, x: torch.Tensor, capacity: int | None = None, bits: int | None = None):
-        y, cache = self.attn.begin_cache(self.ln_1(x), capacity, bits)
+        y, cache = self.attn.begin_cache(self.ln_1(x), capacity, **_given(bits=bits))
         x = x + y
         return x + self.mlp(self.ln_2(x)), cache
 
@@ -341,7 +346,7 @@ class DilutionLM(nn.Module):
         x = self.wte(idx)
         caches = []
         for block in self.h:
-            x, cache = block.begin_cache(x, capacity, cache_bits)
+            x, cache = block.begin_cache(x, capacity, **_given(bits=cache_bits))
             caches.append(cache)
         return self.lm_head(self.ln_f(x[:, [-1], :])), caches
 
@@ -509,7 +514,7 @@ class DilutionLM(nn.Module):
                 raise ValueError("a graph-replayed generation keeps its caches: eviction needs graph=False")
             self._need_production("eviction")
             capacity = min(capacity, max(idx.shape[1], eviction.limit))
-        logits, caches = self.prefill(idx, capacity=capacity, cache_bits=cache_bits)
+        logits, caches = self.prefill(idx, capacity=capacity, **_given(cache_bits=cache_bits))
         tokens = idx
         if graph and max_new_tokens > 0 and not (temperature and temperature > 0.0) and self.graph_decode_eligible():
             last = logits[:, -1, :].float()

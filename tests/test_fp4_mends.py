@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from dilution import _hip, cache, kernels
+from dilution.lm import Block, DilutionLM, LMConfig, SoftmaxAttention
 
 
 @pytest.mark.parametrize("off", [1, 2, 4, 8, 12])
@@ -31,3 +32,28 @@ def test_one_position_is_appended(rows):
     with pytest.raises(ValueError, match="one new position"):
         cache.append_kv(c, x, x)
     assert c["len"] == 5 and not k.codes.any()
+
+
+def test_modules_of_a_callers_own_need_not_know_of_bits():
+    """Attention, blocks and models whose begin_cache and prefill take a capacity alone run as they did."""
+
+    class Attention(SoftmaxAttention):
+        def begin_cache(self, x, capacity=None):
+            return super().begin_cache(x, capacity)
+
+    class Layer(Block):
+        def begin_cache(self, x, capacity=None):
+            return super().begin_cache(x, capacity)
+
+    class Model(DilutionLM):
+        def prefill(self, idx, capacity=None):
+            return super().prefill(idx, capacity)
+
+    cfg = LMConfig(vocab_size=32, n_layers=2, d_model=64, n_heads=4, attention="softmax")
+    plain, model = DilutionLM(cfg), Model(cfg)
+    model.h[0] = Layer(cfg, "softmax")
+    for block in model.h:
+        block.attn = Attention(cfg)
+    model.load_state_dict(plain.state_dict())
+    idx = torch.arange(6)[None]
+    assert torch.equal(model.generate(idx, 4), plain.generate(idx, 4))
