@@ -24,7 +24,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <int D> struct Fp4Row {
   static constexpr int kBlock = D < 32 ? D : 32;      // elements of a scale
   static constexpr int kBlocks = D / kBlock;
-  static constexpr int kBytes = D / 2;                // of codes
 };
 
 // The scale bytes of a row, as one load
