@@ -28,7 +28,8 @@ namespace {
 // One workgroup per slice takes 1024 threads; the chunked step workgroups of 256 over chunks of
 // at most 1024 keys, eight to a CU, so that some load while others reduce, and a rule as the
 // decode step's (decode_chunk): as many chunks as fill whole rounds of what the GPU holds at
-// once.  us per step (bf16, head_dim 64: 128 slices of 16384 keys; 16 and 256 of 131072): 256 threads
+// once.  (At head_dim 256 a CU holds four, by fp4_stats' registers and the shares in fp4_apply's
+// LDS; the chunks are the same there.)  us per step (bf16, head_dim 64: 128 slices of 16384 keys; 16 and 256 of 131072): 256 threads
 // and 1024 keys 37, 38, 440; 512 and 2048 36, 37, 441 (at head_dim 32, 128 slices of 65536 keys, 77
 // against 75); 128 and 512 37, 41, 450; 256 and 512 39, 46, 493; 256 and 2048 36, 39, 454.
 constexpr int kOneThreads = 1024;
@@ -72,7 +73,8 @@ template <int D, int E, int W> struct QLayout {
   static constexpr int kWords = E / 8;
 };
 // Elements of a V row that a lane takes: half a block, whose sums (one an element) leave the
-// registers for eight workgroups of a CU (whole blocks, in the order above: 39, 42, 478 us).
+// registers for eight workgroups of a CU (whole blocks, in the order above: 39, 42, 478 us).  At head_dim
+// 256 both are the same: 64 slices of 32768 keys 120, 128 of 16384 116 us.
 constexpr int kVElems = 16;
 
 template <int W> struct CodeWords {
@@ -238,8 +240,9 @@ __device__ __forceinline__ void split_query(float x, QueryShared<D>& sh) {
   }
 }
 
-// A wave's A operands: in registers, but for head_dim 256, whose 32 registers would halve the
-// waves of a CU: there read from LDS at each use.
+// A wave's A operands: in registers, but for head_dim 256, whose 32 would leave fp4_stats three waves a
+// SIMD instead of four and fp4_one without enough: there read from LDS at each use (64 slices of
+// 32768 keys 120 us, held 119).
 template <int D> struct QueryTiles {
   using T = KeyTiles<D>;
   static constexpr bool kHeld = T::kHalves == 1;
@@ -783,7 +786,14 @@ __global__ __launch_bounds__(ONE ? kOneThreads : 512, ONE && D <= 128 ? 8 : 4) v
 //        6000 63 -> 52; 400 slices 4000 43 -> 49
 //   256: 16 slices 500 10 -> 13, 1000 15 -> 13; 128 slices 1000 16 -> 17, 2000 25 -> 24; 256 slices 4000
 //        54 -> 65; 264 slices 2000 50 -> 42; 400 slices 500 21 -> 23; 512 slices 2000 57 -> 65
-//   16:  16 slices 4000 7.8 -> 9.9, 8000 11.9 -> 10.9; 128 slices 16000 22 -> 22, 32000 40 -> 34
+//   32:  16 slices 4000 8.2 -> 11, 6000 11.4 -> 11.5; 128 slices 8000 15 -> 20, 16000 26 -> 27; 144 slices
+//        16000 27 -> 32, 32000 50 -> 50; 192 slices 16000 30 -> 37, 32000 55 -> 59; 256 slices 16000 35 -> 43,
+//        32000 66 -> 75; 300 slices 16000 46 -> 50; 400 slices 16000 51 -> 62, 32000 113 -> 113; 600 slices
+//        16000 80 -> 86
+//   16:  16 slices 4000 7.8 -> 9.9, 8000 11.9 -> 10.9; 128 slices 16000 22 -> 22, 32000 40 -> 34; 144 slices
+//        16000 23 -> 28, 24000 32 -> 33, 32000 42 -> 40; 192 slices 16000 24 -> 30, 32000 44 -> 46; 256 slices
+//        16000 26 -> 34, 32000 47 -> 58; 300 slices 16000 32 -> 39; 400 slices 16000 35 -> 49, 32000
+//        88 -> 87; 600 slices 16000 56 -> 66
 template <int D>
 int64_t fp4_one_max(int64_t n) {
   constexpr int64_t kKeyBytes = D + 2 * Fp4Row<D>::kBlocks + 8;

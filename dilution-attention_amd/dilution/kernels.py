@@ -576,8 +576,8 @@ class Fp4Rows(NamedTuple):
     over one of 0, 0.5, 1, 1.5, 2, 3, 4, 6, times the power of two 2^(s - 127) of its block
     of min(32, D) elements.  The power is the smallest at which no element of the block
     rounds beyond 6, within 2^-125 and 2^125 (past which elements count as 6): an element
-    is off by at most half a step, and half a step is at most 1/5 of the block's largest
-    element.  s = 255: the block held a NaN or an infinity and is NaN throughout; s = 0:
+    is off by at most half a step of its code, and, where the power is within that range, by at
+    most 1/5 of the block's largest element.  s = 255: the block held a NaN or an infinity and is NaN throughout; s = 0:
     rows that were never written, all 0."""
 
     codes: torch.Tensor

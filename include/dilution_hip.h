@@ -445,7 +445,8 @@ int dil_evict(const void* k_cache, const void* v_cache, const float* committed, 
  * positions from `start` on, or from the int64_t that start_dev points to on the device; rows
  * that this would put outside [0, capacity) are dropped.  Nothing else in the caches changes.
  * dil_fp4_read gives the values of positions [start, start + rows) as (n, rows, head_dim) of
- * `dtype` (exact but for values past the type's range; a 16-byte aligned destination).
+ * `dtype` (exact but for values past the type's range; a 16-byte aligned destination).  A call of
+ * either takes rows * head_dim below 2^34.
  */
 typedef struct dil_fp4_cache {
   void* codes;
